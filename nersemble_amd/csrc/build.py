@@ -42,7 +42,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     hipcc = _hipcc()
     os.makedirs(OBJ, exist_ok=True)
     flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-I", INCLUDE, "-I", HERE,
-             "-Wall", "-Wno-unused-function"]
+             "-Wall", "-Wno-unused-function",
+             # no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     hdrs = _headers()
     jobs = []
     objs = []
