@@ -32,7 +32,7 @@ extern "C" {
 #define NSX_MAX_SLOTS 64
 #define NSX_MAX_ADAM_SLOTS 192   /* gradient planes nsx_adam_hash_factored(_consume) reads (level-parallel runs: one per
                                    (source rank, code row), engine/level_parallel.py) */
-#define NSX_VERSION 128
+#define NSX_VERSION 129
 
 typedef uint16_t nsx_half;
 
@@ -1014,6 +1014,68 @@ int nsx_lp_backward(const nsx_lp_layout* lay, nsx_comm* comm, int emulate_rank, 
                     const uint8_t* gathered, const int64_t* sizes_host, const int32_t* rows_host, const nsx_half* tables,
                     const nsx_grid_geom* sub_geom, const float* window, float* G, float* dz_scratch, float* csum_scratch,
                     uint8_t* ret, uint8_t* ret_recv, float* nonfinite, int rows, float* dx, float* dcode, void* stream);
+
+/* ---- routed experts (csrc/expert_route.hip, expert_linear.hip, expert_combine.hip) ----------------------------------------
+ * (No reference counterpart: the reference's only mixture is the dense blend of all hash grids, hash_ensemble.py:133-156, and
+ * its per-sample networks are the single ones of nersemble_nerfacto_field.py:142-172.  These calls are the sparse mixture of
+ * such networks: every row goes to top_k of E experts.)
+ * A row (a sample, a token) has top_k entries, entry i = row * top_k + choice.  A PLAN orders the entries by expert:
+ *   offsets   [E + 1]   entries of expert e are the ordered rows [offsets[e], offsets[e + 1])
+ *   rows      [T * k]   entry of every ordered row, rising within an expert; -1 behind offsets[E]
+ *   positions [T][k]    ordered row of every entry; -1 for an entry in no segment
+ * The kernels bound every index they take from a plan: numbers of another plan give other results, never an access outside
+ * the arrays.  All arithmetic is in 32 bits and results are rounded once; no call uses floating-point atomics, so equal inputs
+ * give equal bits.  dtype: one of the three below. */
+#define NSX_DTYPE_F32 0
+#define NSX_DTYPE_F16 1
+#define NSX_DTYPE_BF16 2
+#define NSX_MAX_EXPERTS 512
+#define NSX_MAX_TOP_K 64
+#define NSX_MAX_EXPERT_WIDTH 16384
+#define NSX_MAX_EXPERT_ENTRIES 1073741824      /* rows x top_k */
+/* Choice of the experts.  logits [T] rows of E values (row_stride elements apart); scores s = softmax (sigmoid = 0) or
+ * 1 / (1 + exp(-x)) (sigmoid = 1); the choice goes by s + bias (bias [E] or NULL).  n_groups > 1: of the E / n_groups
+ * consecutive experts each, the top_groups groups with the largest sum of their group_top (1 or 2) best experts stay.  Equal
+ * values go by rising index.  weights [T][top_k] = scale * s, over the sum of the chosen s if renormalise; experts [T][top_k]
+ * in falling order of s + bias.  A logit of -inf takes its expert out of the row's choice; slots that find no expert, and rows
+ * with selector[row] = 0 (selector uint8 [T] or NULL), get expert -1 and weight 0.  A row with a NaN (softmax: or +inf) among
+ * its logits gets NaN weights.  Rows behind n_device are not written. */
+int nsx_expert_route_fwd(const void* logits, int dtype, int64_t T, int E, int64_t row_stride, const float* bias,
+                         const uint8_t* selector, int top_k, int sigmoid, int n_groups, int top_groups, int group_top,
+                         int renormalise, float scale, float* weights, int32_t* experts, const int64_t* n_device, void* stream);
+/* dlogits [T][E] (contiguous, the logits' dtype) of dweights [T][top_k], from the forward's weights and experts. */
+int nsx_expert_route_bwd(const void* logits, int dtype, int64_t T, int E, int64_t row_stride, int top_k, int sigmoid,
+                         int renormalise, float scale, const float* weights, const int32_t* experts, const float* dweights,
+                         void* dlogits, const int64_t* n_device, void* stream);
+/* The plan of experts [T][top_k]; an expert outside [0, E) is in no segment, nor are entries of rows behind n_device.
+ * workspace: nsx_expert_plan_workspace(T * top_k, E) bytes. */
+int64_t nsx_expert_plan_workspace(int64_t n_entries, int E);
+int nsx_expert_plan(const int32_t* experts, int64_t T, int top_k, int E, int32_t* offsets, int32_t* rows, int32_t* positions,
+                    void* workspace, const int64_t* n_device, void* stream);
+/* y [R][n_out]: ordered row p of expert e is act(weight[e] x[row]), weight [E][n_out][n_in], act = ReLU if relu.  rows = the
+ * plan's (row = rows[p] / top_k) or NULL (x holds the R ordered rows).  dtype: 16 bits.  Widths are multiples of 8, rows and
+ * matrices 16-byte aligned.  Ordered rows behind offsets[E] become 0. */
+int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, int top_k,
+                          const void* weight, int n_in, int n_out, int E, const int32_t* offsets, int64_t R, int relu, void* y,
+                          void* stream);
+/* dx [R][n_in] in the plan's order (nsx_expert_combine_fwd without weights brings it to the rows).  y: the forward's result if
+ * it had the ReLU (dy counts where y is not 0), else NULL. */
+int nsx_expert_linear_bwd_x(const void* dy, int dtype, int64_t dy_stride, const void* y, int64_t y_stride, const void* weight,
+                            int n_in, int n_out, int E, const int32_t* offsets, int64_t R, void* dx, void* stream);
+/* dw [E][n_out][n_in], of x's dtype or (dw_f32) in 32 bits; 0 for an expert without rows.  workspace:
+ * nsx_expert_linear_bwd_w_workspace bytes (0: none). */
+int64_t nsx_expert_linear_bwd_w_workspace(int64_t R, int E, int n_in, int n_out);
+int nsx_expert_linear_bwd_w(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, int top_k,
+                            const void* dy, int64_t dy_stride, const void* y, int64_t y_stride, int n_in, int n_out, int E,
+                            const int32_t* offsets, int64_t R, int dw_f32, void* dw, void* workspace, void* stream);
+/* out [T][n] = sum_j weights[t][j] * y[positions[t][j]] (weights NULL: 1); choices without a position count nothing.  Rows of
+ * out behind n_device are not written. */
+int nsx_expert_combine_fwd(const void* y, int dtype, int64_t y_stride, int64_t R, int n, const float* weights,
+                           const int32_t* positions, int64_t T, int top_k, void* out, const int64_t* n_device, void* stream);
+/* dy [R][n] and dweights [T][top_k] of dout [T][n] (contiguous); n_routed = &offsets[E]: rows of dy behind it become 0. */
+int nsx_expert_combine_bwd(const void* y, int dtype, int64_t y_stride, int64_t R, int n, const float* weights,
+                           const int32_t* positions, const int32_t* n_routed, int64_t T, int top_k, const void* dout, void* dy,
+                           float* dweights, const int64_t* n_device, void* stream);
 
 #ifdef __cplusplus
 }

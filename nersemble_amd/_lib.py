@@ -13,6 +13,8 @@ NSX_MAX_ADAM_SLOTS = 192
 NSX_OPT_ADAM_BLOCKS_PER_CU, NSX_OPT_MLP_BWD_HALF_BLOCKS_PER_CU, NSX_OPT_MLP_BWD0_HALF_BLOCKS_PER_CU = 0, 1, 2
 NSX_OPT_LP_ONE_LAUNCH = 3
 NSX_COMM_ID_BYTES = 128
+NSX_DTYPE_F32, NSX_DTYPE_F16, NSX_DTYPE_BF16 = 0, 1, 2
+NSX_MAX_EXPERTS, NSX_MAX_TOP_K, NSX_MAX_EXPERT_WIDTH, NSX_MAX_EXPERT_ENTRIES = 512, 64, 16384, 1 << 30
 
 c_void_p, c_int, c_int64, c_float = C.c_void_p, C.c_int, C.c_int64, C.c_float
 
@@ -90,6 +92,23 @@ SIGNATURES = {
     "nsx_mlp_bwd": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_float, c_float, c_void_p, c_int64,
                             c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_void_p, c_void_p]),
+    "nsx_expert_route_fwd": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                     c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nsx_expert_route_bwd": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nsx_expert_plan_workspace": (c_int64, [c_int64, c_int]),
+    "nsx_expert_plan": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nsx_expert_linear_fwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p,
+                                      c_int64, c_int, c_void_p, c_void_p]),
+    "nsx_expert_linear_bwd_x": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p,
+                                        c_int64, c_void_p, c_void_p]),
+    "nsx_expert_linear_bwd_w_workspace": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "nsx_expert_linear_bwd_w": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64,
+                                        c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "nsx_expert_combine_fwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                       c_void_p, c_void_p]),
+    "nsx_expert_combine_bwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nsx_f32_to_f16": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "nsx_sample_positions": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),

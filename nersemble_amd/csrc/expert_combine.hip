@@ -1,0 +1,140 @@
+// expert_combine.hip -- routed experts: the weighted join of a row's expert outputs, and its gradients.
+//
+// out_t = sum_j w_tj y_pos(t,j);  dy_pos(t,j) = w_tj dout_t;  dw_tj = <dout_t, y_pos(t,j)>.  Sums in 32 bits.
+#include "expert_common.h"
+
+namespace nsx {
+
+struct CombineArgs {
+    const void* y; int64_t y_stride;
+    const float* w;                  // NULL: every weight is 1
+    const int32_t* positions; const int32_t* offsets;
+    int64_t T; int k, R, chunks;     // chunks: 8-wide pieces of a row
+    const int64_t* n_dev;
+};
+
+__device__ __forceinline__ int64_t valid_rows(int64_t T, const int64_t* n_dev) {
+    if (!n_dev) return T;
+    const int64_t n = *n_dev;
+    return n < T ? (n < 0 ? 0 : n) : T;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __restrict__ out) {
+    typedef typename Elem<T>::x8 x8;
+    const int64_t total = valid_rows(a.T, a.n_dev) * a.chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / a.chunks;
+        const int c = (int)(i - t * a.chunks);
+        float s[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s[q] = 0.f;
+        for (int j = 0; j < a.k; ++j) {
+            const int p = a.positions[t * a.k + j];
+            if ((unsigned)p >= (unsigned)a.R) continue;
+            const float w = a.w ? a.w[t * a.k + j] : 1.f;
+            const x8 v = *reinterpret_cast<const x8*>(reinterpret_cast<const T*>(a.y) + (int64_t)p * a.y_stride + c * 8);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s[q] += w * (float)v[q];
+        }
+        x8 o;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) o[q] = (T)s[q];
+        *reinterpret_cast<x8*>(out + i * 8) = o;
+    }
+}
+
+// 2^lg lanes per row of `out`: dout is read once per choice (from the caches after the first), y once, dy written once.
+template <typename T>
+__global__ __launch_bounds__(256) void combine_bwd_kernel(CombineArgs a, const T* __restrict__ dout, T* __restrict__ dy,
+                                                          float* __restrict__ dw, int lg) {
+    typedef typename Elem<T>::x8 x8;
+    const int lanes = 1 << lg, sub = threadIdx.x & (lanes - 1);
+    const int64_t T_ = valid_rows(a.T, a.n_dev);
+    const int64_t step = ((int64_t)gridDim.x * 256) >> lg;
+    for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lg; t < T_; t += step) {
+        for (int j = 0; j < a.k; ++j) {
+            const int p = a.positions[t * a.k + j];
+            const bool there = (unsigned)p < (unsigned)a.R;
+            float dot = 0.f;
+            if (there) {
+                const float w = a.w[t * a.k + j];
+                for (int c = sub; c < a.chunks; c += lanes) {
+                    const x8 g = *reinterpret_cast<const x8*>(dout + (t * a.chunks + c) * 8);
+                    const x8 v = *reinterpret_cast<const x8*>(reinterpret_cast<const T*>(a.y) + (int64_t)p * a.y_stride + c * 8);
+                    x8 o;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) { dot += (float)g[q] * (float)v[q]; o[q] = (T)(w * (float)g[q]); }
+                    *reinterpret_cast<x8*>(dy + ((int64_t)p * a.chunks + c) * 8) = o;
+                }
+            }
+            for (int o = 1; o < lanes; o <<= 1) dot += __shfl_xor(dot, o);
+            if (sub == 0) dw[t * a.k + j] = there ? dot : 0.f;
+        }
+    }
+    // rows of dy behind the last segment
+    const int64_t first = (int64_t)min(max(*a.offsets, 0), a.R) * a.chunks, last = (int64_t)a.R * a.chunks;
+    x8 z;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) z[q] = (T)0.f;
+    for (int64_t i = first + (int64_t)blockIdx.x * 256 + threadIdx.x; i < last; i += (int64_t)gridDim.x * 256)
+        *reinterpret_cast<x8*>(dy + i * 8) = z;
+}
+
+}  // namespace nsx
+
+extern "C" {
+
+static int combine_check(const char* what, int dtype, int64_t T, int top_k, int64_t R, int n, int64_t stride, const void* y) {
+    using namespace nsx;
+    NSX_REQUIRE(dtype == NSX_DTYPE_F16 || dtype == NSX_DTYPE_BF16, "%s: dtype %d is not a 16-bit float", what, dtype);
+    NSX_REQUIRE(top_k >= 1 && top_k <= NSX_MAX_TOP_K, "%s: top_k %d not in [1,%d]", what, top_k, NSX_MAX_TOP_K);
+    NSX_REQUIRE(T >= 0 && T <= NSX_MAX_EXPERT_ENTRIES / top_k, "%s: %lld rows of %d choices are too many", what, (long long)T, top_k);
+    NSX_REQUIRE(R >= 0 && R <= NSX_MAX_EXPERT_ENTRIES, "%s: %lld ordered rows", what, (long long)R);
+    NSX_REQUIRE(n >= 8 && n % 8 == 0 && n <= NSX_MAX_EXPERT_WIDTH, "%s: width %d is not a multiple of 8 in [8,%d]", what, n, NSX_MAX_EXPERT_WIDTH);
+    NSX_REQUIRE(stride >= n && stride % 8 == 0 && aligned16(y), "%s: rows of y are not 16-byte aligned (stride %lld)", what, (long long)stride);
+    return NSX_OK;
+}
+
+int nsx_expert_combine_fwd(const void* y, int dtype, int64_t y_stride, int64_t R, int n, const float* weights,
+                           const int32_t* positions, int64_t T, int top_k, void* out, const int64_t* n_device, void* stream) {
+    using namespace nsx;
+    const int rc = combine_check("nsx_expert_combine_fwd", dtype, T, top_k, R, n, y_stride, y);
+    if (rc != NSX_OK) return rc;
+    if (T == 0) return NSX_OK;
+    NSX_REQUIRE(positions && out && (y || R == 0) && aligned16(out), "nsx_expert_combine_fwd: NULL or unaligned pointer");
+    CombineArgs a{y, y_stride, weights, positions, nullptr, T, top_k, (int)R, n / 8, n_device};
+    const int64_t items = T * (n / 8);
+    const int64_t blocks = (items + 255) / 256, most = (int64_t)num_cus() * 32;
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == NSX_DTYPE_F16) combine_fwd_kernel<half_t><<<grid, 256, 0, st>>>(a, (half_t*)out);
+    else combine_fwd_kernel<bf16_t><<<grid, 256, 0, st>>>(a, (bf16_t*)out);
+    NSX_LAUNCH_CHECK("nsx_expert_combine_fwd");
+    return NSX_OK;
+}
+
+int nsx_expert_combine_bwd(const void* y, int dtype, int64_t y_stride, int64_t R, int n, const float* weights,
+                           const int32_t* positions, const int32_t* n_routed, int64_t T, int top_k, const void* dout, void* dy,
+                           float* dweights, const int64_t* n_device, void* stream) {
+    using namespace nsx;
+    const int rc = combine_check("nsx_expert_combine_bwd", dtype, T, top_k, R, n, y_stride, y);
+    if (rc != NSX_OK) return rc;
+    if (T == 0 && R == 0) return NSX_OK;
+    NSX_REQUIRE(n_routed && (T == 0 || (weights && positions && dout && dweights && aligned16(dout))) && (R == 0 || (y && dy && aligned16(dy))),
+                "nsx_expert_combine_bwd: NULL or unaligned pointer");
+    CombineArgs a{y, y_stride, weights, positions, n_routed, T, top_k, (int)R, n / 8, n_device};
+    int lg = 0;
+    while ((1 << lg) < n / 8 && lg < 6) ++lg;
+    const int64_t blocks = ((T << lg) + 255) / 256, most = (int64_t)num_cus() * 32;
+    const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == NSX_DTYPE_F16)
+        combine_bwd_kernel<half_t><<<grid, 256, 0, st>>>(a, (const half_t*)dout, (half_t*)dy, dweights, lg);
+    else
+        combine_bwd_kernel<bf16_t><<<grid, 256, 0, st>>>(a, (const bf16_t*)dout, (bf16_t*)dy, dweights, lg);
+    NSX_LAUNCH_CHECK("nsx_expert_combine_bwd");
+    return NSX_OK;
+}
+
+}  // extern "C"

@@ -11,6 +11,7 @@ import math
 import torch
 from torch import nn
 
+from . import _lib, experts
 from . import functional as F
 
 _ACT = {"None": 0, "Sigmoid": 1}
@@ -77,6 +78,79 @@ class NetworkWithInputEncoding(Network):
         super().__init__(n_input_dims, n_output_dims, network_config, seed)
 
 
+class RoutedNetwork(nn.Module):
+    """A sparse mixture of E fully connected networks of one shape, every row evaluated by ``top_k`` of them
+    (``nersemble_amd.experts``) -- the routed counterpart of ``Network``, for widths that FullyFusedMLP does not have.
+
+    ``network_config``: ``n_neurons`` (a multiple of 8), ``n_hidden_layers`` >= 1, ``activation`` ReLU, ``output_activation``
+    None, ``otype`` CutlassMLP (tcnn's name for networks of any width).  ``routing_config``: ``n_experts``, ``top_k`` and,
+    optionally, ``scores``, ``renormalise``, ``scale``, ``n_groups``, ``top_groups``, ``group_top`` (``route_experts``) and
+    ``balance`` (off by default).
+
+    ``params``: all experts' matrices, flat fp32, layer by layer [E][n_out][n_in] without biases, inputs and outputs padded to
+    multiples of 8; ``gate`` [E, n_input_dims]: the router (logits = x gate^T in fp32); buffer ``balance`` [E], if asked for:
+    added to the scores for the choice alone and moved by ``rebalance``."""
+
+    def __init__(self, n_input_dims: int, n_output_dims: int, network_config: dict, routing_config: dict, seed: int = 1337):
+        super().__init__()
+        if network_config.get("otype", "CutlassMLP") != "CutlassMLP":
+            raise NotImplementedError("RoutedNetwork: otype CutlassMLP (networks of any width)")
+        if network_config.get("activation", "ReLU") != "ReLU" or network_config.get("output_activation", "None") != "None":
+            raise NotImplementedError("RoutedNetwork: ReLU between the layers, no output activation")
+        width, n_hidden = int(network_config.get("n_neurons", 64)), int(network_config.get("n_hidden_layers", 1))
+        if width < 8 or width % 8 or n_hidden < 1 or n_input_dims < 1 or n_output_dims < 1:
+            raise NotImplementedError("RoutedNetwork: n_neurons a multiple of 8, at least one hidden layer, input and output")
+        cfg = dict(routing_config)
+        self.n_experts, self.top_k = int(cfg.pop("n_experts")), int(cfg.pop("top_k"))
+        if not 1 <= self.top_k <= min(self.n_experts, _lib.NSX_MAX_TOP_K) or self.n_experts > _lib.NSX_MAX_EXPERTS:
+            raise NotImplementedError(f"RoutedNetwork: 1 <= top_k <= n_experts <= {_lib.NSX_MAX_EXPERTS}, top_k <= {_lib.NSX_MAX_TOP_K}")
+        unknown = set(cfg) - {"scores", "renormalise", "scale", "n_groups", "top_groups", "group_top", "balance"}
+        if unknown:
+            raise NotImplementedError(f"RoutedNetwork: routing_config has no {sorted(unknown)}")
+        balance = bool(cfg.pop("balance", False))
+        self.routing = cfg
+        self.n_input_dims, self.n_output_dims = n_input_dims, n_output_dims
+        pad = lambda n: -(-n // 8) * 8                                       # noqa: E731
+        dims = [pad(n_input_dims)] + [width] * n_hidden + [pad(n_output_dims)]
+        self.shapes = [(self.n_experts, o, i) for i, o in zip(dims, dims[1:])]
+        gen = torch.Generator().manual_seed(seed)
+        self.params = nn.Parameter(_xavier_flat([(o, i) for e, o, i in self.shapes for _ in range(e)], gen))
+        self.gate = nn.Parameter((torch.rand((self.n_experts, n_input_dims), generator=gen) * 2 - 1) / math.sqrt(n_input_dims))
+        self.register_buffer("balance", torch.zeros(self.n_experts) if balance else None)
+        self.register_buffer("load", torch.zeros(self.n_experts), persistent=False)
+
+    half_weights = Network.half_weights
+
+    def forward(self, x: torch.Tensor, selector: torch.Tensor = None) -> torch.Tensor:
+        """x [B, n_input_dims] (fp16 or fp32) -> [B, n_output_dims] fp16; ``selector`` uint8 [B]: rows with 0 are not evaluated
+        (their output is 0)."""
+        x2 = x.reshape(-1, self.n_input_dims)
+        if _lib.ndev_tensor(x2.shape[0]) is not None:
+            raise RuntimeError("RoutedNetwork: the router's product runs over whole arrays, not over a device-side row count "
+                               "(mask the rows behind it with `selector` instead)")
+        logits = x2.float() @ self.gate.t()
+        weights, chosen = experts.route_experts(logits, self.top_k, bias=self.balance, selector=selector, **self.routing)
+        plan = experts.expert_plan(chosen, self.n_experts)
+        if self.training:
+            self.load.copy_(plan.offsets[1:] - plan.offsets[:-1])
+        h = x2.to(torch.float16)
+        if self.shapes[0][2] != self.n_input_dims:
+            h = nn.functional.pad(h, (0, self.shapes[0][2] - self.n_input_dims))
+        sizes = [e * o * i for e, o, i in self.shapes]
+        layers = zip(torch.split(self.params, sizes), torch.split(self.half_weights(), sizes), self.shapes)
+        for n, (w, w16, shape) in enumerate(layers):
+            h = experts.expert_linear(h, w.view(shape), plan, gather=n == 0, relu=n < len(sizes) - 1, w16=w16.view(shape))
+        return experts.expert_combine(h, weights, plan)[:, :self.n_output_dims]
+
+    @torch.no_grad()
+    def rebalance(self, rate: float = 1e-3) -> None:
+        """One step of the balancing bias against the load of the last training forward: experts above the mean load lose
+        ``rate``, those below gain it."""
+        if self.balance is None:
+            raise RuntimeError("RoutedNetwork: routing_config has no balance")
+        self.balance += rate * torch.sign(self.load.mean() - self.load)
+
+
 class Encoding(nn.Module):
     """``tcnn.Encoding``: ``Identity`` (direction encoding with spherical_harmonics_degree = 0, the default of every
     shipped NeRSemble config, nersemble_instant_ngp.py:46), ``Frequency`` (the field's ``position_encoding``,
@@ -103,7 +177,6 @@ class Encoding(nn.Module):
         elif otype == "HashGrid":
             if n_input_dims != 3 or encoding_config.get("interpolation", "Linear") != "Linear":
                 raise NotImplementedError("native HashGrid: 3-D input, Linear interpolation")
-            from . import _lib
             self.f_enc = int(encoding_config.get("n_features_per_level", 2))
             if self.f_enc not in (2, 4, 8):
                 raise NotImplementedError("native HashGrid: n_features_per_level in {2, 4, 8}")

@@ -1,0 +1,572 @@
+"""GPU parity: the routed-experts operators (choice, plan, products, join, their gradients) against the 64-bit oracle.
+
+Tolerances.  u = 2^-24 is half a step of fp32, h half a step of the 16-bit type (fp16 2^-11, bf16 2^-8).  A sum of n products in
+32 bits is off by at most (n + 2) * 2 * u * sum |terms| whatever its order (2 u a step: the matrix instructions may cut instead
+of rounding); its one rounding to 16 bits adds h * |result|, and fp16 below 2^-14 half of its smallest step, 2^-25."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import experts as ox
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float16: (2.0 ** -11, 2.0 ** -25), torch.bfloat16: (2.0 ** -8, 2.0 ** -130)}
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def _f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _close(got, want, tol, what):
+    got = _f64(got) if isinstance(got, torch.Tensor) else got
+    off = np.abs(got - want)
+    worst = np.max(np.where(tol > 0, off / np.where(tol > 0, tol, 1), np.where(off > 0, np.inf, 0))) if off.size else 0.0
+    assert np.isfinite(got).all() and worst <= 1.0, f"{what}: {worst:.3g} of the tolerance, largest error {off.max():.3g}"
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# choice
+# ---------------------------------------------------------------------------------------------------------------------
+def _route_tol(x, w, k):
+    """Relative: x - max is off by u of its size (at most the logits' span), exp by 2 steps, sums and divisions by u a term."""
+    span = np.nanmax(np.where(np.isfinite(x), np.abs(x), 0.0), initial=0.0) * 2
+    return (span + k + 10) * 2 * U * np.abs(w) + 1e-37
+
+
+ROUTES = [
+    # E, k, scores, bias, groups, top_groups, group_top, renorm, scale
+    (1, 1, "softmax", False, 1, 1, 1, True, 1.0),
+    (2, 1, "softmax", False, 1, 1, 1, False, 1.0),
+    (3, 3, "sigmoid", False, 1, 1, 1, True, 2.5),
+    (16, 2, "softmax", False, 1, 1, 1, True, 1.0),
+    (32, 2, "softmax", True, 1, 1, 1, False, 1.0),
+    (61, 7, "sigmoid", True, 1, 1, 1, True, 1.0),
+    (64, 6, "softmax", False, 1, 1, 1, False, 16.0),
+    (256, 8, "sigmoid", True, 8, 4, 2, True, 2.5),
+    (160, 6, "softmax", False, 8, 3, 1, False, 16.0),
+    (20, 4, "sigmoid", True, 4, 2, 2, True, 1.0),
+    (24, 5, "softmax", True, 3, 2, 1, True, 1.0),
+    (50, 3, "sigmoid", False, 5, 2, 2, False, 1.0),
+    (512, 16, "softmax", True, 1, 1, 1, True, 1.0),
+    (495, 9, "sigmoid", True, 33, 5, 2, True, 1.0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("cfg", ROUTES, ids=lambda c: f"E{c[0]}k{c[1]}{c[2][:3]}{'b' if c[3] else ''}g{c[4]}")
+def test_route(cfg, dtype, cuda):
+    from nersemble_amd import experts as X
+    E, k, sc, has_bias, G, tg, gt, renorm, scale = cfg
+    for T in (1, 7, 130):
+        rng = np.random.default_rng(E * 7 + T)
+        x = torch.from_numpy((rng.standard_normal((T, E)) * 2).astype(np.float32)).to(DT[dtype])
+        bias = torch.from_numpy((rng.standard_normal(E) * 0.1).astype(np.float32)) if has_bias else None
+        xd = x.to(cuda).requires_grad_(True)
+        w, c = X.route_experts(xd, k, scores=sc, bias=None if bias is None else bias.to(cuda), n_groups=G, top_groups=tg,
+                               group_top=gt, renormalise=renorm, scale=scale)
+        assert w.dtype == torch.float32 and c.dtype == torch.int32 and w.shape == c.shape == (T, k)
+        x64 = _f64(x)
+        ww, wc = ox.route(x64, k, sc == "sigmoid", None if bias is None else _f64(bias), G, tg, gt, renorm, scale)
+        assert np.array_equal(c.cpu().numpy(), wc)
+        _close(w, ww, _route_tol(x64, ww, k), "weights")
+        g = rng.standard_normal((T, k)).astype(np.float32)
+        (d,) = torch.autograd.grad(w, [xd], torch.from_numpy(g).to(cuda))
+        want = ox.route_bwd(x64, ww, wc, g, sc == "sigmoid", renorm, scale)
+        # every term of a gradient is a weight (or score) times g: off relatively as the weights are, plus the sum's own steps
+        size = np.zeros_like(x64)
+        total = (np.abs(g) * ww).sum(1, keepdims=True)
+        for j in range(k):
+            size[np.arange(T), wc[:, j]] += ww[:, j] * (np.abs(g[:, j]) + (total[:, 0] / scale if renorm else 0.0))
+        if sc == "softmax" and not renorm:
+            size += ox.scores(x64, False) * total
+        tol = 3 * _route_tol(x64, size, k)
+        if dtype != "fp32":
+            h, tiny = HALF[DT[dtype]]
+            tol = tol + h * np.abs(want) + tiny
+        assert d.dtype == DT[dtype]
+        _close(d, want, tol, "dlogits")
+
+
+def test_route_gradient_against_differences(cuda):
+    """The gradient against central differences of the forward (16 experts whose choice does not change under the step)."""
+    from nersemble_amd import experts as X
+    rng = np.random.default_rng(0)
+    for sc, renorm in (("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)):
+        x = np.stack([rng.permutation(16) * 0.25 for _ in range(4)])            # gaps of 0.25
+        g = rng.standard_normal((4, 3))
+        xd = torch.tensor(x, dtype=torch.float32, device=cuda, requires_grad=True)
+        w, _ = X.route_experts(xd, 3, scores=sc, renormalise=renorm)
+        (d,) = torch.autograd.grad(w, [xd], torch.tensor(g, dtype=torch.float32, device=cuda))
+        step = 2.0 ** -6
+        for e in range(16):
+            hi, lo = x.copy(), x.copy()
+            hi[:, e] += step
+            lo[:, e] -= step
+            f = [(_f64(X.route_experts(torch.tensor(v, dtype=torch.float32, device=cuda), 3, scores=sc, renormalise=renorm)[0]) * g).sum(1)
+                 for v in (hi, lo)]
+            diff = (f[0] - f[1]) / (2 * step)
+            # third derivative of a softmax weight <= 1: step^2 / 6 * sum|g|; rounding of the forward: 16 u * sum|g| / step
+            tol = (step ** 2 / 6 + 32 * U / step) * np.abs(g).sum(1)
+            assert (np.abs(_f64(d)[:, e] - diff) <= tol).all()
+
+
+def test_route_rows_without_experts_and_odd_values(cuda):
+    from nersemble_amd import experts as X
+    inf, nan = float("inf"), float("nan")
+    rows = np.array([[0.5, 1.0, -1.0, 2.0], [-inf, -inf, -inf, -inf], [-inf, 3.0, -inf, -inf], [nan, 1.0, 2.0, 3.0],
+                     [inf, 1.0, 2.0, 3.0], [1.0, 1.0, 1.0, 1.0], [-200.0, -201.0, -300.0, -250.0], [0.0, -0.0, 0.0, -inf]], np.float32)
+    lowest = np.finfo(np.float32).min
+    rows = np.concatenate([rows, np.full((1, 4), lowest, np.float32)])
+    sel = np.ones(len(rows), np.uint8)
+    for sc in ("softmax", "sigmoid"):
+        for bias in (None, np.array([0.0, 0.125, 0.0, 0.0], np.float32)):
+            for renorm in (True, False):
+                for selector in (None, sel * (np.arange(len(rows)) % 3 != 0)):
+                    xd = torch.from_numpy(rows).to(cuda).requires_grad_(True)
+                    w, c = X.route_experts(xd, 2, scores=sc, renormalise=renorm, bias=None if bias is None else torch.from_numpy(bias).to(cuda),
+                                           selector=None if selector is None else torch.from_numpy(selector.astype(np.uint8)).to(cuda))
+                    ww, wc = ox.route(rows, 2, sc == "sigmoid", bias, renormalise=renorm, selector=selector)
+                    assert np.array_equal(c.cpu().numpy(), wc), (sc, renorm)
+                    got = _f64(w)
+                    assert np.array_equal(np.isnan(got), np.isnan(ww))
+                    # (a span of 100 in the sixth row; the last one's scores are equal or 0)
+                    assert np.allclose(got, ww, rtol=(800 + 12) * 2 * U, atol=1e-37, equal_nan=True)
+                    (d,) = torch.autograd.grad(w, [xd], torch.ones_like(w))
+                    d = _f64(d)
+                    fine = ~np.isnan(ww).any(1)
+                    assert np.isfinite(d[fine]).all() and (d[(wc < 0).all(1)] == 0).all()
+
+
+def test_route_equal_values_go_by_index(cuda):
+    from nersemble_amd import experts as X
+    x = torch.zeros((5, 256), device=cuda, dtype=torch.bfloat16)
+    x[1, 100:] = 1
+    for bias in (None, torch.zeros(256, device=cuda)):
+        _, c = X.route_experts(x, 8, bias=bias)
+        assert c[0].tolist() == list(range(8)) and c[1].tolist() == list(range(100, 108))
+        _, c = X.route_experts(x, 8, bias=bias, n_groups=8, top_groups=2, group_top=2)
+        # (experts 100 .. 127 are in group 3, whose two best are as good as those of the groups behind it)
+        assert c[0].tolist() == list(range(8)) and c[1].tolist() == list(range(100, 108))
+        x[2, 127:] = 1                                        # group 3 has one such expert only: 4 and 5 come before it
+        _, c = X.route_experts(x, 8, bias=bias, n_groups=8, top_groups=2, group_top=2)
+        assert c[2].tolist() == list(range(128, 136))
+
+
+@pytest.mark.parametrize("layout", ["strided", "transposed", "offset", "one_row"])
+def test_route_layouts(layout, cuda):
+    from nersemble_amd import experts as X
+    g = torch.Generator(device=cuda).manual_seed(1)
+    base = torch.randn((40, 24), generator=g, device=cuda)
+    x = {"strided": torch.randn((40, 100), generator=g, device=cuda)[:, 3:27], "transposed": torch.randn((24, 40), generator=g, device=cuda).t(),
+         "offset": torch.randn(40 * 24 + 1, generator=g, device=cuda)[1:].view(40, 24), "one_row": base[3:4].expand(1, 24)}[layout]
+    x = x.requires_grad_(True)
+    y = x.detach().contiguous().clone().requires_grad_(True)
+    wa, ca = X.route_experts(x, 3)
+    wb, cb = X.route_experts(y, 3)
+    assert torch.equal(wa, wb) and torch.equal(ca, cb)
+    go = torch.randn(wa.shape, generator=g, device=cuda)
+    assert torch.equal(torch.autograd.grad(wa, [x], go)[0], torch.autograd.grad(wb, [y], go)[0])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# plan
+# ---------------------------------------------------------------------------------------------------------------------
+def _check_plan(plan, want):
+    for got, w in zip((plan.offsets, plan.rows, plan.positions), want):
+        assert got.dtype == torch.int32 and np.array_equal(got.cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("T,k,E", [(0, 2, 4), (1, 1, 1), (1, 8, 64), (63, 1, 3), (257, 3, 512), (1000, 2, 16), (4096, 2, 16),
+                                   (3001, 7, 61), (20000, 8, 256), (300001, 2, 33)])
+def test_plan(T, k, E, cuda):
+    from nersemble_amd import experts as X
+    rng = np.random.default_rng(T + E)
+    c = rng.integers(0, E, (T, k)).astype(np.int32)
+    c[rng.random(T) < 0.2] = -1
+    if T > 10:
+        c[5, 0], c[6, 0], c[7, :] = E, 2 ** 31 - 1, -2 ** 31          # outside the experts
+    _check_plan(X.expert_plan(torch.from_numpy(c).to(cuda), E), ox.plan(np.where((c >= 0) & (c < E), c, -1), E))
+
+
+def test_plan_of_one_expert_and_of_none(cuda):
+    from nersemble_amd import experts as X
+    for T in (5, 5000, 200000):
+        for fill in (-1, 0, 7):
+            c = np.full((T, 2), fill, np.int32)
+            _check_plan(X.expert_plan(torch.from_numpy(c).to(cuda), 8), ox.plan(c, 8))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# products and join
+# ---------------------------------------------------------------------------------------------------------------------
+def _chosen(rng, T, k, E, masked, spread=None):
+    """Distinct experts per row; ``spread``: only that many experts are ever chosen (the others stay without rows)."""
+    use = min(E, spread or E)
+    c = np.argsort(rng.random((T, use)), axis=1)[:, :k].astype(np.int32)
+    c[rng.random(T) < masked] = -1
+    return c
+
+
+def _linear_case(cuda, T, k, E, K, N, dtype, gather, relu, master, masked, spread=None, seed=0):
+    from nersemble_amd import experts as X
+    rng = np.random.default_rng(seed + T + K + N)
+    dt = DT[dtype]
+    chosen = _chosen(rng, T, k, E, masked, spread)
+    plan = X.expert_plan(torch.from_numpy(chosen).to(cuda), E)
+    offsets, rows, positions = ox.plan(chosen, E)
+    R = T * k
+    x = torch.from_numpy(rng.standard_normal((T if gather else R, K)).astype(np.float32)).to(dt)
+    wf = torch.from_numpy((rng.standard_normal((E, N, K)) / np.sqrt(K)).astype(np.float32))
+    w16 = wf.to(dt)
+    dy = torch.from_numpy(rng.standard_normal((R, N)).astype(np.float32)).to(dt)
+    xd = x.to(cuda).requires_grad_(True)
+    wd = (wf if master else w16).to(cuda).requires_grad_(True)
+    y = X.expert_linear(xd, wd, plan, gather=gather, relu=relu)
+    h, tiny = HALF[dt]
+    want, mag = ox.linear(_f64(x), _f64(w16), offsets, rows, k, gather, relu)
+    assert y.dtype == dt and y.shape == (R, N)
+    _close(y, want, h * np.abs(want) + tiny + (K + 2) * 2 * U * mag, "y")
+    with torch.no_grad():
+        assert torch.equal(X.expert_linear(xd, wd, plan, gather=gather, relu=relu), y)
+    dx, dw = torch.autograd.grad(y, [xd, wd], dy.to(cuda))
+    assert dx.dtype == dt and dx.shape == x.shape and dw.dtype == wd.dtype
+    dz = np.where(_f64(y) > 0, _f64(dy), 0.0) if relu else _f64(dy)     # (a value next to 0 falls where the kernel's fell)
+    wx, mx, ww, mw = ox.linear_bwd(_f64(x), _f64(w16), offsets, rows, k, gather, dz)
+    n_e = np.diff(offsets)[:, None, None]
+    tw = (n_e + 2 + 64) * 2 * U * mw + ((h * np.abs(ww) + tiny) if not master else 0)
+    _close(dw, ww, tw, "dw")
+    tx = h * np.abs(wx) + tiny + (N + 2) * 2 * U * mx                    # in the plan's order
+    if gather:
+        one = np.ones((T, k))
+        tx = ox.combine(tx, one, positions)[0]
+        wx, _ = ox.combine(wx, one, positions)
+        tx = tx + h * np.abs(wx) + tiny
+    _close(dx, wx, tx * (1 + 4 * U * k), "dx")
+
+
+WIDTHS = [(8, 8), (16, 8), (32, 64), (64, 16), (64, 64), (40, 24), (176, 128), (128, 128), (72, 200), (264, 520), (1024, 136)]
+
+
+@pytest.mark.parametrize("K,N", WIDTHS)
+@pytest.mark.parametrize("dtype,gather,relu,master", [("fp16", True, True, False), ("bf16", True, False, False), ("fp16", False, False, True),
+                                                      ("bf16", False, True, True)])
+def test_linear_widths(K, N, dtype, gather, relu, master, cuda):
+    _linear_case(cuda, 211, 2, 5, K, N, dtype, gather, relu, master, 0.1)
+
+
+@pytest.mark.parametrize("T,k,E,spread", [(1, 1, 1, None), (1, 2, 8, None), (4, 3, 64, None), (17, 1, 3, None), (64, 2, 2, None), (65, 4, 9, 5),
+                                          (300, 1, 40, 7), (1025, 3, 7, None), (5000, 2, 16, None), (2600, 1, 1, None)])
+@pytest.mark.parametrize("masked", [0.0, 0.4, 1.0])
+def test_linear_rows(T, k, E, spread, masked, cuda):
+    _linear_case(cuda, T, k, E, 72, 48, "fp16", True, True, False, masked, spread, seed=1)
+    _linear_case(cuda, T, k, E, 48, 72, "bf16", False, False, True, masked, spread, seed=2)
+
+
+@pytest.mark.parametrize("K,N,T,k,E", [(512, 768, 700, 2, 6), (1024, 512, 1500, 1, 3), (32, 64, 30000, 2, 16), (64, 16, 30000, 2, 5),
+                                       (2048, 1024, 5, 4, 64), (1024, 2048, 40, 4, 32)])
+def test_linear_larger(K, N, T, k, E, cuda):
+    _linear_case(cuda, T, k, E, K, N, "bf16", True, False, False, 0.1)
+    _linear_case(cuda, T, k, E, K, N, "fp16", False, True, False, 0.0)
+
+
+def test_linear_row_of_infinities_stays_in_its_row(cuda):
+    """What is not finite in one row (or in one expert's weights) reaches that row (those rows) alone."""
+    from nersemble_amd import experts as X
+    T, E, K, N = 150, 3, 40, 24
+    rng = np.random.default_rng(3)
+    c = torch.from_numpy(rng.integers(0, E, (T, 1)).astype(np.int32)).to(cuda)
+    plan = X.expert_plan(c, E)
+    x = torch.from_numpy(rng.standard_normal((T, K)).astype(np.float16)).to(cuda)
+    w = torch.from_numpy(rng.standard_normal((E, N, K)).astype(np.float16)).to(cuda)
+    clean = X.expert_linear(x, w, plan)
+    x2 = x.clone()
+    x2[7], x2[11, 3] = float("inf"), float("nan")
+    got = X.expert_linear(x2, w, plan)
+    hit = torch.zeros(T, dtype=torch.bool, device=cuda)
+    hit[plan.positions[[7, 11], 0].long()] = True
+    assert torch.equal(got[~hit], clean[~hit]) and not torch.isfinite(got[hit]).any()
+    w2 = w.clone()
+    w2[1] = float("nan")
+    got = X.expert_linear(x, w2, plan)
+    mine = torch.zeros(T, dtype=torch.bool, device=cuda)
+    mine[int(plan.offsets[1]):int(plan.offsets[2])] = True
+    assert torch.equal(got[~mine], clean[~mine]) and torch.isnan(got[mine]).all()
+    assert torch.isnan(X.expert_linear(x2, w, plan, relu=True)[plan.positions[11, 0].long()]).all()
+
+
+def test_linear_layouts(cuda):
+    """Strided, transposed and misaligned rows, gradients and weights give what their contiguous copies give."""
+    from nersemble_amd import experts as X
+    g = torch.Generator(device=cuda).manual_seed(2)
+    T, k, E, K, N = 90, 2, 4, 32, 48
+    c = torch.randint(0, E, (T, k), generator=g, device=cuda, dtype=torch.int32)
+    plan = X.expert_plan(c, E)
+
+    def rnd(*s):
+        return torch.randn(s, generator=g, device=cuda).half()
+    xs = [rnd(T, 56)[:, 8:40], rnd(T, 41)[:, 3:35], rnd(K, T).t(), rnd(T * K + 1)[1:].view(T, K), rnd(1, K).expand(T, K)]
+    ws = [rnd(E, N, K), rnd(E, K, N).transpose(1, 2), rnd(E * N * K + 1)[1:].view(E, N, K), rnd(E, N, K), rnd(E, N, K)]
+    dys = [rnd(T * k, N), rnd(T * k, 64)[:, 8:56], rnd(N, T * k).t(), rnd(T * k, 49)[:, 1:], rnd(1, N).expand(T * k, N)]
+    for x, w, dy in zip(xs, ws, dys):
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        a2, b2 = x.detach().contiguous().clone().requires_grad_(True), w.detach().contiguous().clone().requires_grad_(True)
+        y, y2 = X.expert_linear(a, b, plan, relu=True), X.expert_linear(a2, b2, plan, relu=True)
+        assert torch.equal(y, y2)
+        for p, q in zip(torch.autograd.grad(y, [a, b], dy), torch.autograd.grad(y2, [a2, b2], dy.contiguous().clone())):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("T,k,N", [(1, 1, 8), (3, 5, 16), (130, 2, 64), (1000, 8, 24), (77, 3, 520), (50, 4, 2048), (20000, 2, 16)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("masked", [0.0, 0.5, 1.0])
+def test_combine(T, k, N, dtype, masked, cuda):
+    from nersemble_amd import experts as X
+    rng = np.random.default_rng(T + N)
+    E, dt = 9, DT[dtype]
+    chosen = _chosen(rng, T, k, E, masked)
+    chosen[rng.random((T, k)) < 0.1] = -1                 # single choices as well
+    plan = X.expert_plan(torch.from_numpy(chosen).to(cuda), E)
+    _, _, positions = ox.plan(chosen, E)
+    y = torch.from_numpy(rng.standard_normal((T * k, N)).astype(np.float32)).to(dt)
+    w = rng.random((T, k)).astype(np.float32)
+    g = torch.from_numpy(rng.standard_normal((T, N)).astype(np.float32)).to(dt)
+    yd, wd = y.to(cuda).requires_grad_(True), torch.from_numpy(w).to(cuda).requires_grad_(True)
+    out = X.expert_combine(yd, wd, plan)
+    h, tiny = HALF[dt]
+    want, mag = ox.combine(_f64(y), w, positions)
+    assert out.dtype == dt
+    _close(out, want, h * np.abs(want) + tiny + (k + 2) * 2 * U * mag, "out")
+    dy, dw = torch.autograd.grad(out, [yd, wd], g.to(cuda))
+    g64, y64 = _f64(g), _f64(y)
+    wdy, wdw, mdw = np.zeros_like(y64), np.zeros((T, k)), np.zeros((T, k))
+    for t in range(T):
+        for j in range(k):
+            if positions[t, j] >= 0:
+                p = positions[t, j]
+                wdy[p] = w[t, j].astype(np.float64) * g64[t]
+                wdw[t, j], mdw[t, j] = (g64[t] * y64[p]).sum(), (np.abs(g64[t]) * np.abs(y64[p])).sum()
+    _close(dy, wdy, (h + 2 * U) * np.abs(wdy) + tiny, "dy")
+    _close(dw, wdw, (N + 2) * 2 * U * mdw, "dweights")
+
+
+def test_plans_of_other_numbers_stay_inside_the_arrays(cuda):
+    """A plan whose numbers are not a plan's gives other results, but the kernels bound every index that they take from it."""
+    from nersemble_amd import experts as X
+    T, k, E, K, N = 64, 2, 4, 32, 48
+    x = torch.randn((T, K), device=cuda).half().requires_grad_(True)
+    w = torch.randn((E, N, K), device=cuda).half().requires_grad_(True)
+    wt = torch.rand((T, k), device=cuda, requires_grad=True)
+    big, low = 2 ** 31 - 1, -2 ** 31
+    offs = [[0, 500, 100, -7, big], [big, big, 0, 5, 9], [low, -1, low, 128, 128]]
+    fill = [big, low, 129]
+    for o, f in zip(offs, fill):
+        plan = X.ExpertPlan(torch.tensor(o, dtype=torch.int32, device=cuda), torch.full((T * k,), f, dtype=torch.int32, device=cuda),
+                            torch.full((T, k), f, dtype=torch.int32, device=cuda))
+        y = X.expert_linear(x, w, plan, relu=True)
+        out = X.expert_combine(y, wt, plan)
+        grads = torch.autograd.grad(out, [x, w, wt], torch.ones_like(out))
+        torch.cuda.synchronize()
+        assert out.shape == (T, N) and (out == 0).all() and all((q == 0).all() for q in grads)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# a run of them
+# ---------------------------------------------------------------------------------------------------------------------
+def _mixture(x, logits, w1, w2, E, k, selector=None, bias=None):
+    """The whole path of a routed network with one hidden layer."""
+    from nersemble_amd import experts as X
+    weights, chosen = X.route_experts(logits, k, bias=bias, selector=selector)
+    plan = X.expert_plan(chosen, E)
+    h = X.expert_linear(x, w1, plan, gather=True, relu=True)
+    y = X.expert_linear(h, w2, plan, gather=False)
+    return X.expert_combine(y, weights, plan)
+
+
+def _mixture64(x, logits, w1, w2, k, selector=None):
+    """The same, densely: every expert on every row, in 64 bits; rows without experts are 0."""
+    s = torch.softmax(logits, 1)
+    top = torch.sort(s, dim=1, descending=True, stable=True).indices[:, :k]
+    u = s.gather(1, top)
+    w = u / u.sum(1, keepdim=True)
+    if selector is not None:
+        w = w * selector[:, None]
+    y = torch.relu(torch.matmul(x, w1.transpose(1, 2).contiguous()))                    # [E, T, hidden]
+    y = torch.matmul(y, w2.transpose(1, 2).contiguous()).transpose(0, 1)                # [T, E, n]
+    return (w[..., None] * y.gather(1, top[..., None].expand(-1, -1, y.shape[2]))).sum(1)
+
+
+def _mixture_inputs(T, E, K, H, N, seed, dev):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g)                               # noqa: E731
+    x, logits = r(T, K).half(), r(T, E)
+    w1, w2 = (r(E, H, K) / K ** 0.5).half(), (r(E, N, H) / H ** 0.5).half()
+    return [v.to(dev).requires_grad_(True) for v in (x, logits, w1, w2)], r(T, N).half().to(dev)
+
+
+@pytest.mark.parametrize("T,E,k,K,H,N", [(1, 4, 2, 32, 64, 16), (501, 8, 2, 32, 64, 16), (333, 5, 3, 40, 128, 24)])
+def test_routed_chain(T, E, k, K, H, N, cuda):
+    """Route -> plan -> linear -> linear -> combine with all gradients, against dense 64-bit autograd.  Tolerance: the hidden row
+    is rounded to 16 bits (h of each term), as are y, dy and dh on the way; every one of the at most 4 roundings a path passes
+    moves a result by h times a norm-like sum of its terms, so 8 h relative to the largest entry of the tensor, and a hidden
+    unit that changes sides next to 0 by no more than that either."""
+    (x, logits, w1, w2), go = _mixture_inputs(T, E, K, H, N, 5, cuda)
+    sel = (torch.arange(T, device=cuda) % 5 != 3).to(torch.uint8)
+    out = _mixture(x, logits, w1, w2, E, k, sel)
+    grads = torch.autograd.grad(out, [x, logits, w1, w2], go)
+    leaves = [v.detach().double().cpu().requires_grad_(True) for v in (x, logits, w1, w2)]
+    want = _mixture64(*leaves, k, sel.double().cpu())
+    wg = torch.autograd.grad(want, leaves, go.double().cpu())
+    for name, a, b in zip(("out", "dx", "dlogits", "dw1", "dw2"), (out,) + grads, (want,) + wg):
+        tol = 8 * 2.0 ** -11 * float(b.abs().max())
+        assert float((a.detach().double().cpu() - b).abs().max()) <= tol, name
+
+
+def test_calls_repeat_bit_for_bit_and_on_another_stream(cuda):
+    (x, logits, w1, w2), go = _mixture_inputs(3000, 16, 32, 64, 16, 6, cuda)
+    first = None
+    for where in range(3):
+        s = torch.cuda.Stream() if where == 2 else torch.cuda.current_stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            out = _mixture(x, logits, w1, w2, 16, 2)
+            got = [out.detach()] + list(torch.autograd.grad(out, [x, logits, w1, w2], go))
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        if first is None:
+            first = got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+def test_two_graphs_of_a_step_replay(cuda):
+    """Forward and backward captured twice (two batches), replayed in turn with eager work between: every replay is the eager
+    result of what its inputs hold then."""
+    def inputs(seed, T):
+        return _mixture_inputs(T, 8, 32, 64, 16, seed, cuda)
+
+    def step(leaves, go):
+        leaves = [v.detach().requires_grad_(True) for v in leaves]
+        out = _mixture(*leaves, 8, 2)
+        return [out.detach()] + list(torch.autograd.grad(out, leaves, go))
+    graphs = []
+    side = torch.cuda.Stream()
+    for seed, T in ((1, 700), (2, 90000)):
+        leaves, go = inputs(seed, T)
+        static = [v.detach().clone() for v in leaves]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(static, go)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = step(static, go)
+        graphs.append((graph, static, go, res, T))
+    for turn in range(3):
+        for n, (graph, static, go, res, T) in enumerate(graphs):
+            new, _ = inputs(10 * turn + n, T)
+            for s, v in zip(static, new):
+                s.copy_(v.detach())
+            graph.replay()
+            want = step(static, go)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(res, want)), (turn, n)
+
+
+def test_device_side_row_count(cuda):
+    """Under ``device_count`` the rows behind the count are neither routed nor written, whatever they hold."""
+    from nersemble_amd import _lib
+    from nersemble_amd import experts as X
+    T, n, E, k = 600, 437, 8, 2
+    (x, logits, w1, w2), go = _mixture_inputs(T, E, 32, 64, 16, 7, cuda)
+    with torch.no_grad():
+        want = _mixture(x[:n], logits[:n], w1, w2, E, k)
+        x2, l2 = x.detach().clone(), logits.detach().clone()
+        x2[n:], l2[n:] = float("nan"), float("nan")
+        for count in (n, 0, T, -3):
+            c = torch.tensor([count], dtype=torch.int64, device=cuda)
+            with _lib.device_count(c, T):
+                weights, chosen = X.route_experts(l2 if count <= n else logits, k)
+                plan = X.expert_plan(chosen, E)
+                h = X.expert_linear(x2 if count <= n else x, w1, plan, relu=True)
+                out = X.expert_combine(X.expert_linear(h, w2, plan, gather=False), weights, plan)
+            routed = max(0, min(count, T)) * k
+            assert int(plan.offsets[-1]) == routed and (plan.rows[routed:] == -1).all() and (plan.positions[routed // k:] == -1).all()
+            assert torch.isfinite(h).all()
+            m = min(n, max(0, count))
+            assert torch.equal(out[:m], want[:m])
+    # gradients: weights see the valid rows alone
+    c = torch.tensor([n], dtype=torch.int64, device=cuda)
+    leaves = [v.detach().clone().requires_grad_(True) for v in (x2, l2, w1, w2)]
+    ref = [v.detach().clone().requires_grad_(True) for v in (x[:n], logits[:n], w1, w2)]
+    want = torch.autograd.grad(_mixture(*ref, E, k), ref, go[:n])
+    with _lib.device_count(c, T):
+        got = torch.autograd.grad(_mixture(*leaves, E, k), leaves, go)
+    assert torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
+    assert torch.equal(got[0][:n], want[0]) and torch.equal(got[1][:n], want[1])
+
+
+def test_the_same_tensor_twice_and_shared_plans(cuda):
+    """One weight in two products, one plan for two inputs, the gradients of both uses added."""
+    from nersemble_amd import experts as X
+    (x, logits, w1, _), _ = _mixture_inputs(200, 4, 64, 64, 16, 8, cuda)
+    _, chosen = X.route_experts(logits.detach(), 2)
+    plan = X.expert_plan(chosen, 4)
+    y = X.expert_linear(X.expert_linear(x, w1, plan, relu=True), w1, plan, gather=False)
+    dx, dw = torch.autograd.grad(y.float().sum(), [x, w1])
+    a, b = w1.detach().clone().requires_grad_(True), w1.detach().clone().requires_grad_(True)
+    y2 = X.expert_linear(X.expert_linear(x, a, plan, relu=True), b, plan, gather=False)
+    dx2, da, db = torch.autograd.grad(y2.float().sum(), [x, a, b])
+    assert torch.equal(dx, dx2) and torch.equal(dw, da + db)
+
+
+@pytest.mark.parametrize("n_in,n_out,n_hidden,routing", [
+    (32, 16, 1, dict(n_experts=4, top_k=2)), (35, 3, 2, dict(n_experts=6, top_k=1, renormalise=False)),
+    (16, 8, 1, dict(n_experts=8, top_k=3, scores="sigmoid", n_groups=4, top_groups=2, balance=True))])
+def test_routed_network(n_in, n_out, n_hidden, routing, cuda):
+    """tcnn.RoutedNetwork trains: finite gradients of every parameter, equal to those of the same mixture evaluated expert by
+    expert in 64 bits (tolerance as for the chain, one more rounding per hidden layer), and a step changes its output."""
+    from nersemble_amd import tcnn
+    net = tcnn.RoutedNetwork(n_in, n_out, {"n_neurons": 64, "n_hidden_layers": n_hidden}, routing).to(cuda)
+    g = torch.Generator().manual_seed(n_in)
+    x = torch.randn((301, n_in), generator=g).half()
+    go = torch.randn((301, n_out), generator=g).half()
+    xd = x.to(cuda).requires_grad_(True)
+    out = net(xd)
+    assert out.shape == (301, n_out) and out.dtype == torch.float16
+    got = torch.autograd.grad(out, [xd, net.gate, net.params], go.to(cuda))
+    # 64 bits, densely (the choice is the network's own: gaps of the scores are far above the rounding of the logits)
+    x64 = x.double().requires_grad_(True)
+    gate, params = (p.detach().double().cpu().requires_grad_(True) for p in (net.gate, net.params))
+    logits = x64 @ gate.t()
+    s = torch.sigmoid(logits) if routing.get("scores") == "sigmoid" else torch.softmax(logits, 1)
+    E, k = routing["n_experts"], routing["top_k"]
+    from nersemble_amd import experts as X
+    _, chosen = X.route_experts((xd.detach().float() @ net.gate.detach().t()), k, bias=net.balance, **net.routing)
+    idx = chosen.long().cpu()
+    u = s.gather(1, idx)
+    w = u / u.sum(1, keepdim=True) if routing.get("renormalise", True) else u
+    h = torch.nn.functional.pad(x64, (0, net.shapes[0][2] - n_in)).expand(E, -1, -1)
+    for n, (m, shape) in enumerate(zip(torch.split(params, [a * b * c for a, b, c in net.shapes]), net.shapes)):
+        m16 = m + (m.detach().half().double() - m.detach())                  # the fp16 values, the fp32 parameters' gradient
+        h = torch.matmul(h, m16.view(shape).transpose(1, 2))
+        h = torch.relu(h) if n < len(net.shapes) - 1 else h
+    y = h.transpose(0, 1).gather(1, idx[..., None].expand(-1, -1, h.shape[2]))
+    want = (w[..., None] * y).sum(1)[:, :n_out]
+    wg = torch.autograd.grad(want, [x64, gate, params], go.double())
+    for name, a, b in zip(("out", "dx", "dgate", "dparams"), (out,) + got, (want,) + wg):
+        tol = (6 + 4 * n_hidden) * 2.0 ** -11 * float(b.abs().max())
+        assert float((a.detach().double().cpu() - b).abs().max()) <= tol, name
+    assert int(net.load.sum()) == 301 * k
+    opt = torch.optim.Adam(net.parameters(), lr=1e-2)
+    net.gate.grad, net.params.grad = got[1], got[2]
+    opt.step()
+    assert not torch.equal(net(xd), out)
+    assert (net(xd, selector=torch.zeros(301, dtype=torch.uint8, device=cuda)) == 0).all()
+    if routing.get("balance"):
+        net.rebalance(0.5)
+        assert set(net.balance.abs().tolist()) <= {0.0, 0.5}
+    else:
+        with pytest.raises(RuntimeError):
+            net.rebalance()
