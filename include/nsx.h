@@ -1033,6 +1033,7 @@ int nsx_lp_backward(const nsx_lp_layout* lay, nsx_comm* comm, int emulate_rank, 
 #define NSX_MAX_TOP_K 64
 #define NSX_MAX_EXPERT_WIDTH 16384
 #define NSX_MAX_EXPERT_ENTRIES 1073741824      /* rows x top_k */
+#define NSX_MAX_EXPERT_STRIDE 1048576          /* elements from one row to the next in the products */
 /* Choice of the experts.  logits [T] rows of E values (row_stride elements apart); scores s = softmax (sigmoid = 0) or
  * 1 / (1 + exp(-x)) (sigmoid = 1); the choice goes by s + bias (bias [E] or NULL).  n_groups > 1: of the E / n_groups
  * consecutive experts each, the top_groups groups with the largest sum of their group_top (1 or 2) best experts stay.  Equal
@@ -1053,8 +1054,8 @@ int64_t nsx_expert_plan_workspace(int64_t n_entries, int E);
 int nsx_expert_plan(const int32_t* experts, int64_t T, int top_k, int E, int32_t* offsets, int32_t* rows, int32_t* positions,
                     void* workspace, const int64_t* n_device, void* stream);
 /* y [R][n_out]: ordered row p of expert e is act(weight[e] x[row]), weight [E][n_out][n_in], act = ReLU if relu.  rows = the
- * plan's (row = rows[p] / top_k) or NULL (x holds the R ordered rows).  dtype: 16 bits.  Widths are multiples of 8, rows and
- * matrices 16-byte aligned.  Ordered rows behind offsets[E] become 0. */
+ * plan's (row = rows[p] / top_k) or NULL (x holds the R ordered rows).  dtype: 16 bits.  Widths are multiples of 8, rows
+ * (at most NSX_MAX_EXPERT_STRIDE apart) and matrices 16-byte aligned.  Ordered rows behind offsets[E] become 0. */
 int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, int top_k,
                           const void* weight, int n_in, int n_out, int E, const int32_t* offsets, int64_t R, int relu, void* y,
                           void* stream);

@@ -15,6 +15,7 @@ NSX_OPT_LP_ONE_LAUNCH = 3
 NSX_COMM_ID_BYTES = 128
 NSX_DTYPE_F32, NSX_DTYPE_F16, NSX_DTYPE_BF16 = 0, 1, 2
 NSX_MAX_EXPERTS, NSX_MAX_TOP_K, NSX_MAX_EXPERT_WIDTH, NSX_MAX_EXPERT_ENTRIES = 512, 64, 16384, 1 << 30
+NSX_MAX_EXPERT_STRIDE = 1 << 20
 
 c_void_p, c_int, c_int64, c_float = C.c_void_p, C.c_int, C.c_int64, C.c_float
 

@@ -6,16 +6,24 @@
 //   forward  m = output feature, c = ordered row,      q = input feature    P = W (q contiguous)  Q = x (q contiguous)
 //   dx       m = input feature,  c = ordered row,      q = output feature   P = W (m contiguous)  Q = dz (q contiguous)
 //   dW       m = input feature,  c = output feature,   q = ordered row      P = x (m contiguous)  Q = dz (c contiguous)
-// One kernel: 16-bit tiles of P and Q in LDS with q contiguous (128 B per row, 16-byte pieces permuted by the row's number so
-// that neither the stores nor the fragment reads of 16 rows share banks), v_mfma_f32_16x16x32, 32-bit accumulators.  What is
-// not q-contiguous in memory is turned on its way through the registers: 4 q x 8 m per thread, 16 byte permutations, eight
-// 8-byte stores.  A lane holds 4 consecutive m of one c: 8-byte (16-byte for 32-bit gradients) stores.
+// One kernel: a workgroup makes a TM x TC tile in steps of 64 q.  16-bit tiles of P and Q lie in LDS with q contiguous;
+// v_mfma_f32_32x32x16 with 32-bit accumulators, a wave's tile up to 128 x 64.  What is not q-contiguous in memory is turned on
+// its way through the registers: 4 q x 8 m per thread, 16 byte permutations, eight 8-byte stores.
+//   * One LDS buffer and two or three workgroups per CU: while one stores its next tile and waits, another multiplies.  (Two
+//     buffers with one barrier per step, one workgroup of 8 waves and a 256 x 256 tile came to the same rate within 5 %, at a
+//     coarser grain: ragged segments and the last round of workgroups cost more.)
+//   * A step's global loads are issued under the first quarter of the previous step's products and stay in flight through
+//     them.  The fragments of a quarter step are read while its predecessor is multiplied, a P fragment into the registers of
+//     the one just used: 32 x 32 x 16 products need half the fragment registers of 16 x 16 x 32 (which spilled).
+//   * 16-bit results leave through LDS as whole rows.
 // Segments are read from the plan on the device: the grid covers the most tiles that any split of R rows over E experts can
 // have, every workgroup finds its (expert, tile) by one scan of the offsets.
 #include "expert_common.h"
+#include <algorithm>
 
 namespace nsx {
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 enum LinMode { LIN_FWD, LIN_DX, LIN_DW };
 
 struct LinArgs {
@@ -27,20 +35,24 @@ struct LinArgs {
     FastDiv top_k;
     int E, R, x_rows;
     int M, C, K;                     // extents of m, c (dW) and q (forward, dx)
-    int m_tiles, c_tiles, splits, relu;
-    float* partial;                  // dW with splits > 1: [split][E][C][M]
+    int m_tiles, c_tiles, relu;
+    int chunk;                       // dW: rows per partial sum (0: a whole segment, no partial sums)
+    float* partial;                  // [chunk][C][M]
 };
 
-template <typename T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
-template <> __device__ __forceinline__ f32x4 mfma16<half_t>(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(Elem<half_t>::x8, a), __builtin_bit_cast(Elem<half_t>::x8, b), c, 0, 0, 0);
+template <typename T> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mfma32<half_t>(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(Elem<half_t>::x8, a), __builtin_bit_cast(Elem<half_t>::x8, b), c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ f32x4 mfma16<bf16_t>(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Elem<bf16_t>::x8, a), __builtin_bit_cast(Elem<bf16_t>::x8, b), c, 0, 0, 0);
+template <> __device__ __forceinline__ f32x16 mfma32<bf16_t>(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Elem<bf16_t>::x8, a), __builtin_bit_cast(Elem<bf16_t>::x8, b), c, 0, 0, 0);
 }
 
-constexpr int LIN_BQ = 64;           // q per step: 128 B of 16-bit values
-__device__ __forceinline__ uint32_t lds_piece(int row, int ch) { return (uint32_t)(row * 128 + ((ch ^ (row ^ (row >> 3))) & 7) * 16); }
+constexpr int LIN_BQ = 64;           // q per step: rows of 128 B in LDS
+constexpr uint32_t lin_rows(uint32_t rows) { return rows * 128; }
+// Byte of a 16-byte piece of a row.  The permutation: a phase of a fragment read takes 16 rows (half of the 64 banks each), and
+// the turned stores take rows 8 apart -- both have to fall on different banks.
+__device__ __forceinline__ uint32_t lin_piece(int row, int ch) { return row * 128 + ((ch ^ (row >> 1) ^ ((row >> 4) & 3)) & 7) * 16; }
 
 // both 16-bit halves of `v` kept where those of `y` (not negative) are not zero
 __device__ __forceinline__ uint32_t keep_where(uint32_t v, uint32_t y) {
@@ -48,76 +60,31 @@ __device__ __forceinline__ uint32_t keep_where(uint32_t v, uint32_t y) {
     return v & (t | (t - (t >> 15)));
 }
 
-// One operand's share of a thread: ROWS rows (of m or c) x 64 q per step, by NT threads.
-template <int ROWS, int NT, bool MASK>
-struct AlongQ {                      // q contiguous in memory
-    static constexpr int N = ROWS * 8 / NT;
-    const char* at[N]; const char* mk[MASK ? N : 1];
-    u32x4 v[N], y[MASK ? N : 1];
-    __device__ __forceinline__ void load(int q0, int q_end) {
-        const int q = q0 + (threadIdx.x & 7) * 8;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const bool ok = at[i] && q < q_end;
-            v[i] = ok ? *reinterpret_cast<const u32x4*>(at[i] + (int64_t)q * 2) : u32x4{0, 0, 0, 0};
-            if (MASK) y[i] = ok ? *reinterpret_cast<const u32x4*>(mk[i] + (int64_t)q * 2) : u32x4{0, 0, 0, 0};
-        }
-    }
-    __device__ __forceinline__ void store(char* lds) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (MASK)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) v[i][w] = keep_where(v[i][w], y[i][w]);
-            const int id = threadIdx.x + i * NT;
-            *reinterpret_cast<u32x4*>(lds + lds_piece(id >> 3, id & 7)) = v[i];
-        }
-    }
-};
+// 0 for gathered rows that are not there: what is loaded without a branch is loaded from here
+__device__ u32x4 lin_zeros[NSX_MAX_EXPERT_WIDTH / 8 + LIN_BQ / 8];
+__device__ __forceinline__ const char* zero_row() { return reinterpret_cast<const char*>(lin_zeros); }
+__device__ __forceinline__ u32x4 load16(const char* p) { return *reinterpret_cast<const u32x4*>(p); }
+// reads behind `bytes` give 0
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t lin_buffer(const char* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)min(bytes, (int64_t)0x7fffffff), 0x00020000);
+}
+__device__ __forceinline__ u32x4 lin_load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0));
+}
 
-template <int ROWS, int NT, bool MASK>
-struct AcrossQ {                     // the other index contiguous in memory
-    static constexpr int ITEMS = ROWS * 2, N = (ITEMS + NT - 1) / NT;
-    u32x4 v[N][4], y[MASK ? N : 1][4];
-    // at(q) -> address of the row of q (NULL: nothing there); m: first index of the tile, m_end: its extent
-    template <class At, class Mk>
-    __device__ __forceinline__ void load(int q0, int q_end, int m, int m_end, At at, Mk mk) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = threadIdx.x + i * NT, m8 = id % (ROWS / 8), q4 = id / (ROWS / 8);
-            const bool in = (ITEMS % NT == 0 || id < ITEMS) && m + m8 * 8 < m_end;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int q = q0 + q4 * 4 + r;
-                const char* src = in && q < q_end ? at(q) : nullptr;
-                v[i][r] = src ? *reinterpret_cast<const u32x4*>(src + (int64_t)(m + m8 * 8) * 2) : u32x4{0, 0, 0, 0};
-                if (MASK) y[i][r] = src ? *reinterpret_cast<const u32x4*>(mk(q) + (int64_t)(m + m8 * 8) * 2) : u32x4{0, 0, 0, 0};
-            }
-        }
+// ---- which tile ---------------------------------------------------------------------------------------------------
+// row tiles of all segments and of the rows behind the last one
+__device__ __forceinline__ int count_tiles(const int32_t* __restrict__ offsets, int E, int R, int rows) {
+    int n = 0;
+    for (int e = threadIdx.x & 63; e <= E; e += kWave) {
+        int a, b;
+        if (e < E) segment(offsets, e, R, a, b);
+        else { a = min(max(offsets[E], 0), R); b = R; }
+        n += (b - a + rows - 1) / rows;
     }
-    __device__ __forceinline__ void store(char* lds) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = threadIdx.x + i * NT, m8 = id % (ROWS / 8), q4 = id / (ROWS / 8);
-            if (ITEMS % NT != 0 && id >= ITEMS) continue;
-            if (MASK)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) v[i][r][w] = keep_where(v[i][r][w], y[i][r][w]);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t sel = h ? 0x07060302u : 0x05040100u;
-                    const u32x2 o = {__builtin_amdgcn_perm(v[i][1][w], v[i][0][w], sel), __builtin_amdgcn_perm(v[i][3][w], v[i][2][w], sel)};
-                    *reinterpret_cast<u32x2*>(lds + lds_piece(m8 * 8 + w * 2 + h, q4 >> 1) + (q4 & 1) * 8) = o;
-                }
-            }
-        }
-    }
-};
-
+    for (int o = 1; o < kWave; o <<= 1) n += __shfl_xor(n, o);
+    return __builtin_amdgcn_readfirstlane(n);
+}
 // (expert, first row, end) of row tile `tile`; expert E: the rows behind the last segment; false: there is no such tile
 __device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, int E, int R, int rows, int tile, int& e, int& a, int& b) {
     const int lane = threadIdx.x & 63;
@@ -133,159 +100,290 @@ __device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, i
         if (tile < base + total) {
             const int l = __ffsll((unsigned long long)__ballot(base + incl > tile)) - 1;
             e = e0 + l;
-            a = __builtin_amdgcn_readlane(sa, l) + (tile - base - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l))) * rows;
-            b = min(a + rows, __builtin_amdgcn_readlane(sb, l));
-            return true;
+            const int start = __builtin_amdgcn_readlane(sa, l), end = __builtin_amdgcn_readlane(sb, l);
+            a = start + (tile - base - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l))) * rows;
+            b = min(a + rows, end);
+            return a >= start && a < b;                    // (always, of a plan's offsets)
         }
         base += total;
     }
     return false;
 }
+// Consecutive workgroups go to the 8 XCDs in turn; those that run on one at a time should share what they read through its L2.
+// Forward and dx: each XCD takes a stretch of its own of an order in which 8 row tiles pass through all m tiles.
+constexpr int LIN_GROUP = 8;
+__device__ __forceinline__ bool lin_order(int tiles, int m_tiles, int block, int& tile, int& m) {
+    const int64_t all = (int64_t)tiles * m_tiles, per = (all + 7) / 8, id = (block & 7) * per + (block >> 3);
+    if ((block >> 3) >= per || id >= all) return false;
+    const int group = (int)(id / (LIN_GROUP * m_tiles)), rest = (int)(id - (int64_t)group * (LIN_GROUP * m_tiles));
+    const int n = min(LIN_GROUP, tiles - group * LIN_GROUP);
+    m = rest / n;
+    tile = group * LIN_GROUP + rest - m * n;
+    return true;
+}
+// dW: an XCD takes blocks of 4 x 4 tiles of one segment (or chunk of one) in turn with the others
+__device__ __forceinline__ bool lin_order_dw(const LinArgs& g, int block, int& s, int& m, int& c) {
+    const int gm = (g.m_tiles + 3) / 4, gc = (g.c_tiles + 3) / 4;
+    const int local = block >> 3, within = local & 15;
+    int group = (local >> 4) * 8 + (block & 7);
+    m = group % gm * 4 + (within & 3); group /= gm;
+    c = group % gc * 4 + (within >> 2);
+    s = group / gc;
+    return m < g.m_tiles && c < g.c_tiles;
+}
 
+// ---- the products -------------------------------------------------------------------------------------------------
 template <typename T, int MODE, int TM, int TC, int WM, int WC, bool MASK, bool F32>
-__global__ __launch_bounds__(WM * WC * kWave) void expert_linear_kernel(LinArgs g) {
-    constexpr int NT = WM * WC * kWave, FM = TM / WM / 16, FC = TC / WC / 16, STAGE = (TM + TC) * 128;
+__global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lin_lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wc = wave / WM;
-    int e, a, b, m0, c0 = 0, split = 0;
+    constexpr bool P_ALONG = MODE == LIN_FWD, Q_ALONG = MODE != LIN_DW;
+    constexpr int NT = WM * WC * kWave, FM = TM / WM / 32, FC = TC / WC / 32, NP = TM * 8 / NT, NQ = TC * 8 / NT, RPT = NT / 8;
+    constexpr uint32_t Q_AT = lin_rows(TM);
+    static_assert(NP % 4 == 0 && NQ % 4 == 0, "a thread turns 4 rows of q");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wc = wave / WM;
+    int e, a, b, m0, c0 = 0, chunk = 0;
     if (MODE == LIN_DW) {
-        int id = blockIdx.x;
-        m0 = (id % g.m_tiles) * TM; id /= g.m_tiles;
-        c0 = (id % g.c_tiles) * TC; id /= g.c_tiles;
-        e = id % g.E; split = id / g.E;
-        segment(g.offsets, e, g.R, a, b);
-        if (g.splits > 1) {
-            const int len = ((b - a + g.splits - 1) / g.splits + LIN_BQ - 1) / LIN_BQ * LIN_BQ;
-            a = (int)min((int64_t)a + (int64_t)split * len, (int64_t)b);
-            b = min(a + len, b);
+        if (!lin_order_dw(g, blockIdx.x, chunk, m0, c0)) return;
+        m0 *= TM; c0 *= TC;
+        if (g.chunk > 0) {
+            if (chunk >= g.R / g.chunk + g.E || !find_tile(g.offsets, g.E, g.R, g.chunk, chunk, e, a, b) || e == g.E) return;
+        } else {
+            if (chunk >= g.E) return;
+            e = chunk;
+            segment(g.offsets, e, g.R, a, b);
         }
     } else {
-        m0 = (blockIdx.x % g.m_tiles) * TM;
-        if (!find_tile(g.offsets, g.E, g.R, TC, blockIdx.x / g.m_tiles, e, a, b)) return;
+        int tile;
+        if (!lin_order(count_tiles(g.offsets, g.E, g.R, TC), g.m_tiles, blockIdx.x, tile, m0)) return;
+        m0 *= TM;
+        if (!find_tile(g.offsets, g.E, g.R, TC, tile, e, a, b)) return;
     }
     const bool nothing = MODE != LIN_DW && e == g.E;
-    const T* P = reinterpret_cast<const T*>(g.p) + (MODE != LIN_DW && !nothing ? e * g.p_expert : 0);
-    const T* Q = reinterpret_cast<const T*>(g.q);
-    const T* Y = reinterpret_cast<const T*>(g.mask);
+    const char* P = reinterpret_cast<const char*>(g.p) + (MODE != LIN_DW && !nothing ? e * g.p_expert * 2 : 0);
+    const char* Q = reinterpret_cast<const char*>(g.q);
+    const char* Y = reinterpret_cast<const char*>(g.mask);
     const int q_begin = MODE == LIN_DW ? a : 0, q_end = MODE == LIN_DW ? b : (nothing ? 0 : g.K);
 
-    f32x4 acc[FM][FC];
+    f32x16 acc[FM][FC];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FC; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < FC; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    typedef typename std::conditional<MODE == LIN_FWD, AlongQ<TM, NT, false>, AcrossQ<TM, NT, false>>::type StageP;
-    typedef typename std::conditional<MODE == LIN_DW, AcrossQ<TC, NT, MASK>, AlongQ<TC, NT, MASK>>::type StageQ;
-    StageP sp;
-    StageQ sq;
-    if constexpr (MODE == LIN_FWD) {
+    // Global reads.  Along q: rows tid / 8 + RPT i, piece tid % 8; across q: pieces tid % (rows / 8) of rows of q, 4 to a thread.
+    // What has no rows to gather goes through a buffer descriptor whose range ends where the data does (0 behind it).
+    constexpr int PM = TM / 8, QC = TC / 8;
+    const int pm = min(m0 + (tid % PM) * 8, g.M - 8) * 2, qc = min(c0 + (tid % QC) * 8, g.C - 8) * 2;
+    const uint32_t q_row = (uint32_t)g.ldq * 2, y_row = (uint32_t)g.ldmask * 2, p_row = (uint32_t)g.ldp * 2;
+    auto quad = [&](int rows8, int k) { return (tid / rows8 + k * (NT / rows8)) ^ (rows8 >= 16 ? (tid >> 3) & 1 : 0); };
+    auto p_across = [&](int i) { return quad(PM, i >> 2) * 4 + (i & 3); };
+    auto q_across = [&](int i) { return quad(QC, i >> 2) * 4 + (i & 3); };
+    constexpr int NROW = MODE == LIN_FWD ? NQ : MODE == LIN_DW ? NP : 1;
+    int row[NROW];                               // gathered rows: of Q (forward), of P one step ahead (dW)
+    if (MODE == LIN_FWD)
 #pragma unroll
-        for (int i = 0; i < StageP::N; ++i) {
-            const int m = m0 + ((threadIdx.x + i * NT) >> 3);
-            sp.at[i] = m < g.M ? reinterpret_cast<const char*>(P + (int64_t)m * g.ldp) : nullptr;
+        for (int i = 0; i < NROW; ++i) {
+            const int p = min(a + (tid >> 3) + RPT * i, b - 1);
+            row[i] = p;
+            if (g.rows) { row[i] = g.rows[p]; row[i] = row[i] >= 0 ? g.top_k(row[i]) : -1; }
+            if (row[i] >= g.x_rows) row[i] = -1;
         }
-    }
-    if constexpr (MODE != LIN_DW) {
+    auto locate = [&](int q0) {                  // (the entry as it is: what follows from it is computed where it is used)
+        if (MODE == LIN_DW)
 #pragma unroll
-        for (int i = 0; i < StageQ::N; ++i) {
-            const int p = a + ((threadIdx.x + i * NT) >> 3);
-            const char *src = nullptr, *my = nullptr;
-            if (p < b && !nothing) {
-                int row = p;
-                if (MODE == LIN_FWD && g.rows) { row = g.rows[p]; row = row >= 0 ? g.top_k(row) : g.x_rows; }
-                if (MODE != LIN_FWD || (unsigned)row < (unsigned)g.x_rows) src = reinterpret_cast<const char*>(Q + (int64_t)row * g.ldq);
-                if (MASK) my = reinterpret_cast<const char*>(Y + (int64_t)row * g.ldmask);
+            for (int r = 0; r < NROW; ++r) {
+                const int q = min(q0 + p_across(r), q_end - 1);
+                row[r] = g.rows ? g.rows[q] : q;
             }
-            sq.at[i] = src;
-            if (MASK) sq.mk[i] = my;
-        }
-    }
-    auto load = [&](int q0) {
-        if constexpr (MODE == LIN_FWD) sp.load(q0, q_end);
-        else if constexpr (MODE == LIN_DX)
-            sp.load(q0, q_end, m0, g.M, [&](int q) { return reinterpret_cast<const char*>(P + (int64_t)q * g.ldp); }, [](int) { return (const char*)nullptr; });
-        else
-            sp.load(q0, q_end, m0, g.M, [&](int q) {
-                int row = q;
-                if (g.rows) { row = g.rows[q]; row = row >= 0 ? g.top_k(row) : g.x_rows; }
-                return (unsigned)row < (unsigned)g.x_rows ? reinterpret_cast<const char*>(P + (int64_t)row * g.ldp) : nullptr;
-            }, [](int) { return (const char*)nullptr; });
-        if constexpr (MODE == LIN_DW)
-            sq.load(q0, q_end, c0, g.C, [&](int q) { return reinterpret_cast<const char*>(Q + (int64_t)q * g.ldq); },
-                    [&](int q) { return reinterpret_cast<const char*>(Y + (int64_t)q * g.ldmask); });
-        else sq.load(q0, q_end);
     };
-    auto store = [&](int buf) { sp.store(lin_lds + buf * STAGE); sq.store(lin_lds + buf * STAGE + TM * 128); };
+    auto row_of = [&](int q, int r) {
+        int v = row[r];
+        if (g.rows) v = v >= 0 ? g.top_k(v) : -1;
+        return q < q_end && v < g.x_rows ? v : -1;
+    };
+    u32x4 pv[NP], qv[NQ], yv[MASK ? NQ : 1];
+    const auto p_buf = lin_buffer(P, MODE == LIN_DW ? 0 : (int64_t)g.p_expert * 2);
+    const auto q_buf = lin_buffer(Q + (MODE == LIN_DX ? (int64_t)a * q_row : 0), MODE == LIN_DX ? (int64_t)(b - a) * q_row : 0);
+    const auto y_buf = lin_buffer(MASK ? Y + (MODE == LIN_DX ? (int64_t)a * y_row : 0) : Q, MODE == LIN_DX ? (int64_t)(b - a) * y_row : 0);
+    auto load_p = [&](int q0, int i) {
+        const int q = q0 + (tid & 7) * 8;
+        if (MODE == LIN_FWD) pv[i] = lin_load(p_buf, (uint32_t)(m0 + (tid >> 3) + RPT * i) * p_row + q * 2 | (q >= q_end ? 0x80000000u : 0u));
+        else if (MODE == LIN_DX) pv[i] = lin_load(p_buf, (uint32_t)(q0 + p_across(i)) * p_row + pm);
+        else {
+            const int r = row_of(q0 + p_across(i), i);
+            pv[i] = load16(r < 0 ? zero_row() : P + (uint64_t)(uint32_t)r * p_row + pm);
+        }
+    };
+    auto load_q = [&](int q0, int i) {
+        const int q = q0 + (tid & 7) * 8;
+        const uint32_t past = q >= q_end ? 0x80000000u : 0u;         // (behind every range)
+        if (MODE == LIN_FWD) qv[i] = load16(past || row[i] < 0 ? zero_row() : Q + (uint64_t)(uint32_t)row[i] * q_row + q * 2);
+        else if (MODE == LIN_DX) {
+            qv[i] = lin_load(q_buf, (uint32_t)((tid >> 3) + RPT * i) * q_row + q * 2 | past);
+            if (MASK) yv[i] = lin_load(y_buf, (uint32_t)((tid >> 3) + RPT * i) * y_row + q * 2 | past);
+        } else {
+            const int64_t left = max(q_end - q0, 0);
+            qv[i] = lin_load(lin_buffer(Q + (int64_t)q0 * q_row, left * q_row), (uint32_t)q_across(i) * q_row + qc);
+            if (MASK) yv[i] = lin_load(lin_buffer(Y + (int64_t)q0 * y_row, left * y_row), (uint32_t)q_across(i) * y_row + qc);
+        }
+    };
+    auto mask_q = [&](int i) {
+        if (MASK)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) qv[i][w] = keep_where(qv[i][w], yv[i][w]);
+    };
+    const uint32_t st_along = lin_piece(tid >> 3, tid & 7);
+    auto put_across = [&](uint32_t base, int rows8, const u32x4* v, int i) {     // (v: 4 rows of q; i: which two of 8 rows of m or c)
+        const int k = i >> 2, w = i & 3, q4 = quad(rows8, k);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t sel = h ? 0x07060302u : 0x05040100u;
+            const u32x2 o = {__builtin_amdgcn_perm(v[k * 4 + 1][w], v[k * 4][w], sel), __builtin_amdgcn_perm(v[k * 4 + 3][w], v[k * 4 + 2][w], sel)};
+            *reinterpret_cast<u32x2*>(lin_lds + base + lin_piece((tid % rows8) * 8 + w * 2 + h, q4 >> 1) + (q4 & 1) * 8) = o;
+        }
+    };
+    auto put_p = [&](int i) {
+        if (P_ALONG) *reinterpret_cast<u32x4*>(lin_lds + (st_along ^ (RPT * i >> 4 & 3) * 16) + i * lin_rows(RPT)) = pv[i];
+        else put_across(0, PM, pv, i);
+    };
+    auto put_q = [&](int i) {
+        if (Q_ALONG) *reinterpret_cast<u32x4*>(lin_lds + Q_AT + (st_along ^ (RPT * i >> 4 & 3) * 16) + i * lin_rows(RPT)) = qv[i];
+        else put_across(Q_AT, QC, qv, i);
+    };
+    // fragments: row 32 i + (lane & 31) of the wave's rows, piece 2 s + lane / 32
+    const uint32_t fr_p = wm * lin_rows(TM / WM), fr_q = Q_AT + wc * lin_rows(TC / WC);
+    uint32_t fr[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) fr[s] = lin_piece(lane & 31, 2 * s + (lane >> 5));
+    auto frag = [&](uint32_t at, int row0, int s, int i) {
+        return *reinterpret_cast<const u32x4*>(lin_lds + at + (fr[s] ^ ((row0 >> 5) + i & 1) * 32) + i * lin_rows(32));
+    };
+    u32x4 fp[FM], fq[2][FC];
 
     if (q_begin < q_end) {
-        load(q_begin);
-        store(0);
-        __syncthreads();
-        int buf = 0;
+        locate(q_begin);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) load_p(q_begin, i);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) load_q(q_begin, i);
+        locate(q_begin + LIN_BQ);
         for (int q0 = q_begin; q0 < q_end; q0 += LIN_BQ) {
-            const bool more = q0 + LIN_BQ < q_end;
-            if (more) load(q0 + LIN_BQ);
-            const char* lp = lin_lds + buf * STAGE;
-            const char* lq = lp + TM * 128;
+            if (q0 > q_begin) __syncthreads();
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                u32x4 fp[FM], fq[FC];
+            for (int i = 0; i < NP; ++i) put_p(i);
 #pragma unroll
-                for (int i = 0; i < FM; ++i)
-                    fp[i] = *reinterpret_cast<const u32x4*>(lp + lds_piece(wm * (TM / WM) + i * 16 + (lane & 15), s * 4 + (lane >> 4)));
+            for (int i = 0; i < NQ; ++i) mask_q(i);
 #pragma unroll
-                for (int j = 0; j < FC; ++j)
-                    fq[j] = *reinterpret_cast<const u32x4*>(lq + lds_piece(wc * (TC / WC) + j * 16 + (lane & 15), s * 4 + (lane >> 4)));
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < FC; ++j) acc[i][j] = mfma16<T>(fp[i], fq[j], acc[i][j]);
-            }
-            if (more) store(buf ^ 1);
+            for (int i = 0; i < NQ; ++i) put_q(i);
             __syncthreads();
-            buf ^= 1;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fp[i] = frag(fr_p, wm * (TM / WM), 0, i);
+#pragma unroll
+            for (int j = 0; j < FC; ++j) fq[0][j] = frag(fr_q, wc * (TC / WC), 0, j);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+#pragma unroll
+                    for (int j = 0; j < FC; ++j) acc[i][j] = mfma32<T>(fp[i], fq[s & 1][j], acc[i][j]);
+                    if (s < 3) {
+                        fp[i] = frag(fr_p, wm * (TM / WM), s + 1, i);
+#pragma unroll
+                        for (int j = i * FC / FM; j < (i + 1) * FC / FM; ++j) fq[(s + 1) & 1][j] = frag(fr_q, wc * (TC / WC), s + 1, j);
+                    }
+                    if (s == 0) {
+#pragma unroll
+                        for (int k = i * NP / FM; k < (i + 1) * NP / FM; ++k) load_p(q0 + LIN_BQ, k);
+#pragma unroll
+                        for (int k = i * NQ / FM; k < (i + 1) * NQ / FM; ++k) load_q(q0 + LIN_BQ, k);
+                        if (i == FM - 1) locate(q0 + 2 * LIN_BQ);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
         }
     }
 
-    const int c_base = wc * (TC / WC) + (lane & 15), m_base = m0 + wm * (TM / WM) + (lane >> 4) * 4;
+    const int c_first = (MODE == LIN_DW ? c0 : a) + wc * (TC / WC), c_end = MODE == LIN_DW ? g.C : b, m_first = m0 + wm * (TM / WM);
+    if (F32) {
+        float* D = g.chunk > 0 ? g.partial + (int64_t)chunk * g.C * g.M : reinterpret_cast<float*>(g.d) + e * g.d_expert;
+        const int64_t ldd = g.chunk > 0 ? g.M : g.ldd;
+#pragma unroll
+        for (int j = 0; j < FC; ++j) {
+            const int c = c_first + j * 32 + (lane & 31);
+            if (c >= c_end) continue;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int m = m_first + i * 32 + u * 8 + (lane >> 5) * 4;
+                    if (m < g.M) *reinterpret_cast<f32x4*>(D + (int64_t)c * ldd + m) = f32x4{acc[i][j][u * 4], acc[i][j][u * 4 + 1], acc[i][j][u * 4 + 2], acc[i][j][u * 4 + 3]};
+                }
+        }
+        return;
+    }
+    // 16-bit results: 32 rows of the wave's tile at a time through LDS, so that whole rows leave (as the lanes hold them they are
+    // 16 bytes of each of 32 rows per instruction: 40 % of all requests to L2 at 1024 -> 2048, 8 % of the time)
+    constexpr int ROW = TM / WM * 2 + 16, LPR = TM / WM / 8;                 // bytes per row in LDS; lanes per row
+    char* mine = lin_lds + wave * 32 * ROW;
+    T* D = reinterpret_cast<T*>(g.d) + (MODE == LIN_DW ? e * g.d_expert : 0);
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < FC; ++j) {
-        const int c = MODE == LIN_DW ? c0 + c_base + j * 16 : a + c_base + j * 16;
-        if (c >= (MODE == LIN_DW ? g.C : b)) continue;
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const int m = m_base + i * 16;
-            if (m >= g.M) continue;
-            f32x4 v = acc[i][j];
-            if (MODE == LIN_FWD && g.relu)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = v[r] <= 0.f ? 0.f : v[r];         // (NaN stays)
-            if (MODE == LIN_DW && g.splits > 1) {
-                *reinterpret_cast<f32x4*>(g.partial + (((int64_t)split * g.E + e) * g.C + c) * g.M + m) = v;
-            } else if (F32) {
-                *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(g.d) + e * g.d_expert + (int64_t)c * g.ldd + m) = v;
-            } else {
+            for (int u = 0; u < 4; ++u) {
                 typename Elem<T>::x4 o;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] = (T)v[r];
-                *reinterpret_cast<typename Elem<T>::x4*>(reinterpret_cast<T*>(g.d) + (MODE == LIN_DW ? e * g.d_expert : 0) + (int64_t)c * g.ldd + m) = o;
+                for (int r = 0; r < 4; ++r) {
+                    float v = acc[i][j][u * 4 + r];
+                    if (MODE == LIN_FWD && g.relu) v = v <= 0.f ? 0.f : v;            // (NaN stays)
+                    o[r] = (T)v;
+                }
+                *reinterpret_cast<typename Elem<T>::x4*>(mine + (lane & 31) * ROW + (i * 32 + u * 8 + (lane >> 5) * 4) * 2) = o;
             }
-        }
-    }
-}
-
-// sums of the splits, in the order of the splits
-template <typename T>
-__global__ __launch_bounds__(256) void expert_sum_splits_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ d) {
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-        f32x4 s = *reinterpret_cast<const f32x4*>(part + i);
-        for (int q = 1; q < splits; ++q) s += *reinterpret_cast<const f32x4*>(part + q * n + i);
+        wave_lds_fence();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) d[i + r] = (T)s[r];
+        for (int k = 0; k < 32 * LPR / kWave; ++k) {
+            const int r = k * (kWave / LPR) + lane / LPR, c = c_first + j * 32 + r, m = m_first + lane % LPR * 8;
+            if (c < c_end && m < g.M)
+                *reinterpret_cast<u32x4*>(D + (int64_t)c * g.ldd + m) = *reinterpret_cast<const u32x4*>(mine + r * ROW + lane % LPR * 16);
+        }
+        wave_lds_fence();
     }
 }
 
+// dW of an expert = the sum of its chunks, in their order.  16 chunks at a time side by side, 16 x 4 values per workgroup.
+template <typename T>
+__global__ __launch_bounds__(256) void expert_sum_chunks_kernel(LinArgs g, T* __restrict__ d) {
+    __shared__ f32x4 part[16][16];
+    const int e = blockIdx.y, lane = threadIdx.x & 63, who = threadIdx.x >> 4, at = threadIdx.x & 15;
+    int first = 0, a, b;
+    for (int q = lane; q < e; q += kWave) { segment(g.offsets, q, g.R, a, b); first += (b - a + g.chunk - 1) / g.chunk; }
+    for (int o = 1; o < kWave; o <<= 1) first += __shfl_xor(first, o);
+    segment(g.offsets, e, g.R, a, b);
+    const int n = min((b - a + g.chunk - 1) / g.chunk, g.R / g.chunk + g.E - first);
+    const int64_t size = (int64_t)g.C * g.M;
+    for (int64_t i0 = (int64_t)blockIdx.x * 64; i0 < size; i0 += (int64_t)gridDim.x * 64) {
+        const int64_t i = i0 + at * 4;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        if (i < size)
+            for (int q = who; q < n; q += 16) s += *reinterpret_cast<const f32x4*>(g.partial + (first + q) * size + i);
+        part[who][at] = s;
+        __syncthreads();
+        if (who == 0 && i < size) {
+            for (int q = 1; q < 16; ++q) s += part[q][at];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d[(int64_t)e * size + i + r] = (T)s[r];
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------
 static int lin_check(const char* what, int dtype, int n_in, int n_out, int E, int64_t R, int top_k, const int32_t* offsets) {
     NSX_REQUIRE(dtype == NSX_DTYPE_F16 || dtype == NSX_DTYPE_BF16, "%s: dtype %d is not a 16-bit float", what, dtype);
     NSX_REQUIRE(E >= 1 && E <= NSX_MAX_EXPERTS, "%s: n_experts %d not in [1,%d]", what, E, NSX_MAX_EXPERTS);
@@ -296,22 +394,41 @@ static int lin_check(const char* what, int dtype, int n_in, int n_out, int E, in
     NSX_REQUIRE(offsets, "%s: NULL offsets", what);
     return NSX_OK;
 }
+static bool lin_stride(int64_t stride, int n) { return stride >= n && stride % 8 == 0 && stride <= NSX_MAX_EXPERT_STRIDE; }
 
 template <typename T, int MODE, int TM, int TC, int WM, int WC, bool F32>
-static void lin_launch(const LinArgs& g, int64_t blocks, hipStream_t st) {
-    constexpr int lds = 2 * (TM + TC) * 128;
+static int lin_launch_tile(LinArgs g, hipStream_t st) {
+    constexpr int lds = std::max((int)lin_rows(TM + TC), WM * WC * 32 * (TM / WM * 2 + 16));
+    static_assert(lds <= 65536, "");
+    g.m_tiles = (g.M + TM - 1) / TM;
+    g.c_tiles = (g.C + TC - 1) / TC;
+    int64_t blocks;
+    if (MODE == LIN_DW) {
+        const int64_t groups = (g.chunk > 0 ? g.R / g.chunk + g.E : g.E) * (int64_t)((g.m_tiles + 3) / 4) * ((g.c_tiles + 3) / 4);
+        blocks = (groups + 7) / 8 * 128;
+    } else {
+        blocks = ((int64_t)g.R / TC + g.E + 1) * g.m_tiles;
+        blocks = (blocks + 7) / 8 * 8;
+    }
+    NSX_REQUIRE(blocks <= 0x7fffffff, "expert_linear: %lld tiles", (long long)blocks);
     if (g.mask) expert_linear_kernel<T, MODE, TM, TC, WM, WC, true, F32><<<(unsigned)blocks, WM * WC * kWave, lds, st>>>(g);
     else expert_linear_kernel<T, MODE, TM, TC, WM, WC, false, F32><<<(unsigned)blocks, WM * WC * kWave, lds, st>>>(g);
+    return NSX_OK;
 }
 
-static int64_t row_tiles(int64_t R, int E, int rows) { return R / rows + E + 1; }
+template <typename T, int MODE, bool F32>
+static int lin_launch(const LinArgs& g, hipStream_t st) {
+    return lin_launch_tile<T, MODE, 128, 128, 2, 2, F32>(g, st);
+}
 
-static int dw_splits(int64_t R, int E, int n_in, int n_out) {
-    const int64_t tiles = (int64_t)E * ((n_in + 63) / 64) * ((n_out + 63) / 64);
-    int64_t s = (4 * (int64_t)num_cus() + tiles - 1) / tiles;
-    const int64_t most = R / ((int64_t)E * 256);
-    if (s > most) s = most;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// Rows per partial sum of dW: enough workgroups for all CUs (three of 128 x 128 tiles run on one) where the matrices alone
+// have too few tiles; 0: they have enough.
+static int dw_chunk(int64_t R, int E, int n_in, int n_out) {
+    const int64_t tiles = (int64_t)((n_in + 127) / 128) * ((n_out + 127) / 128), want = 3 * (int64_t)num_cus();
+    if (tiles * E >= want || R < 512) return 0;
+    int64_t chunk = R * tiles / want;
+    chunk = (chunk + LIN_BQ - 1) / LIN_BQ * LIN_BQ;
+    return (int)std::max<int64_t>(chunk, 4 * LIN_BQ);
 }
 
 }  // namespace nsx
@@ -322,20 +439,18 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
                           const void* weight, int n_in, int n_out, int E, const int32_t* offsets, int64_t R, int relu, void* y,
                           void* stream) {
     using namespace nsx;
-    const int rc = lin_check("nsx_expert_linear_fwd", dtype, n_in, n_out, E, R, top_k, offsets);
+    int rc = lin_check("nsx_expert_linear_fwd", dtype, n_in, n_out, E, R, top_k, offsets);
     if (rc != NSX_OK) return rc;
     if (R == 0) return NSX_OK;
-    NSX_REQUIRE(weight && y && (x || x_rows == 0) && aligned16(x) && aligned16(weight) && aligned16(y) && x_stride >= n_in && x_stride % 8 == 0,
+    NSX_REQUIRE(weight && y && (x || x_rows == 0) && aligned16(x) && aligned16(weight) && aligned16(y) && lin_stride(x_stride, n_in),
                 "nsx_expert_linear_fwd: NULL or unaligned pointer or row stride %lld", (long long)x_stride);
     NSX_REQUIRE(x_rows >= 0 && x_rows <= NSX_MAX_EXPERT_ENTRIES && (rows || x_rows == R), "nsx_expert_linear_fwd: x has %lld rows", (long long)x_rows);
     LinArgs g{};
     g.p = weight; g.q = x; g.d = y; g.ldp = n_in; g.ldq = x_stride; g.ldd = n_out; g.p_expert = (int64_t)n_in * n_out;
     g.offsets = offsets; g.rows = rows; g.top_k = fast_div(top_k); g.E = E; g.R = (int)R; g.x_rows = (int)x_rows;
-    g.M = n_out; g.K = n_in; g.relu = relu; g.m_tiles = (n_out + 63) / 64;
-    const int64_t blocks = row_tiles(R, E, 64) * g.m_tiles;
-    NSX_REQUIRE(blocks <= 0x7fffffff, "nsx_expert_linear_fwd: %lld tiles", (long long)blocks);
-    if (dtype == NSX_DTYPE_F16) lin_launch<half_t, LIN_FWD, 64, 64, 2, 2, false>(g, blocks, (hipStream_t)stream);
-    else lin_launch<bf16_t, LIN_FWD, 64, 64, 2, 2, false>(g, blocks, (hipStream_t)stream);
+    g.M = n_out; g.K = n_in; g.relu = relu;
+    rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_FWD, false>(g, (hipStream_t)stream) : lin_launch<bf16_t, LIN_FWD, false>(g, (hipStream_t)stream);
+    if (rc != NSX_OK) return rc;
     NSX_LAUNCH_CHECK("nsx_expert_linear_fwd");
     return NSX_OK;
 }
@@ -343,20 +458,18 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
 int nsx_expert_linear_bwd_x(const void* dy, int dtype, int64_t dy_stride, const void* y, int64_t y_stride, const void* weight,
                             int n_in, int n_out, int E, const int32_t* offsets, int64_t R, void* dx, void* stream) {
     using namespace nsx;
-    const int rc = lin_check("nsx_expert_linear_bwd_x", dtype, n_in, n_out, E, R, 1, offsets);
+    int rc = lin_check("nsx_expert_linear_bwd_x", dtype, n_in, n_out, E, R, 1, offsets);
     if (rc != NSX_OK) return rc;
     if (R == 0) return NSX_OK;
-    NSX_REQUIRE(dy && weight && dx && aligned16(dy) && aligned16(y) && aligned16(weight) && aligned16(dx) && dy_stride >= n_out &&
-                    dy_stride % 8 == 0 && (!y || (y_stride >= n_out && y_stride % 8 == 0)),
+    NSX_REQUIRE(dy && weight && dx && aligned16(dy) && aligned16(y) && aligned16(weight) && aligned16(dx) && lin_stride(dy_stride, n_out) &&
+                    (!y || lin_stride(y_stride, n_out)),
                 "nsx_expert_linear_bwd_x: NULL or unaligned pointer or row stride");
     LinArgs g{};
     g.p = weight; g.q = dy; g.mask = y; g.d = dx; g.ldp = n_in; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in;
     g.p_expert = (int64_t)n_in * n_out; g.offsets = offsets; g.E = E; g.R = (int)R; g.x_rows = (int)R;
-    g.M = n_in; g.K = n_out; g.m_tiles = (n_in + 63) / 64;
-    const int64_t blocks = row_tiles(R, E, 64) * g.m_tiles;
-    NSX_REQUIRE(blocks <= 0x7fffffff, "nsx_expert_linear_bwd_x: %lld tiles", (long long)blocks);
-    if (dtype == NSX_DTYPE_F16) lin_launch<half_t, LIN_DX, 64, 64, 2, 2, false>(g, blocks, (hipStream_t)stream);
-    else lin_launch<bf16_t, LIN_DX, 64, 64, 2, 2, false>(g, blocks, (hipStream_t)stream);
+    g.M = n_in; g.K = n_out;
+    rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(g, (hipStream_t)stream) : lin_launch<bf16_t, LIN_DX, false>(g, (hipStream_t)stream);
+    if (rc != NSX_OK) return rc;
     NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_x");
     return NSX_OK;
 }
@@ -366,44 +479,37 @@ int64_t nsx_expert_linear_bwd_w_workspace(int64_t R, int E, int n_in, int n_out)
     int32_t some = 0;
     const int rc = lin_check("nsx_expert_linear_bwd_w_workspace", NSX_DTYPE_F16, n_in, n_out, E, R, 1, &some);
     if (rc != NSX_OK) return rc;
-    const int s = dw_splits(R, E, n_in, n_out);
-    return s > 1 ? (int64_t)s * E * n_in * n_out * 4 : 0;
+    const int chunk = dw_chunk(R, E, n_in, n_out);
+    return chunk > 0 ? (R / chunk + E) * n_in * n_out * 4 : 0;
 }
 
 int nsx_expert_linear_bwd_w(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, int top_k,
                             const void* dy, int64_t dy_stride, const void* y, int64_t y_stride, int n_in, int n_out, int E,
                             const int32_t* offsets, int64_t R, int dw_f32, void* dw, void* workspace, void* stream) {
     using namespace nsx;
-    const int rc = lin_check("nsx_expert_linear_bwd_w", dtype, n_in, n_out, E, R, top_k, offsets);
+    int rc = lin_check("nsx_expert_linear_bwd_w", dtype, n_in, n_out, E, R, top_k, offsets);
     if (rc != NSX_OK) return rc;
-    NSX_REQUIRE(dw && aligned16(dw) && (R == 0 || dy) && (x || x_rows == 0) && aligned16(x) && aligned16(dy) && aligned16(y) && x_stride >= n_in &&
-                    x_stride % 8 == 0 && dy_stride >= n_out && dy_stride % 8 == 0 && (!y || (y_stride >= n_out && y_stride % 8 == 0)),
+    NSX_REQUIRE(dw && aligned16(dw) && (R == 0 || dy) && (x || x_rows == 0) && aligned16(x) && aligned16(dy) && aligned16(y) &&
+                    lin_stride(x_stride, n_in) && lin_stride(dy_stride, n_out) && (!y || lin_stride(y_stride, n_out)),
                 "nsx_expert_linear_bwd_w: NULL or unaligned pointer or row stride");
     NSX_REQUIRE(x_rows >= 0 && x_rows <= NSX_MAX_EXPERT_ENTRIES && (rows || x_rows == R), "nsx_expert_linear_bwd_w: x has %lld rows", (long long)x_rows);
     LinArgs g{};
-    g.splits = dw_splits(R, E, n_in, n_out);
-    NSX_REQUIRE(g.splits == 1 || (workspace && aligned16(workspace)), "nsx_expert_linear_bwd_w: no workspace");
+    g.chunk = dw_chunk(R, E, n_in, n_out);
+    NSX_REQUIRE(g.chunk == 0 || (workspace && aligned16(workspace)), "nsx_expert_linear_bwd_w: no workspace");
     g.p = x; g.q = dy; g.mask = y; g.d = dw; g.ldp = x_stride; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in;
     g.d_expert = (int64_t)n_in * n_out; g.offsets = offsets; g.rows = rows; g.top_k = fast_div(top_k); g.E = E; g.R = (int)R;
-    g.x_rows = (int)x_rows; g.M = n_in; g.C = n_out; g.m_tiles = (n_in + 63) / 64; g.c_tiles = (n_out + 63) / 64;
-    g.partial = (float*)workspace;
-    const int64_t blocks = (int64_t)E * g.m_tiles * g.c_tiles * g.splits, n = (int64_t)E * n_in * n_out;
-    NSX_REQUIRE(blocks <= 0x7fffffff, "nsx_expert_linear_bwd_w: %lld tiles", (long long)blocks);
+    g.x_rows = (int)x_rows; g.M = n_in; g.C = n_out; g.partial = (float*)workspace;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == NSX_DTYPE_F16) {
-        if (dw_f32) lin_launch<half_t, LIN_DW, 64, 64, 2, 2, true>(g, blocks, st);
-        else lin_launch<half_t, LIN_DW, 64, 64, 2, 2, false>(g, blocks, st);
-    } else {
-        if (dw_f32) lin_launch<bf16_t, LIN_DW, 64, 64, 2, 2, true>(g, blocks, st);
-        else lin_launch<bf16_t, LIN_DW, 64, 64, 2, 2, false>(g, blocks, st);
-    }
+    const bool f32 = dw_f32 || g.chunk > 0;
+    if (dtype == NSX_DTYPE_F16) rc = f32 ? lin_launch<half_t, LIN_DW, true>(g, st) : lin_launch<half_t, LIN_DW, false>(g, st);
+    else rc = f32 ? lin_launch<bf16_t, LIN_DW, true>(g, st) : lin_launch<bf16_t, LIN_DW, false>(g, st);
+    if (rc != NSX_OK) return rc;
     NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_w");
-    if (g.splits > 1) {
-        const int64_t need = (n / 4 + 255) / 256, most = (int64_t)num_cus() * 8;
-        const unsigned grid = (unsigned)(need < most ? need : most);
-        if (dw_f32) expert_sum_splits_kernel<float><<<grid, 256, 0, st>>>(g.partial, g.splits, n, (float*)dw);
-        else if (dtype == NSX_DTYPE_F16) expert_sum_splits_kernel<half_t><<<grid, 256, 0, st>>>(g.partial, g.splits, n, (half_t*)dw);
-        else expert_sum_splits_kernel<bf16_t><<<grid, 256, 0, st>>>(g.partial, g.splits, n, (bf16_t*)dw);
+    if (g.chunk > 0) {
+        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)n_in * n_out + 63) / 64, 4096), E);
+        if (dw_f32) expert_sum_chunks_kernel<float><<<grid, 256, 0, st>>>(g, (float*)dw);
+        else if (dtype == NSX_DTYPE_F16) expert_sum_chunks_kernel<half_t><<<grid, 256, 0, st>>>(g, (half_t*)dw);
+        else expert_sum_chunks_kernel<bf16_t><<<grid, 256, 0, st>>>(g, (bf16_t*)dw);
         NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_w");
     }
     return NSX_OK;

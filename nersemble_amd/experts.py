@@ -56,7 +56,7 @@ def _rows_of(t: torch.Tensor, align: int) -> Tuple[torch.Tensor, int]:
     ``align`` > 1), and that distance; copied where it is laid out otherwise."""
     n, w = t.shape
     s = t.stride(0) if n > 1 else -(-w // align) * align
-    if (w > 1 and t.stride(1) != 1) or s < w or s % align or (align > 1 and t.data_ptr() % 16):
+    if (w > 1 and t.stride(1) != 1) or s < w or s % align or (align > 1 and (t.data_ptr() % 16 or s > _lib.NSX_MAX_EXPERT_STRIDE)):
         t, s = t.contiguous(), w
         if align > 1 and t.data_ptr() % 16:
             t = t.clone()
