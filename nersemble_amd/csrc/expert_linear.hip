@@ -139,7 +139,7 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
     constexpr bool P_ALONG = MODE == LIN_FWD, Q_ALONG = MODE != LIN_DW;
     constexpr int NT = WM * WC * kWave, FM = TM / WM / 32, FC = TC / WC / 32, NP = TM * 8 / NT, NQ = TC * 8 / NT, RPT = NT / 8;
     constexpr uint32_t Q_AT = lin_rows(TM);
-    static_assert(NP % 4 == 0 && NQ % 4 == 0, "a thread turns 4 rows of q");
+    static_assert(NT >= 128 && (P_ALONG || NP % 4 == 0) && (Q_ALONG || NQ % 4 == 0), "a thread turns 4 rows of q");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wc = wave / WM;
     int e, a, b, m0, c0 = 0, chunk = 0;
     if (MODE == LIN_DW) {
@@ -416,20 +416,40 @@ static int lin_launch_tile(LinArgs g, hipStream_t st) {
     return NSX_OK;
 }
 
+// ---- which tile size ----------------------------------------------------------------------------------------------
+// Forward and dx, us by (rows x choices of experts, n_in -> n_out), bf16, 64 x 64 | 128 x 128 tiles:
+//   16384 x 2 of 16, 1024 -> 2048   339 | 177       4096 x 2 of 16, 1024 -> 1024    38 | 33       1024 x 2 of 16, 512 -> 512   9.5 | 11.0
+//   4 x 8 of 64, 1024 -> 1024      14.8 | 16.9      32 x 8 of 64, 1024 -> 1024    21.9 | 23.9     256 x 8 of 64, 1024 -> 1024 28.5 | 25.5
+//   262144 x 2 of 16, 32 -> 64     29.7 | 38.9      262144 x 2 of 16, 64 -> 16    26.3 | 35.1
+// The small tile where the result is no wider than it, where a segment has but a few rows, or where the large ones are fewer
+// than the CUs.
+static bool small_tiles(const LinArgs& g) {
+    const int64_t rows = g.R / 128 + std::min<int64_t>(g.E, g.R);
+    return g.M <= 64 || g.R < 16 * (int64_t)g.E || rows * ((g.M + 127) / 128) < num_cus();
+}
+// dW, chunk (0: none) and tile.  us with chunks of 256 | 512 | 1024 | 2048 rows:
+//   262144 x 2 of 16,  32 ->  64   64 x 64 tiles  75 | 63 | 63 | 70     128 x 128 tiles 174 | 143 | 135 | 143
+//    65536 x 2 of 16, 128 -> 128   64 x 64 tiles  47 | 43 | 45 | 67     128 x 128 tiles  70 |  59 |  63 |  67
+//    65536 x 2 of 16, 256 -> 256   64 x 64 tiles 119 | 84 | 82 | 85     128 x 128 tiles 164 | 109 | 104 | 114
+//     5003 x 3 of 23, 176 -> 136   64 x 64 tiles  25 | 28 | 35 | 40     128 x 128 tiles  31 |  31 |  42 |  46
+// Short chunks fill the card, long ones keep the partial sums small beside what is read: about two and a half workgroups per CU.
+// Without chunks (the matrices have tiles enough) the larger tiles are faster: 16384 x 2 of 16, 1024 -> 2048: 570 | 180.
+struct DwPlan { int chunk; bool small; };
+static DwPlan dw_plan(int64_t R, int E, int n_in, int n_out) {
+    const int64_t large = (int64_t)((n_in + 127) / 128) * ((n_out + 127) / 128), small = (int64_t)((n_in + 63) / 64) * ((n_out + 63) / 64);
+    if (large * E >= 2 * (int64_t)num_cus()) return {0, false};
+    if (small * E >= 4 * (int64_t)num_cus() || R < 8 * (int64_t)LIN_BQ) return {0, true};
+    int64_t chunk = R * small * 2 / (5 * (int64_t)num_cus());
+    chunk = (chunk + LIN_BQ - 1) / LIN_BQ * LIN_BQ;
+    return {(int)std::min<int64_t>(std::max<int64_t>(chunk, 4 * LIN_BQ), 1024), true};
+}
+
 template <typename T, int MODE, bool F32>
-static int lin_launch(const LinArgs& g, hipStream_t st) {
+static int lin_launch(const LinArgs& g, bool small, hipStream_t st) {
+    if (small) return lin_launch_tile<T, MODE, 64, 64, 1, 2, F32>(g, st);
     return lin_launch_tile<T, MODE, 128, 128, 2, 2, F32>(g, st);
 }
 
-// Rows per partial sum of dW: enough workgroups for all CUs (three of 128 x 128 tiles run on one) where the matrices alone
-// have too few tiles; 0: they have enough.
-static int dw_chunk(int64_t R, int E, int n_in, int n_out) {
-    const int64_t tiles = (int64_t)((n_in + 127) / 128) * ((n_out + 127) / 128), want = 3 * (int64_t)num_cus();
-    if (tiles * E >= want || R < 512) return 0;
-    int64_t chunk = R * tiles / want;
-    chunk = (chunk + LIN_BQ - 1) / LIN_BQ * LIN_BQ;
-    return (int)std::max<int64_t>(chunk, 4 * LIN_BQ);
-}
 
 }  // namespace nsx
 
@@ -449,7 +469,8 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
     g.p = weight; g.q = x; g.d = y; g.ldp = n_in; g.ldq = x_stride; g.ldd = n_out; g.p_expert = (int64_t)n_in * n_out;
     g.offsets = offsets; g.rows = rows; g.top_k = fast_div(top_k); g.E = E; g.R = (int)R; g.x_rows = (int)x_rows;
     g.M = n_out; g.K = n_in; g.relu = relu;
-    rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_FWD, false>(g, (hipStream_t)stream) : lin_launch<bf16_t, LIN_FWD, false>(g, (hipStream_t)stream);
+    rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_FWD, false>(g, small_tiles(g), (hipStream_t)stream)
+                                 : lin_launch<bf16_t, LIN_FWD, false>(g, small_tiles(g), (hipStream_t)stream);
     if (rc != NSX_OK) return rc;
     NSX_LAUNCH_CHECK("nsx_expert_linear_fwd");
     return NSX_OK;
@@ -468,7 +489,8 @@ int nsx_expert_linear_bwd_x(const void* dy, int dtype, int64_t dy_stride, const 
     g.p = weight; g.q = dy; g.mask = y; g.d = dx; g.ldp = n_in; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in;
     g.p_expert = (int64_t)n_in * n_out; g.offsets = offsets; g.E = E; g.R = (int)R; g.x_rows = (int)R;
     g.M = n_in; g.K = n_out;
-    rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(g, (hipStream_t)stream) : lin_launch<bf16_t, LIN_DX, false>(g, (hipStream_t)stream);
+    rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(g, small_tiles(g), (hipStream_t)stream)
+                                 : lin_launch<bf16_t, LIN_DX, false>(g, small_tiles(g), (hipStream_t)stream);
     if (rc != NSX_OK) return rc;
     NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_x");
     return NSX_OK;
@@ -479,7 +501,7 @@ int64_t nsx_expert_linear_bwd_w_workspace(int64_t R, int E, int n_in, int n_out)
     int32_t some = 0;
     const int rc = lin_check("nsx_expert_linear_bwd_w_workspace", NSX_DTYPE_F16, n_in, n_out, E, R, 1, &some);
     if (rc != NSX_OK) return rc;
-    const int chunk = dw_chunk(R, E, n_in, n_out);
+    const int chunk = dw_plan(R, E, n_in, n_out).chunk;
     return chunk > 0 ? (R / chunk + E) * n_in * n_out * 4 : 0;
 }
 
@@ -494,15 +516,16 @@ int nsx_expert_linear_bwd_w(const void* x, int dtype, int64_t x_stride, int64_t 
                 "nsx_expert_linear_bwd_w: NULL or unaligned pointer or row stride");
     NSX_REQUIRE(x_rows >= 0 && x_rows <= NSX_MAX_EXPERT_ENTRIES && (rows || x_rows == R), "nsx_expert_linear_bwd_w: x has %lld rows", (long long)x_rows);
     LinArgs g{};
-    g.chunk = dw_chunk(R, E, n_in, n_out);
+    const DwPlan how = dw_plan(R, E, n_in, n_out);
+    g.chunk = how.chunk;
     NSX_REQUIRE(g.chunk == 0 || (workspace && aligned16(workspace)), "nsx_expert_linear_bwd_w: no workspace");
     g.p = x; g.q = dy; g.mask = y; g.d = dw; g.ldp = x_stride; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in;
     g.d_expert = (int64_t)n_in * n_out; g.offsets = offsets; g.rows = rows; g.top_k = fast_div(top_k); g.E = E; g.R = (int)R;
     g.x_rows = (int)x_rows; g.M = n_in; g.C = n_out; g.partial = (float*)workspace;
     hipStream_t st = (hipStream_t)stream;
     const bool f32 = dw_f32 || g.chunk > 0;
-    if (dtype == NSX_DTYPE_F16) rc = f32 ? lin_launch<half_t, LIN_DW, true>(g, st) : lin_launch<half_t, LIN_DW, false>(g, st);
-    else rc = f32 ? lin_launch<bf16_t, LIN_DW, true>(g, st) : lin_launch<bf16_t, LIN_DW, false>(g, st);
+    if (dtype == NSX_DTYPE_F16) rc = f32 ? lin_launch<half_t, LIN_DW, true>(g, how.small, st) : lin_launch<half_t, LIN_DW, false>(g, how.small, st);
+    else rc = f32 ? lin_launch<bf16_t, LIN_DW, true>(g, how.small, st) : lin_launch<bf16_t, LIN_DW, false>(g, how.small, st);
     if (rc != NSX_OK) return rc;
     NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_w");
     if (g.chunk > 0) {

@@ -11,50 +11,48 @@ module built on these calls.)  All four launch on torch's current stream, keep n
 ``_lib.device_count`` rows behind the device-side count are not routed, and not written by ``route_experts`` and
 ``expert_combine``.  A plan's numbers are bounded inside the kernels; equal inputs give equal bits.
 """
-import ctypes as C
-from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, lib, ndev, ptr, stream
+from ._lib import check, lib, ndev, ptr
 
+# (What is small here runs on the host in the time of one such call -- 10 to 40 us -- so the wrappers below read every tensor
+# property once, hand plain integers to the library and take the fast way where nothing has to be copied.)
 _DTYPE = {torch.float32: _lib.NSX_DTYPE_F32, torch.float16: _lib.NSX_DTYPE_F16, torch.bfloat16: _lib.NSX_DTYPE_BF16}
 _SCORES = {"softmax": 0, "sigmoid": 1}
+_F32, _I32 = torch.float32, torch.int32
+_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-@dataclass(frozen=True)
 class ExpertPlan:
     """Entries (row * top_k + choice) ordered by expert (``expert_plan``): int32 device tensors.
 
     offsets [E + 1]: the ordered rows of expert e are offsets[e] .. offsets[e + 1]; rows [T * top_k]: entry of every ordered
     row, -1 behind the last segment; positions [T, top_k]: ordered row of every entry, -1 for an entry that is not routed."""
-    offsets: torch.Tensor
-    rows: torch.Tensor
-    positions: torch.Tensor
+    __slots__ = ("offsets", "rows", "positions", "n_experts", "n_rows", "top_k", "n_entries")
 
-    @property
-    def n_experts(self) -> int:
-        return self.offsets.shape[0] - 1
-
-    @property
-    def top_k(self) -> int:
-        return self.positions.shape[1]
-
-
-def _plan_check(plan: ExpertPlan, what: str) -> None:
-    o, r, p = plan.offsets, plan.rows, plan.positions
-    if o.dim() != 1 or o.shape[0] < 2 or r.dim() != 1 or p.dim() != 2 or p.numel() != r.shape[0]:
-        raise RuntimeError(f"{what}: the plan's offsets [E + 1], rows [T * top_k], positions [T, top_k] have shapes "
-                           f"{tuple(o.shape)}, {tuple(r.shape)}, {tuple(p.shape)}")
+    def __init__(self, offsets: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor):
+        o, r, p = offsets.shape, rows.shape, positions.shape
+        if len(o) != 1 or o[0] < 2 or len(r) != 1 or len(p) != 2 or p[0] * p[1] != r[0] \
+                or not offsets.dtype == rows.dtype == positions.dtype == _I32:
+            raise RuntimeError(f"ExpertPlan: offsets [E + 1], rows [T * top_k] and positions [T, top_k] are int32 (got {tuple(o)} "
+                               f"{offsets.dtype}, {tuple(r)} {rows.dtype}, {tuple(p)} {positions.dtype})")
+        if not (offsets.is_contiguous() and rows.is_contiguous() and positions.is_contiguous()):
+            offsets, rows, positions = offsets.contiguous(), rows.contiguous(), positions.contiguous()
+        self.offsets, self.rows, self.positions = offsets, rows, positions
+        self.n_experts, self.n_entries = o[0] - 1, r[0]
+        self.n_rows, self.top_k = p
 
 
 def _rows_of(t: torch.Tensor, align: int) -> Tuple[torch.Tensor, int]:
     """``t`` as rows of consecutive values whose distance is a multiple of ``align`` elements (and which start on 16 bytes if
     ``align`` > 1), and that distance; copied where it is laid out otherwise."""
     n, w = t.shape
+    if t.is_contiguous() and w % align == 0 and (align == 1 or t.data_ptr() % 16 == 0):
+        return t, w
     s = t.stride(0) if n > 1 else -(-w // align) * align
     if (w > 1 and t.stride(1) != 1) or s < w or s % align or (align > 1 and (t.data_ptr() % 16 or s > _lib.NSX_MAX_EXPERT_STRIDE)):
         t, s = t.contiguous(), w
@@ -63,51 +61,69 @@ def _rows_of(t: torch.Tensor, align: int) -> Tuple[torch.Tensor, int]:
     return t, s
 
 
-def _at(t: torch.Tensor) -> C.c_void_p:
-    """``ptr`` for rows that need not lie next to each other."""
-    if t.is_contiguous():
-        return ptr(t)
-    ptr(t[:1, :1])                   # (device checks)
-    return C.c_void_p(t.data_ptr())
+def _here(t: torch.Tensor) -> int:
+    """The current device, which has to be ``t``'s."""
+    d = t.get_device()
+    if d < 0 or d != _device():
+        ptr(t)
+    return d
+
+
+def _at(t: torch.Tensor, dev: int) -> int:
+    """Address of a tensor of the current device (``ptr`` says what is wrong with any other)."""
+    if t.get_device() != dev:
+        ptr(t)
+    return t.data_ptr()
 
 
 # ------------------------------------------------------------------------------------------------
 # choice
 # ------------------------------------------------------------------------------------------------
-def _route(logits, stride, bias, selector, top_k, sigmoid, n_groups, top_groups, group_top, renorm, scale):
-    T, E = logits.shape
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
-    chosen = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
-    check(lib().nsx_expert_route_fwd(_at(logits), _DTYPE[logits.dtype], T, E, stride, ptr(bias, torch.float32),
-                                     ptr(selector, torch.uint8), top_k, sigmoid, n_groups, top_groups, group_top, renorm, scale,
-                                     ptr(weights), ptr(chosen), ndev(T), stream()), "nsx_expert_route_fwd")
+def _route(x, stride, bias, selector, top_k, sigmoid, n_groups, top_groups, group_top, renorm, scale):
+    T, E = x.shape
+    dev = _here(x)
+    weights = x.new_empty((T, top_k), dtype=_F32)
+    chosen = x.new_empty((T, top_k), dtype=_I32)
+    check(lib().nsx_expert_route_fwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, None if bias is None else _at(bias, dev),
+                                     None if selector is None else _at(selector, dev), top_k, sigmoid, n_groups, top_groups, group_top,
+                                     renorm, scale, weights.data_ptr(), chosen.data_ptr(), ndev(T), _raw_stream(dev)),
+          "nsx_expert_route_fwd")
     return weights, chosen
+
+
+def _route_bwd(ctx, g, _):
+    if g is None:
+        return None, None, None, None
+    x, weights, chosen = ctx.saved_tensors
+    stride, top_k, sigmoid, renorm, scale = ctx.cfg
+    T, E = x.shape
+    if g.dtype != _F32 or not g.is_contiguous():
+        g = g.to(_F32).contiguous()
+    dev = _here(x)
+    d = torch.empty((T, E), dtype=x.dtype, device=x.device)
+    check(lib().nsx_expert_route_bwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, top_k, sigmoid, renorm, scale, weights.data_ptr(),
+                                     chosen.data_ptr(), _at(g, dev), d.data_ptr(), ndev(T), _raw_stream(dev)),
+          "nsx_expert_route_bwd")
+    return d, None, None, None
 
 
 class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, selector, cfg):
-        x, stride = _rows_of(logits.detach(), 1)
+        x, stride = _rows_of(logits, 1)
         weights, chosen = _route(x, stride, bias, selector, *cfg)
         ctx.save_for_backward(x, weights, chosen)
-        ctx.cfg, ctx.stride = cfg, stride
+        ctx.cfg = (stride, cfg[0], cfg[1], cfg[5], cfg[6])
         ctx.mark_non_differentiable(chosen)
         ctx.set_materialize_grads(False)
         return weights, chosen
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, _):
-        if g is None:
-            return None, None, None, None
-        x, weights, chosen = ctx.saved_tensors
-        top_k, sigmoid, _, _, _, renorm, scale = ctx.cfg
-        T, E = x.shape
-        g = g.to(torch.float32).contiguous()
-        d = torch.empty((T, E), dtype=x.dtype, device=x.device)
-        check(lib().nsx_expert_route_bwd(_at(x), _DTYPE[x.dtype], T, E, ctx.stride, top_k, sigmoid, renorm, scale, ptr(weights),
-                                         ptr(chosen), ptr(g), ptr(d), ndev(T), stream()), "nsx_expert_route_bwd")
-        return d, None, None, None
+        return (_route_bwd_once if torch.is_grad_enabled() else _route_bwd)(ctx, g, _)
+
+
+_route_bwd_once = once_differentiable(_route_bwd)        # (under create_graph: a second differentiation raises)
 
 
 def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -128,20 +144,22 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
         raise RuntimeError(f"route_experts: scores are 'softmax' or 'sigmoid' (got {scores!r})")
     T, E = logits.shape
     if bias is not None:
-        if bias.shape != (E,):
-            raise RuntimeError(f"route_experts: bias has shape {tuple(bias.shape)}, not ({E},)")
+        if bias.shape != (E,) or bias.dtype != _F32:
+            raise RuntimeError(f"route_experts: bias is {tuple(bias.shape)} {bias.dtype}, not ({E},) fp32")
         bias = bias.detach().contiguous()
     if selector is not None:
         if selector.numel() != T:
             raise RuntimeError(f"route_experts: selector has {selector.numel()} entries for {T} rows")
-        selector = selector.detach().reshape(-1).contiguous()
+        selector = selector.reshape(-1).contiguous()
         if selector.dtype == torch.bool:
             selector = selector.view(torch.uint8)
+        if selector.dtype != torch.uint8:
+            raise RuntimeError(f"route_experts: selector is uint8 or bool (got {selector.dtype})")
     cfg = (int(top_k), _SCORES[scores], int(n_groups), int(n_groups if top_groups is None else top_groups), int(group_top),
            int(bool(renormalise)), float(scale))
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteFn.apply(logits, bias, selector, cfg)
-    x, stride = _rows_of(logits.detach(), 1)
+    x, stride = _rows_of(logits, 1)
     return _route(x, stride, bias, selector, *cfg)
 
 
@@ -161,11 +179,12 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
         check(need, "nsx_expert_plan_workspace")
     # one allocation: offsets | rows | positions | workspace (16-byte steps)
     o, r = -(-(n_experts + 1) // 4) * 4, -(-(T * k) // 4) * 4
-    buf = torch.empty((o + 2 * r + need // 4,), dtype=torch.int32, device=dev)
-    plan = ExpertPlan(buf[:n_experts + 1], buf[o:o + T * k], buf[o + r:o + r + T * k].view(T, k))
-    check(lib().nsx_expert_plan(ptr(chosen), T, k, n_experts, ptr(plan.offsets), ptr(plan.rows), ptr(plan.positions),
-                                ptr(buf[o + 2 * r:]), ndev(T), stream()), "nsx_expert_plan")
-    return plan
+    dev = _here(chosen)
+    buf = chosen.new_empty((o + 2 * r + need // 4,))
+    base = buf.data_ptr()
+    check(lib().nsx_expert_plan(chosen.data_ptr(), T, k, n_experts, base, base + 4 * o, base + 4 * (o + r), base + 4 * (o + 2 * r), ndev(T),
+                                _raw_stream(dev)), "nsx_expert_plan")
+    return ExpertPlan(buf[:n_experts + 1], buf[o:o + T * k], buf[o + r:o + r + T * k].view(T, k))
 
 
 # ------------------------------------------------------------------------------------------------
@@ -173,53 +192,60 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
 # ------------------------------------------------------------------------------------------------
 def _linear(x, x_stride, w16, plan, gather, relu):
     E, N, K = w16.shape
-    R = plan.rows.shape[0]
-    y = torch.empty((R, N), dtype=x.dtype, device=x.device)
-    check(lib().nsx_expert_linear_fwd(_at(x), _DTYPE[x.dtype], x_stride, x.shape[0],
-                                      ptr(plan.rows, torch.int32) if gather else None, plan.top_k, ptr(w16), K, N, E,
-                                      ptr(plan.offsets, torch.int32), R, int(relu), ptr(y), stream()), "nsx_expert_linear_fwd")
+    dev = _here(x)
+    y = x.new_empty((plan.n_entries, N))
+    check(lib().nsx_expert_linear_fwd(x.data_ptr(), _DTYPE[x.dtype], x_stride, x.shape[0], _at(plan.rows, dev) if gather else None, plan.top_k,
+                                      _at(w16, dev), K, N, E, _at(plan.offsets, dev), plan.n_entries, relu, y.data_ptr(),
+                                      _raw_stream(dev)), "nsx_expert_linear_fwd")
     return y
+
+
+def _linear_bwd(ctx, dy):
+    x, w16, y, offsets, rows, positions = ctx.saved_tensors
+    x_stride, x_rows, (E, N, K), gather, w_dtype, need_x, need_w = ctx.cfg
+    R, top_k = rows.shape[0], positions.shape[1]
+    g, g_stride = _rows_of(dy, 8)
+    dev, code, L = _here(g), _DTYPE[g.dtype], lib()
+    stream = _raw_stream(dev)
+    g_at, o_at, y_at = g.data_ptr(), _at(offsets, dev), None if y is None else _at(y, dev)
+    dx = dw = None
+    if need_x:
+        dx = torch.empty((R, K), dtype=g.dtype, device=g.device)
+        check(L.nsx_expert_linear_bwd_x(g_at, code, g_stride, y_at, N, _at(w16, dev), K, N, E, o_at, R, dx.data_ptr(), stream),
+              "nsx_expert_linear_bwd_x")
+        if gather:
+            # a row's choices summed in 32 bits; their gradients lie in 16 bits between the two launches (twice the
+            # memory traffic otherwise): an error of at most half a step of each term beside the sum's own rounding
+            dx = _combine(dx, K, None, positions)
+    if need_w:
+        need = L.nsx_expert_linear_bwd_w_workspace(R, E, K, N)
+        if need < 0:
+            check(need, "nsx_expert_linear_bwd_w_workspace")
+        ws = torch.empty((need,), dtype=torch.uint8, device=g.device) if need else None
+        dw = torch.empty((E, N, K), dtype=w_dtype, device=g.device)
+        check(L.nsx_expert_linear_bwd_w(_at(x, dev), code, x_stride, x_rows, _at(rows, dev) if gather else None, top_k, g_at, g_stride,
+                                        y_at, N, K, N, E, o_at, R, w_dtype == _F32, dw.data_ptr(),
+                                        None if ws is None else ws.data_ptr(), stream), "nsx_expert_linear_bwd_w")
+    return dx, dw, None, None, None, None
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, w16, plan, gather, relu):
-        xr, x_stride = _rows_of(x.detach(), 8)
+        xr, x_stride = _rows_of(x, 8)
         y = _linear(xr, x_stride, w16, plan, gather, relu)
         need_x, need_w = ctx.needs_input_grad[:2]
         ctx.save_for_backward(xr if need_w else None, w16 if need_x else None, y if relu else None,
                               plan.offsets, plan.rows, plan.positions)
-        ctx.cfg = (x_stride, tuple(x.shape), tuple(w16.shape), gather, weight.dtype)
+        ctx.cfg = (x_stride, x.shape[0], w16.shape, gather, weight.dtype, need_x, need_w)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, w16, y, offsets, rows, positions = ctx.saved_tensors
-        x_stride, x_shape, (E, N, K), gather, w_dtype = ctx.cfg
-        plan = ExpertPlan(offsets, rows, positions)
-        R, code, dev = rows.shape[0], _DTYPE[dy.dtype], dy.device
-        g, g_stride = _rows_of(dy, 8)
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.empty((R, K), dtype=g.dtype, device=dev)
-            check(lib().nsx_expert_linear_bwd_x(_at(g), code, g_stride, ptr(y), N, ptr(w16), K, N, E, ptr(offsets), R, ptr(dx),
-                                                stream()), "nsx_expert_linear_bwd_x")
-            if gather:
-                # a row's choices summed in 32 bits; their gradients lie in 16 bits between the two launches (twice the
-                # memory traffic otherwise): an error of at most half a step of each term beside the sum's own rounding
-                dx = _combine(dx, K, None, positions)
-        if ctx.needs_input_grad[1]:
-            need = int(lib().nsx_expert_linear_bwd_w_workspace(R, E, K, N))
-            if need < 0:
-                check(need, "nsx_expert_linear_bwd_w_workspace")
-            ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-            dw = torch.empty((E, N, K), dtype=w_dtype, device=dev)
-            check(lib().nsx_expert_linear_bwd_w(_at(x), code, x_stride, x_shape[0], ptr(rows) if gather else None, plan.top_k,
-                                                _at(g), g_stride, ptr(y), N, K, N, E, ptr(offsets), R,
-                                                int(w_dtype == torch.float32), ptr(dw), ptr(ws), stream()),
-                  "nsx_expert_linear_bwd_w")
-        return dx, dw, None, None, None, None
+        return (_linear_bwd_once if torch.is_grad_enabled() else _linear_bwd)(ctx, dy)
+
+
+_linear_bwd_once = once_differentiable(_linear_bwd)
 
 
 def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gather: bool = True, relu: bool = False,
@@ -230,27 +256,28 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gathe
     x: fp16 or bf16, [T, n_in] rows (``gather``) or [T * top_k, n_in] in the plan's order.  weight [E, n_out, n_in]: of x's
     dtype, or fp32 parameters whose copy in x's dtype is ``w16`` (made here if it is not given); the gradient has the dtype of
     ``weight``.  n_in and n_out are multiples of 8."""
-    _plan_check(plan, "expert_linear")
-    if x.dim() != 2 or x.dtype not in (torch.float16, torch.bfloat16):
-        raise RuntimeError(f"expert_linear: x is [rows, n_in] in fp16 or bf16 (got {tuple(x.shape)} {x.dtype})")
-    if weight.dim() != 3 or weight.dtype not in (x.dtype, torch.float32):
-        raise RuntimeError(f"expert_linear: weight is [E, n_out, n_in] in {x.dtype} or fp32 (got {tuple(weight.shape)} {weight.dtype})")
-    E, N, K = weight.shape
-    if E != plan.n_experts or x.shape[1] != K:
-        raise RuntimeError(f"expert_linear: weight {tuple(weight.shape)} for rows of {x.shape[1]} and a plan of {plan.n_experts} experts")
-    if x.shape[0] != (plan.positions.shape[0] if gather else plan.rows.shape[0]):
-        raise RuntimeError(f"expert_linear: x has {x.shape[0]} rows for a plan of {tuple(plan.positions.shape)} entries "
-                           f"(gather={bool(gather)})")
+    xs, ws, xt, wt = x.shape, weight.shape, x.dtype, weight.dtype
+    if len(xs) != 2 or xt not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"expert_linear: x is [rows, n_in] in fp16 or bf16 (got {tuple(xs)} {xt})")
+    if len(ws) != 3 or (wt != xt and wt != _F32):
+        raise RuntimeError(f"expert_linear: weight is [E, n_out, n_in] in {xt} or fp32 (got {tuple(ws)} {wt})")
+    if ws[0] != plan.n_experts or xs[1] != ws[2]:
+        raise RuntimeError(f"expert_linear: weight {tuple(ws)} for rows of {xs[1]} and a plan of {plan.n_experts} experts")
+    if xs[0] != (plan.n_rows if gather else plan.n_entries):
+        raise RuntimeError(f"expert_linear: x has {xs[0]} rows for a plan of {plan.n_rows} x {plan.top_k} entries (gather={bool(gather)})")
     if w16 is None:
-        w16 = weight.detach() if weight.dtype == x.dtype else weight.detach().to(x.dtype)
-    elif w16.shape != weight.shape or w16.dtype != x.dtype:
-        raise RuntimeError(f"expert_linear: w16 is {tuple(w16.shape)} {w16.dtype}, not {tuple(weight.shape)} {x.dtype}")
-    w16 = w16.detach().contiguous()
+        w16 = weight.detach() if wt == xt else weight.detach().to(xt)
+    elif w16.shape != ws or w16.dtype != xt:
+        raise RuntimeError(f"expert_linear: w16 is {tuple(w16.shape)} {w16.dtype}, not {tuple(ws)} {xt}")
+    else:
+        w16 = w16.detach()
+    if not w16.is_contiguous():
+        w16 = w16.contiguous()
     if w16.data_ptr() % 16:
         w16 = w16.clone()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _LinearFn.apply(x, weight, w16, plan, bool(gather), bool(relu))
-    xr, x_stride = _rows_of(x.detach(), 8)
+    xr, x_stride = _rows_of(x, 8)
     return _linear(xr, x_stride, w16, plan, bool(gather), bool(relu))
 
 
@@ -259,46 +286,58 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gathe
 # ------------------------------------------------------------------------------------------------
 def _combine(y, y_stride, weights, positions):
     T, k = positions.shape
-    out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
-    check(lib().nsx_expert_combine_fwd(_at(y), _DTYPE[y.dtype], y_stride, y.shape[0], y.shape[1], ptr(weights),
-                                       ptr(positions, torch.int32), T, k, ptr(out), ndev(T), stream()), "nsx_expert_combine_fwd")
+    R, n = y.shape
+    dev = _here(y)
+    out = y.new_empty((T, n))
+    check(lib().nsx_expert_combine_fwd(y.data_ptr(), _DTYPE[y.dtype], y_stride, R, n, None if weights is None else _at(weights, dev),
+                                       _at(positions, dev), T, k, out.data_ptr(), ndev(T), _raw_stream(dev)), "nsx_expert_combine_fwd")
     return out
+
+
+def _combine_bwd(ctx, dout):
+    y, w, offsets, positions = ctx.saved_tensors
+    stride, w_dtype = ctx.cfg
+    T, k = positions.shape
+    R, n = y.shape
+    if not dout.is_contiguous():
+        dout = dout.contiguous()
+    if dout.data_ptr() % 16:
+        dout = dout.clone()
+    dev = _here(y)
+    dy = torch.empty((R, n), dtype=y.dtype, device=y.device)
+    dw = torch.empty((T, k), dtype=_F32, device=y.device)
+    check(lib().nsx_expert_combine_bwd(y.data_ptr(), _DTYPE[y.dtype], stride, R, n, _at(w, dev), _at(positions, dev),
+                                       _at(offsets, dev) + 4 * (offsets.shape[0] - 1), T, k, _at(dout, dev), dy.data_ptr(),
+                                       dw.data_ptr(), ndev(T), _raw_stream(dev)), "nsx_expert_combine_bwd")
+    return dy, dw if w_dtype == _F32 else dw.to(w_dtype), None
 
 
 class _CombineFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, plan):
-        yr, stride = _rows_of(y.detach(), 8)
-        w = weights.detach().to(torch.float32).contiguous()
+        yr, stride = _rows_of(y, 8)
+        w = weights if weights.dtype == _F32 and weights.is_contiguous() else weights.to(_F32).contiguous()
         ctx.save_for_backward(yr, w, plan.offsets, plan.positions)
-        ctx.stride, ctx.w_dtype = stride, weights.dtype
+        ctx.cfg = (stride, weights.dtype)
         return _combine(yr, stride, w, plan.positions)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        y, w, offsets, positions = ctx.saved_tensors
-        T, k = positions.shape
-        R, n = y.shape
-        dout = dout.contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
-        dy = torch.empty((R, n), dtype=y.dtype, device=y.device)
-        dw = torch.empty((T, k), dtype=torch.float32, device=y.device)
-        check(lib().nsx_expert_combine_bwd(_at(y), _DTYPE[y.dtype], ctx.stride, R, n, ptr(w), ptr(positions), ptr(offsets[-1:]), T, k,
-                                           ptr(dout), ptr(dy), ptr(dw), ndev(T), stream()), "nsx_expert_combine_bwd")
-        return dy, dw.to(ctx.w_dtype), None
+        return (_combine_bwd_once if torch.is_grad_enabled() else _combine_bwd)(ctx, dout)
+
+
+_combine_bwd_once = once_differentiable(_combine_bwd)
 
 
 def expert_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """[T, n]: sum over a row's choices of ``weights[t, j] * y[plan.positions[t, j]]``, differentiable w.r.t. ``y`` [T * top_k,
     n] (fp16 or bf16, n a multiple of 8) and ``weights`` [T, top_k]; choices that are not routed count nothing."""
-    _plan_check(plan, "expert_combine")
-    if y.dim() != 2 or y.dtype not in (torch.float16, torch.bfloat16) or y.shape[0] != plan.rows.shape[0]:
-        raise RuntimeError(f"expert_combine: y is [{plan.rows.shape[0]}, n] in fp16 or bf16 (got {tuple(y.shape)} {y.dtype})")
+    ys = y.shape
+    if len(ys) != 2 or ys[0] != plan.n_entries or y.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"expert_combine: y is [{plan.n_entries}, n] in fp16 or bf16 (got {tuple(ys)} {y.dtype})")
     if weights.shape != plan.positions.shape or not weights.is_floating_point():
         raise RuntimeError(f"expert_combine: weights are {tuple(plan.positions.shape)} (got {tuple(weights.shape)} {weights.dtype})")
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
         return _CombineFn.apply(y, weights, plan)
-    yr, stride = _rows_of(y.detach(), 8)
-    return _combine(yr, stride, weights.detach().to(torch.float32).contiguous(), plan.positions)
+    yr, stride = _rows_of(y, 8)
+    return _combine(yr, stride, weights.to(_F32).contiguous(), plan.positions)
