@@ -7,13 +7,16 @@
 // choice; w_j = scale * s_j / sum_i s_i (renormalised) or scale * s_j.
 //   * Without a bias (and with groups that count for their largest c) the order of c IS the order of x: the logits are
 //     compared as they are and no score is formed for experts that are not chosen.
-//   * Otherwise c is formed in 64 bits: two experts whose 32-bit sums round to the same value, or change places, would make
-//     the choice depend on the order of the summation behind the softmax.
+//   * Otherwise the choice is that of c in 64 bits: two experts whose 32-bit sums round to the same value, or change places,
+//     would make it depend on the order of the summation behind the softmax.  c is formed in 32 bits; only where neighbours in
+//     the order lie closer than its error is the wave's part done again in 64.
 //   * Renormalised weights are ratios: of the softmax only exp(x_j - max over the chosen) is left, of the sigmoid
 //     exp(x_j - min(max, 0)) / (1 + exp(x_j)) -- neither underflows where all chosen scores are tiny.
-// A row is held by L lanes of a wave, V consecutive experts in each (64 / L rows per wave): a row is read once, 16 bytes per
-// lane, and the k rounds of "largest value, lowest index" are log2(L) exchanges each.
+// A row is held by L lanes of a wave, V consecutive experts in each (64 / L rows per wave): a row is read once, 16 or 32 bytes
+// per lane.  A round of "largest value, lowest index" is log2(L) exchanges of the value within the lanes (DPP), a ballot of the
+// lanes that hold it, and the first of them takes its expert out.
 #include "expert_common.h"
+#include <algorithm>
 
 namespace nsx {
 
@@ -23,6 +26,7 @@ struct RouteArgs {
     int k, G, top_groups, group_top, sigmoid, renorm; float scale;
     float* w; int32_t* idx; const int64_t* n_dev;
     int lg_L, lg_Lg;                 // lanes per row and per group of it, as powers of two
+    FastDiv by_k;
 };
 
 constexpr int ROUTE_WAVES = 4;
@@ -30,7 +34,7 @@ constexpr int ROUTE_WAVES = 4;
 template <typename T, int V, bool VEC>
 __device__ __forceinline__ void load_logits(const T* __restrict__ p, int n, float (&x)[V]) {
     if (VEC) {
-        struct alignas(sizeof(T) * V) Pack { T v[V]; };
+        struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack { T v[V]; };
         if (n > 0) {
             const Pack q = *reinterpret_cast<const Pack*>(p);
 #pragma unroll
@@ -45,18 +49,29 @@ __device__ __forceinline__ void load_logits(const T* __restrict__ p, int n, floa
     }
 }
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-
-template <typename K>
-__device__ __forceinline__ K row_max(K v, int L) {
-    for (int o = 1; o < L; o <<= 1) { const K u = __shfl_xor(v, o); v = u > v ? u : v; }
+// ---- exchanges within the 2^n lanes of a row ----
+template <int CTRL> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+template <int CTRL> __device__ __forceinline__ float dpp(float v) { return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(int, v))); }
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+    const u32x2 b = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(double, u32x2{(uint32_t)dpp<CTRL>((int)b[0]), (uint32_t)dpp<CTRL>((int)b[1])});
+}
+struct TakeMax { template <typename K> __device__ __forceinline__ K operator()(K a, K b) const { return a > b ? a : b; } };
+struct TakeSum { template <typename K> __device__ __forceinline__ K operator()(K a, K b) const { return a + b; } };
+// every lane of a row gets the same bits (the operations commute); L is the same for all: the branches are scalar
+template <class Op, typename K>
+__device__ __forceinline__ K row_all(K v, int L) {
+    const Op op;
+    if (L > 1) v = op(v, dpp<0xB1>(v));           // quad_perm 1 0 3 2
+    if (L > 2) v = op(v, dpp<0x4E>(v));           // quad_perm 2 3 0 1
+    if (L > 4) v = op(v, dpp<0x141>(v));          // row_half_mirror: the other quad
+    if (L > 8) v = op(v, dpp<0x140>(v));          // row_mirror: the other half of 16
+    if (L > 16) v = op(v, __shfl_xor(v, 16));
+    if (L > 32) v = op(v, __shfl_xor(v, 32));
     return v;
 }
-template <typename K>
-__device__ __forceinline__ K row_sum(K v, int L) {
-    for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
-    return v;
+__device__ __forceinline__ uint64_t row_lanes(uint64_t mask, int r, int lg_L) {
+    return (mask >> (r << lg_L)) & (lg_L == 6 ? ~0ull : ((1ull << (1 << lg_L)) - 1));
 }
 
 // s / (what the renormalisation divides out): see the head of the file; m = 0 keeps s itself
@@ -64,9 +79,78 @@ __device__ __forceinline__ float sigmoid_over(float x, float m) {
     return x <= 0.f ? expf(x - m) / (1.f + expf(x)) : 1.f / (1.f + expf(-x));
 }
 
-template <typename T, typename K, int V, bool VEC>
+// One pass of the choice over the wave's rows: values c (taken from it as they are chosen) -> entries of `out`, k + 1 of them
+// if `more` (the one that just missed).  out: per row top_k + 1 of {value, logit, expert}.
+template <typename K> struct Chosen { K c; float x; int32_t e; };
+template <typename K, int V>
+__device__ __forceinline__ void choose(const RouteArgs& a, K (&c)[V], const float (&x)[V], int e0, int r, int sub, int rounds,
+                                       Chosen<K>* __restrict__ out) {
+    const int L = 1 << a.lg_L;
+    for (int j = 0; j < rounds; ++j) {
+        K best = c[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = c[i] > best ? c[i] : best;
+        const K top = row_all<TakeMax>(best, L);
+        const uint64_t holders = row_lanes(__ballot(best == top), r, a.lg_L);
+        if (__ffsll((unsigned long long)holders) - 1 == sub) {
+            int at = V - 1;
+#pragma unroll
+            for (int i = V - 2; i >= 0; --i) at = c[i] == top ? i : at;
+            float xv = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                xv = i == at ? x[i] : xv;
+                c[i] = i == at ? (K)-INFINITY : c[i];
+            }
+            out[j] = Chosen<K>{top, xv, top > (K)-INFINITY ? e0 + at : -1};
+        }
+    }
+    wave_lds_fence();
+}
+
+// groups that stay: the values of the others become -inf.  Returns the distance between the last group that stays and the first
+// that does not, and the former's value.
+template <typename K, int V>
+__device__ __forceinline__ K keep_groups(const RouteArgs& a, K (&c)[V], int r, int g, K& lowest) {
+    K b1 = (K)-INFINITY, b2 = (K)-INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        b2 = c[i] > b1 ? b1 : (c[i] > b2 ? c[i] : b2);
+        b1 = c[i] > b1 ? c[i] : b1;
+    }
+    for (int o = 1; o < 1 << a.lg_Lg; o <<= 1) {
+        const K p1 = __shfl_xor(b1, o), p2 = __shfl_xor(b2, o);
+        const K lo = p1 < b1 ? p1 : b1;
+        b1 = p1 > b1 ? p1 : b1;
+        b2 = p2 > b2 ? p2 : b2;
+        b2 = lo > b2 ? lo : b2;
+    }
+    const K mine = a.group_top == 2 ? b1 + b2 : b1;
+    int before = 0;
+    for (int h = 0; h < a.G; ++h) {
+        const K other = __shfl(mine, (r << a.lg_L) + (h << a.lg_Lg));
+        before += (other > mine || (other == mine && h < g)) ? 1 : 0;
+    }
+    const bool stays = before < a.top_groups && g < a.G;
+    if (!stays)
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = (K)-INFINITY;
+    lowest = -row_all<TakeMax>(stays ? -mine : (K)-INFINITY, 1 << a.lg_L);
+    const K highest = row_all<TakeMax>(stays || g >= a.G ? (K)-INFINITY : mine, 1 << a.lg_L);
+    return lowest - highest;
+}
+
+// Distance below which two 32-bit values of the choice may have changed places: twice the error of one.  Sigmoid: the
+// exponential is off by (|x| + 2) 2^-23 relatively, which s (1 - s) takes below 3e-7; reciprocal and sums add 2e-7.  Softmax: the
+// exponential by |x - max| 2^-24 + 2^-23 relatively, at most 1.5e-7 of 1 after exp(x - max); its sum of up to 512 terms by
+// 3e-6 relatively.  Adding the bias rounds once more.
+__device__ __forceinline__ float unsure(float v, int sigmoid) { return (sigmoid ? 1e-6f : 8e-6f) + 2.5e-7f * fabsf(v); }
+
+// SCORES: the choice goes by scores (32 bits first; rows in which neighbours of the choice lie closer than `unsure` are done
+// again in 64 bits), else by the logits themselves.
+template <typename T, int V, bool VEC, bool SCORES>
 __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArgs a) {
-    extern __shared__ float route_lds[];
+    extern __shared__ __attribute__((aligned(16))) char route_lds[];
     int64_t T_ = a.T;
     if (a.n_dev) { const int64_t n = *a.n_dev; T_ = n < T_ ? (n < 0 ? 0 : n) : T_; }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -83,111 +167,96 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
     bool odd = false;                                          // a logit that leaves the row without a choice to speak of
 #pragma unroll
     for (int i = 0; i < V; ++i) odd |= (x[i] != x[i]) || (!a.sigmoid && x[i] == INFINITY);
-    const uint64_t odd_lanes = __ballot(odd);
-    const bool bad = ((odd_lanes >> (r << a.lg_L)) & (L == 64 ? ~0ull : ((1ull << L) - 1))) != 0;
+    const bool bad = row_lanes(__ballot(odd), r, a.lg_L) != 0;
 
-    // values to choose by; -inf = not there (or already taken)
-    K c[V];
-    float xmax = 0.f, Z = 1.f;
-    if constexpr (sizeof(K) == 4) {
+    const int slots = a.k + (SCORES ? 1 : 0);
+    char* mine = route_lds + (size_t)(wave * rpw + r) * slots * (SCORES ? sizeof(Chosen<double>) : sizeof(Chosen<float>));
+    Chosen<float>* out = reinterpret_cast<Chosen<float>*>(mine);
+    float xmax = 0.f, Z = 1.f;                                 // softmax over the whole row, where it is asked for
+    if (!a.sigmoid && (SCORES || !a.renorm)) {
+        float m = x[0], z = 0.f;
+#pragma unroll
+        for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
+        xmax = row_all<TakeMax>(m, L);
+#pragma unroll
+        for (int i = 0; i < V; ++i) z += x[i] > -INFINITY ? expf(x[i] - xmax) : 0.f;
+        Z = row_all<TakeSum>(z, L);
+    }
+    float c[V];
+    bool again = false;
+    if (!SCORES) {
 #pragma unroll
         for (int i = 0; i < V; ++i) c[i] = bad ? -INFINITY : x[i];
-        if (!a.sigmoid && !a.renorm) {
-            float m = -INFINITY, z = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
-            xmax = row_max(m, L);
-#pragma unroll
-            for (int i = 0; i < V; ++i) z += x[i] > -INFINITY ? expf(x[i] - xmax) : 0.f;
-            Z = row_sum(z, L);
-        }
+        float lowest;
+        if (a.top_groups < a.G) keep_groups(a, c, r, g, lowest);
+        choose(a, c, x, e0, r, sub, a.k, out);
     } else {
-        double m = -INFINITY, z = 0.0, s[V];
-        if (!a.sigmoid) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) m = fmax(m, (double)x[i]);
-            m = row_max(m, L);
-        }
+        float bias[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const double xi = (double)x[i];
-            s[i] = !(x[i] > -INFINITY) ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-xi)) : exp(xi - m);
-            z += s[i];
+            bias[i] = (a.bias && i < nv) ? a.bias[e0 + i] : 0.f;
+            const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-x[i])) : expf(x[i] - xmax) * (1.f / Z);
+            const float v = s + bias[i];
+            c[i] = (!bad && x[i] > -INFINITY && v == v) ? v : -INFINITY;
         }
-        if (!a.sigmoid) {
-            z = row_sum(z, L);
-#pragma unroll
-            for (int i = 0; i < V; ++i) s[i] /= z;
-            xmax = (float)m; Z = (float)z;
+        if (a.top_groups < a.G) {
+            float lowest;
+            const float gap = keep_groups(a, c, r, g, lowest);                      // (of sums of up to two)
+            again = !(gap > 2.f * unsure(lowest, a.sigmoid)) && !bad;
         }
+        choose(a, c, x, e0, r, sub, a.k + 1, out);
+        for (int j = sub; j < a.k; j += L) {
+            const Chosen<float> p = out[j], q = out[j + 1];
+            // (equal logits and biases are equal in 64 bits as well -- unless a third that is not may come between the last
+            // that is chosen and the first that is not)
+            if (q.e >= 0 && !(p.c - q.c > unsure(p.c, a.sigmoid)))
+                again |= j == a.k - 1 || !(p.x == q.x && (!a.bias || a.bias[p.e] == a.bias[q.e]));
+        }
+        wave_lds_fence();
+        if (__ballot(again && on) != 0) {
+            Chosen<double>* wide = reinterpret_cast<Chosen<double>*>(mine);
+            double d[V], m = -INFINITY, z = 0.0;
+            if (!a.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const double b = (a.bias && i < nv) ? (double)a.bias[e0 + i] : 0.0;
-            const double v = s[i] + b;
-            c[i] = (!bad && x[i] > -INFINITY && v == v) ? (K)v : (K)-INFINITY;
+                for (int i = 0; i < V; ++i) m = fmax(m, (double)x[i]);
+                m = row_all<TakeMax>(m, L);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double xi = (double)x[i];
+                d[i] = !(x[i] > -INFINITY) ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-xi)) : exp(xi - m);
+                z += d[i];
+            }
+            if (!a.sigmoid) z = row_all<TakeSum>(z, L);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double v = (a.sigmoid ? d[i] : d[i] / z) + (double)bias[i];
+                d[i] = (!bad && x[i] > -INFINITY && v == v) ? v : -INFINITY;
+            }
+            double lowest;
+            if (a.top_groups < a.G) keep_groups(a, d, r, g, lowest);
+            choose(a, d, x, e0, r, sub, a.k, wide);
+            // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from)
+            if (sub == 0)
+                for (int j = 0; j < a.k; ++j) { const Chosen<double> w = wide[j]; out[j] = Chosen<float>{(float)w.c, w.x, w.e}; }
+            wave_lds_fence();
         }
     }
-
-    if (a.top_groups < a.G) {
-        // every lane of a group learns the group's value, then how many groups come before it
-        K b1 = (K)-INFINITY, b2 = (K)-INFINITY;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            b2 = c[i] > b1 ? b1 : (c[i] > b2 ? c[i] : b2);
-            b1 = c[i] > b1 ? c[i] : b1;
-        }
-        for (int o = 1; o < Lg; o <<= 1) {
-            const K p1 = __shfl_xor(b1, o), p2 = __shfl_xor(b2, o);
-            const K lo = p1 < b1 ? p1 : b1;
-            b1 = p1 > b1 ? p1 : b1;
-            b2 = p2 > b2 ? p2 : b2;
-            b2 = lo > b2 ? lo : b2;
-        }
-        const K mine = a.group_top == 2 ? b1 + b2 : b1;
-        int before = 0;
-        for (int h = 0; h < a.G; ++h) {
-            const K other = __shfl(mine, (r << a.lg_L) + (h << a.lg_Lg));
-            before += (other > mine || (other == mine && h < g)) ? 1 : 0;
-        }
-        if (before >= a.top_groups)
-#pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = (K)-INFINITY;
-    }
-
-    float* chosen_x = route_lds + (size_t)wave * rpw * a.k * 2 + (size_t)r * a.k;
-    int32_t* chosen_e = reinterpret_cast<int32_t*>(route_lds + (size_t)wave * rpw * a.k * 2 + (size_t)rpw * a.k) + (size_t)r * a.k;
-    for (int j = 0; j < a.k; ++j) {
-        K best = (K)-INFINITY;
-        int be = 0x7fffffff;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (c[i] > best) { best = c[i]; be = e0 + i; }
-        for (int o = 1; o < L; o <<= 1) {
-            const K ob = __shfl_xor(best, o);
-            const int oe = __shfl_xor(be, o);
-            if (ob > best || (ob == best && oe < be)) { best = ob; be = oe; }
-        }
-        if (sub == 0 && be == 0x7fffffff) chosen_e[j] = -1;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < nv && e0 + i == be) { c[i] = (K)-INFINITY; chosen_x[j] = x[i]; chosen_e[j] = be; }
-    }
-    wave_lds_fence();
     if (t >= T_) return;
     float m = 0.f, S = 1.f;
     if (a.renorm) {
         m = -INFINITY; S = 0.f;
-        for (int j = 0; j < a.k; ++j) if (chosen_e[j] >= 0) m = fmaxf(m, chosen_x[j]);
+        for (int j = 0; j < a.k; ++j) if (out[j].e >= 0) m = fmaxf(m, out[j].x);
         if (a.sigmoid) m = fminf(m, 0.f);
         for (int j = 0; j < a.k; ++j)
-            if (chosen_e[j] >= 0) S += a.sigmoid ? sigmoid_over(chosen_x[j], m) : expf(chosen_x[j] - m);
+            if (out[j].e >= 0) S += a.sigmoid ? sigmoid_over(out[j].x, m) : expf(out[j].x - m);
     } else if (!a.sigmoid) {
         m = xmax; S = Z;
     }
     for (int j = sub; j < a.k; j += L) {
-        int e = chosen_e[j];
+        int e = out[j].e;
         float w = 0.f;
-        if (e >= 0) w = a.scale * ((a.sigmoid ? sigmoid_over(chosen_x[j], m) : expf(chosen_x[j] - m)) / S);
+        if (e >= 0) w = a.scale * ((a.sigmoid ? sigmoid_over(out[j].x, m) : expf(out[j].x - m)) / S);
         if (!on) e = -1;
         else if (bad) { e = j; w = __builtin_nanf(""); }
         a.w[t * a.k + j] = w;
@@ -199,70 +268,79 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
 // With A = sum_i g_i w_i / scale:  renormalised softmax  dx_j = w_j (g_j - A), zero elsewhere (the chosen logits alone set the
 // ratios); renormalised sigmoid  dx_j = w_j (1 - s_j) (g_j - A);  sigmoid  dx_j = w_j (1 - s_j) g_j;
 // softmax  dx_e = [e chosen] w_e g_e - s_e sum_i g_i w_i.  Only the last one reads whole rows of logits again.
+// A wave's rows lie in LDS as 32-bit values: cleared, the chosen places written by one lane per entry, read back and stored
+// whole -- the entries are read once and no lane compares its experts with them.
 template <typename T, int V, bool VEC>
 __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a, const float* __restrict__ dw, T* __restrict__ dx) {
+    extern __shared__ __attribute__((aligned(16))) char route_lds[];
     int64_t T_ = a.T;
     if (a.n_dev) { const int64_t n = *a.n_dev; T_ = n < T_ ? (n < 0 ? 0 : n) : T_; }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int L = 1 << a.lg_L, rpw = kWave >> a.lg_L, sub = lane & (L - 1), r = lane >> a.lg_L;
     const int64_t t0 = ((int64_t)blockIdx.x * ROUTE_WAVES + wave) * rpw, t = t0 + r;
     if (t0 >= T_) return;
-    const bool on = t < T_;
-    const int64_t tt = on ? t : t0;
-    const int e0 = sub * V, nv = min(max(a.E - e0, 0), V);
-    const T* xp = reinterpret_cast<const T*>(a.x) + tt * a.stride + (nv > 0 ? e0 : 0);
-    float d[V];
+    const int rows = (int)min((int64_t)rpw, T_ - t0), e0 = sub * V, nv = r < rows ? min(max(a.E - e0, 0), V) : 0;
+    const bool whole = !a.sigmoid && !a.renorm;
+    float* d = reinterpret_cast<float*>(route_lds) + (size_t)wave * (64 * V + ((rpw * a.k + 3) & ~3));   // [rpw][L * V]
+    float* gw = d + 64 * V;                                                                     // [rpw][k]
+    f32x4* own = reinterpret_cast<f32x4*>(d + lane * V);
+    float x[V];
+    if (whole) load_logits<T, V, VEC>(reinterpret_cast<const T*>(a.x) + (r < rows ? t : t0) * a.stride + (nv > 0 ? e0 : 0), nv, x);
 #pragma unroll
-    for (int i = 0; i < V; ++i) d[i] = 0.f;
-    float A = 0.f;
-    bool mine = false, any = false;
-    for (int j = 0; j < a.k; ++j) {
-        const int e = a.idx[tt * a.k + j];
-        if (e >= 0) {
-            any = true;
-            A += dw[tt * a.k + j] * a.w[tt * a.k + j];
-            mine |= e >= e0 && e < e0 + nv;
+    for (int i = 0; i < V / 4; ++i) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int n = rows * a.k;
+    for (int i = lane; i < n; i += kWave) {
+        const int64_t at = t0 * a.k + i;
+        gw[i] = a.idx[at] >= 0 ? dw[at] * a.w[at] : 0.f;
+    }
+    wave_lds_fence();
+    for (int i = lane; i < n; i += kWave) {
+        const int64_t at = t0 * a.k + i;
+        const int row = a.by_k(i), e = a.idx[at];
+        float v = gw[i];
+        if (a.renorm) {
+            float A = 0.f;
+            for (int j = 0; j < a.k; ++j) A += gw[row * a.k + j];
+            v -= a.w[at] * (A / a.scale);
+        }
+        if ((unsigned)e < (unsigned)a.E) {
+            if (a.sigmoid) v *= 1.f / (1.f + expf((float)reinterpret_cast<const T*>(a.x)[(t0 + row) * a.stride + e]));
+            d[row * (L * V) + e] = v;
         }
     }
-    const bool whole = !a.sigmoid && !a.renorm;
-    float x[V];
-    if (whole || (a.sigmoid && mine)) load_logits<T, V, VEC>(xp, nv, x);
-    if (mine) {
-        const float shift = a.renorm ? A / a.scale : 0.f;
-        for (int j = 0; j < a.k; ++j) {
-            const int e = a.idx[tt * a.k + j];
+    wave_lds_fence();
+    float o[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i < nv && e == e0 + i) {
-                    float v = a.w[tt * a.k + j] * (dw[tt * a.k + j] - shift);
-                    if (a.sigmoid) v *= 1.f / (1.f + expf(x[i]));
-                    d[i] += v;
-                }
-        }
+    for (int i = 0; i < V / 4; ++i) {
+        const f32x4 v = own[i];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[i * 4 + q] = v[q];
     }
     if (whole) {
-        float m = -INFINITY, z = 0.f;
+        float m = x[0], z = 0.f, s[V], A = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
-        m = row_max(m, L);
-        float s[V];
+        for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
+        m = row_all<TakeMax>(m, L);
 #pragma unroll
         for (int i = 0; i < V; ++i) { s[i] = x[i] > -INFINITY ? expf(x[i] - m) : (x[i] != x[i] ? x[i] : 0.f); z += s[i]; }
-        z = row_sum(z, L);
+        z = row_all<TakeSum>(z, L);
+        bool any = false;
+        if (r < rows)
+            for (int j = 0; j < a.k; ++j) { A += gw[r * a.k + j]; any |= a.idx[t * a.k + j] >= 0; }
         if (any)
 #pragma unroll
-            for (int i = 0; i < V; ++i) d[i] -= s[i] / z * A;
+            for (int i = 0; i < V; ++i) o[i] -= s[i] / z * A;
     }
-    if (!on || nv == 0) return;
-    T* out = dx + t * (int64_t)a.E + e0;
+    if (nv == 0) return;
+    T* p = dx + t * (int64_t)a.E + e0;
     if (VEC) {
-        struct alignas(sizeof(T) * V) Pack { T v[V]; } q;
+        struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack { T v[V]; } q;
 #pragma unroll
-        for (int i = 0; i < V; ++i) q.v[i] = (T)d[i];
-        *reinterpret_cast<Pack*>(out) = q;
+        for (int i = 0; i < V; ++i) q.v[i] = (T)o[i];
+        *reinterpret_cast<Pack*>(p) = q;
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) if (i < nv) out[i] = (T)d[i];
+        for (int i = 0; i < V; ++i) if (i < nv) p[i] = (T)o[i];
     }
 }
 
@@ -270,136 +348,179 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a, const float
 // Entry i = row * top_k + choice.  An entry whose expert is not in [0, E), or whose row lies behind the device-side count, is
 // in no segment: its position is -1.  Blocks own consecutive stretches of entries, the waves of a block consecutive parts of
 // them; what a wave counts in order lands in order, so equal inputs give equal plans.
-constexpr int PLAN_THREADS = 256, PLAN_WAVES = PLAN_THREADS / kWave, PLAN_MAX_E = 512, PLAN_MAX_BLOCKS = 256;
+constexpr int PLAN_WAVES = 16, PLAN_THREADS = PLAN_WAVES * kWave, PLAN_MAX_BLOCKS = 256;
+constexpr int PLAN_LANE = 8, PLAN_PIECE = PLAN_LANE * kWave;      // entries that a lane, a wave loads at a time
 
-__device__ __forceinline__ int plan_expert(const int32_t* __restrict__ experts, int i, int end, int E) {
-    if (i >= end) return -1;
-    const int e = experts[i];
-    return (e >= 0 && e < E) ? e : -1;
+__device__ __forceinline__ void plan_load(const int32_t* __restrict__ experts, int i0, int end, int E, int (&e)[PLAN_LANE]) {
+#pragma unroll
+    for (int q = 0; q < PLAN_LANE; ++q) {
+        const int i = i0 + q * kWave + (threadIdx.x & 63);
+        e[q] = i < end ? experts[i] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < PLAN_LANE; ++q) e[q] = (unsigned)e[q] < (unsigned)E ? e[q] : -1;
+}
+__device__ __forceinline__ int plan_end(int n, int k, const int64_t* __restrict__ n_dev) {
+    if (!n_dev) return n;
+    const int64_t m = *n_dev;
+    return m < 0 ? 0 : (m < n / k ? (int)m * k : n);
 }
 
+// entries per expert of each block
 __global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(const int32_t* __restrict__ experts, int n, int k, int E, int per_block,
                                                                   int32_t* __restrict__ counts, const int64_t* __restrict__ n_dev) {
-    __shared__ int32_t hist[PLAN_MAX_E];
+    __shared__ int32_t hist[NSX_MAX_EXPERTS];
     for (int e = threadIdx.x; e < E; e += PLAN_THREADS) hist[e] = 0;
     __syncthreads();
-    int end = n;
-    if (n_dev) { const int64_t m = *n_dev * k; end = m < n ? (m < 0 ? 0 : (int)m) : n; }
-    const int a = blockIdx.x * per_block, b = min(a + per_block, n);
-    for (int i = a + threadIdx.x; i < b; i += PLAN_THREADS) {
-        const int e = plan_expert(experts, i, end, E);
-        if (e >= 0) atomicAdd(&hist[e], 1);
+    const int wave = threadIdx.x >> 6, a = blockIdx.x * per_block, b = min(a + per_block, plan_end(n, k, n_dev));
+    for (int i = a + wave * PLAN_PIECE; i < b; i += PLAN_WAVES * PLAN_PIECE) {
+        int e[PLAN_LANE];
+        plan_load(experts, i, b, E, e);
+#pragma unroll
+        for (int q = 0; q < PLAN_LANE; ++q) if (e[q] >= 0) atomicAdd(&hist[e[q]], 1);
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += PLAN_THREADS) counts[(int64_t)blockIdx.x * E + e] = hist[e];
 }
 
-__global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(const int32_t* __restrict__ experts, int n, int k, int E, int per_block,
+// bits: of an expert's number; lg_E: threads per column sum of the blocks' counts, as a power of two >= E
+__global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(const int32_t* __restrict__ experts, int n, int k, int E, int bits, int per_block,
                                                                   const int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
                                                                   int32_t* __restrict__ rows, int32_t* __restrict__ positions,
                                                                   const int64_t* __restrict__ n_dev) {
-    __shared__ int32_t cursor[PLAN_WAVES][PLAN_MAX_E];     // next free place of the wave's part, per expert
-    __shared__ int32_t base[PLAN_MAX_E];
-    __shared__ int32_t wave_total[PLAN_WAVES];
+    __shared__ int32_t cursor[PLAN_WAVES][NSX_MAX_EXPERTS];     // next free place of the wave's part, per expert
+    __shared__ int32_t part_all[PLAN_THREADS], part_before[PLAN_THREADS];
+    __shared__ int32_t all[NSX_MAX_EXPERTS], first[NSX_MAX_EXPERTS];
+    __shared__ int32_t routed;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blocks = gridDim.x;
-    int end = n;
-    if (n_dev) { const int64_t m = *n_dev * k; end = m < n ? (m < 0 ? 0 : (int)m) : n; }
-    for (int e = threadIdx.x; e < PLAN_WAVES * PLAN_MAX_E; e += PLAN_THREADS) (&cursor[0][0])[e] = 0;
+    const int end = plan_end(n, k, n_dev);
+    for (int w = 0; w < PLAN_WAVES; ++w)
+        for (int e = threadIdx.x; e < E; e += PLAN_THREADS) cursor[w][e] = 0;
     __syncthreads();
-    // this wave's part
-    const int a0 = blockIdx.x * per_block, b0 = min(a0 + per_block, n);
-    const int part = per_block / PLAN_WAVES;
-    const int a = min(a0 + wave * part, b0), b = min(a + part, b0);
-    for (int i = a + lane; i < b; i += kWave) {
-        const int e = plan_expert(experts, i, end, E);
-        if (e >= 0) atomicAdd(&cursor[wave][e], 1);
-    }
-    // segment starts (exclusive sum over the experts of all blocks' counts) and what earlier blocks put in front
-    int total[PLAN_MAX_E / PLAN_THREADS], before[PLAN_MAX_E / PLAN_THREADS], sum = 0;
+    const int a0 = blockIdx.x * per_block, b0 = min(a0 + per_block, n), part = per_block / PLAN_WAVES;
+    const int a = min(a0 + wave * part, b0), b = min(a + part, b0), live = min(b, end);
+    int e[PLAN_LANE];
+    for (int i = a; i < live; i += PLAN_PIECE) {
+        plan_load(experts, i, live, E, e);
 #pragma unroll
-    for (int q = 0; q < PLAN_MAX_E / PLAN_THREADS; ++q) {
-        const int e = threadIdx.x * (PLAN_MAX_E / PLAN_THREADS) + q;
-        int tot = 0, bef = 0;
-        if (e < E)
-            for (int h = 0; h < blocks; ++h) {
-                const int v = counts[(int64_t)h * E + e];
-                tot += v;
-                bef += h < (int)blockIdx.x ? v : 0;
+        for (int q = 0; q < PLAN_LANE; ++q) if (e[q] >= 0) atomicAdd(&cursor[wave][e[q]], 1);
+    }
+    // of every expert: all entries, and those of earlier blocks
+    if (blocks > 1) {
+        const int col = threadIdx.x & ((1 << bits) - 1), parts = PLAN_THREADS >> bits;
+        int sum = 0, before = 0;
+        if (col < E) {
+#pragma unroll 8
+            for (int h = threadIdx.x >> bits; h < blocks; h += parts) {
+                const int v = counts[(int64_t)h * E + col];
+                sum += v;
+                before += h < (int)blockIdx.x ? v : 0;
             }
-        total[q] = tot; before[q] = bef; sum += tot;
+        }
+        part_all[threadIdx.x] = sum;
+        part_before[threadIdx.x] = before;
     }
-    int scan = sum;
-    for (int o = 1; o < kWave; o <<= 1) { const int v = __shfl_up(scan, o); if (lane >= o) scan += v; }
-    if (lane == 63) wave_total[wave] = scan;
     __syncthreads();
-    int start = scan - sum, all = 0;
-    for (int w = 0; w < PLAN_WAVES; ++w) { if (w < wave) start += wave_total[w]; all += wave_total[w]; }
+    for (int x = threadIdx.x; x < E; x += PLAN_THREADS) {
+        int sum = 0, before = 0;
+        if (blocks > 1) {
+            for (int h = x; h < PLAN_THREADS; h += 1 << bits) { sum += part_all[h]; before += part_before[h]; }
+        } else {
+            for (int w = 0; w < PLAN_WAVES; ++w) sum += cursor[w][x];
+        }
+        all[x] = sum;
+        first[x] = before;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        constexpr int PER = NSX_MAX_EXPERTS / kWave;
+        int sum = 0;
 #pragma unroll
-    for (int q = 0; q < PLAN_MAX_E / PLAN_THREADS; ++q) {
-        const int e = threadIdx.x * (PLAN_MAX_E / PLAN_THREADS) + q;
-        if (e < E) {
-            base[e] = start + before[q];
-            if (blockIdx.x == 0) offsets[e] = start;
-            start += total[q];
+        for (int q = 0; q < PER; ++q) { const int x = lane * PER + q; if (x < E) sum += all[x]; }
+        int scan = sum;
+        for (int o = 1; o < kWave; o <<= 1) { const int v = __shfl_up(scan, o); if (lane >= o) scan += v; }
+        int start = scan - sum;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int x = lane * PER + q;
+            if (x < E) {
+                first[x] += start;
+                if (blockIdx.x == 0) offsets[x] = start;
+                start += all[x];
+            }
+        }
+        if (lane == 63) {
+            routed = scan;
+            if (blockIdx.x == 0) offsets[E] = scan;
         }
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) offsets[E] = all;
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += PLAN_THREADS) {
-        int p = base[e];
-        for (int w = 0; w < PLAN_WAVES; ++w) { const int v = cursor[w][e]; cursor[w][e] = p; p += v; }
+    for (int x = threadIdx.x; x < E; x += PLAN_THREADS) {
+        int p = first[x];
+        for (int w = 0; w < PLAN_WAVES; ++w) { const int v = cursor[w][x]; cursor[w][x] = p; p += v; }
     }
     __syncthreads();
-    for (int i0 = a; i0 < b; i0 += kWave) {
-        const int i = i0 + lane;
-        const int e = i < b ? plan_expert(experts, i, end, E) : -1;
-        uint64_t same = __ballot(e >= 0);
+    const bool kept = b - a <= PLAN_PIECE;                        // (the entries are still in registers)
+    for (int i0 = a; i0 < b; i0 += PLAN_PIECE) {
+        if (!kept || i0 >= live) plan_load(experts, i0, live, E, e);
 #pragma unroll
-        for (int bit = 0; bit < 9; ++bit) {
-            const uint64_t m = __ballot((e >> bit) & 1);
-            same &= ((e >> bit) & 1) ? m : ~m;
+        for (int q = 0; q < PLAN_LANE; ++q) {
+            const int i = i0 + q * kWave + lane;
+            // lanes with the same expert, by its bits; the lowest free place, then one more for each of them
+            uint64_t same = __ballot(e[q] >= 0);
+            for (int bit = 0; bit < bits; ++bit) {
+                const bool set = (e[q] >> bit) & 1;
+                const uint64_t m = __ballot(set);
+                same &= set ? m : ~m;
+            }
+            int place = -1;
+            if (e[q] >= 0) place = cursor[wave][e[q]] + __popcll(same & ((1ull << lane) - 1));
+            wave_lds_fence();
+            if (e[q] >= 0 && (same >> lane) == 1) cursor[wave][e[q]] = place + 1;         // the last of them
+            wave_lds_fence();
+            if (i < b) positions[i] = place;
+            if (place >= 0) rows[place] = i;
         }
-        int place = -1;
-        if (e >= 0) place = cursor[wave][e] + __popcll(same & ((1ull << lane) - 1));
-        wave_lds_fence();
-        if (e >= 0 && (same >> lane) == 1) cursor[wave][e] = place + 1;         // the last one of its expert
-        wave_lds_fence();
-        if (i < b) positions[i] = place;
-        if (place >= 0) rows[place] = i;
     }
     // rows behind the last segment: this block's share of them
-    for (int i = max(a0, all) + threadIdx.x; i < b0; i += PLAN_THREADS) rows[i] = -1;
+    for (int i = max(a0, routed) + threadIdx.x; i < b0; i += PLAN_THREADS) rows[i] = -1;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 static int lg2_ceil(int v) { int l = 0; while ((1 << l) < v) ++l; return l; }
 
 static int plan_blocks(int64_t n) {
-    const int64_t b = (n + 2047) / 2048;
+    const int64_t b = (n + PLAN_WAVES * PLAN_PIECE - 1) / (PLAN_WAVES * PLAN_PIECE);
     return (int)(b < 1 ? 1 : b > PLAN_MAX_BLOCKS ? PLAN_MAX_BLOCKS : b);
 }
 
-template <typename T, typename K, int V>
-static void launch_route_fwd(const RouteArgs& a, bool vec, hipStream_t st) {
-    const int rpw = kWave >> a.lg_L;
-    const int64_t blocks = (a.T + (int64_t)rpw * ROUTE_WAVES - 1) / ((int64_t)rpw * ROUTE_WAVES);
-    const size_t lds = (size_t)ROUTE_WAVES * rpw * a.k * 8;
-    if (vec) route_fwd_kernel<T, K, V, true><<<(unsigned)blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
-    else route_fwd_kernel<T, K, V, false><<<(unsigned)blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
-}
-
 template <typename T, int V>
-static void launch_route(const RouteArgs& a, bool wide, bool vec, hipStream_t st) {
-    if (wide) launch_route_fwd<T, double, V>(a, vec, st);
-    else launch_route_fwd<T, float, V>(a, vec, st);
+static void launch_route(const RouteArgs& a, bool by_scores, bool vec, hipStream_t st) {
+    const int rpw = kWave >> a.lg_L;
+    const unsigned blocks = (unsigned)((a.T + (int64_t)rpw * ROUTE_WAVES - 1) / ((int64_t)rpw * ROUTE_WAVES));
+    const size_t lds = (size_t)ROUTE_WAVES * rpw * (by_scores ? (a.k + 1) * sizeof(Chosen<double>) : a.k * sizeof(Chosen<float>));
+    if (by_scores) {
+        if (vec) route_fwd_kernel<T, V, true, true><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
+        else route_fwd_kernel<T, V, false, true><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
+    } else {
+        if (vec) route_fwd_kernel<T, V, true, false><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
+        else route_fwd_kernel<T, V, false, false><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
+    }
 }
 
 template <typename T, int V>
 static void launch_route_bwd(const RouteArgs& a, bool vec, const float* dw, void* dx, hipStream_t st) {
     const int rpw = kWave >> a.lg_L;
-    const int64_t blocks = (a.T + (int64_t)rpw * ROUTE_WAVES - 1) / ((int64_t)rpw * ROUTE_WAVES);
-    if (vec) route_bwd_kernel<T, V, true><<<(unsigned)blocks, 256, 0, st>>>(a, dw, (T*)dx);
-    else route_bwd_kernel<T, V, false><<<(unsigned)blocks, 256, 0, st>>>(a, dw, (T*)dx);
+    const unsigned blocks = (unsigned)((a.T + (int64_t)rpw * ROUTE_WAVES - 1) / ((int64_t)rpw * ROUTE_WAVES));
+    const size_t lds = (size_t)ROUTE_WAVES * (64 * V + ((rpw * a.k + 3) & ~3)) * 4;
+    if (vec) route_bwd_kernel<T, V, true><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a, dw, (T*)dx);
+    else route_bwd_kernel<T, V, false><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a, dw, (T*)dx);
+}
+
+// rows of logits can be read (and written) V at a time
+static bool route_vec(const void* p, int V, int esize, int64_t stride, int group) {
+    const size_t align = std::min<size_t>(16, (size_t)V * esize);
+    return group % V == 0 && (size_t)stride * esize % align == 0 && reinterpret_cast<uintptr_t>(p) % align == 0;
 }
 
 static int route_check(const char* what, int dtype, int64_t T, int E, int64_t stride, int k) {
@@ -432,13 +553,13 @@ int nsx_expert_route_fwd(const void* logits, int dtype, int64_t T, int E, int64_
     NSX_REQUIRE(logits && weights && experts, "nsx_expert_route_fwd: NULL pointer");
     const int Eg = E / n_groups, lg_G = lg2_ceil(n_groups);
     RouteArgs a{logits, row_stride, T, E, bias, selector, top_k, n_groups, top_groups, group_top, sigmoid, renormalise, scale,
-                weights, experts, n_device, 0, 0};
+                weights, experts, n_device, 0, 0, fast_div(top_k)};
     // 16 bytes per lane where the groups are whole numbers of them, else as few values per lane as 64 lanes allow
-    int V = dtype == NSX_DTYPE_F32 ? 4 : 8;
+    int V = 8;
     const int esize = dtype == NSX_DTYPE_F32 ? 4 : 2;
     while (V > 4 && Eg % V) V >>= 1;
     while (lg_G + lg2_ceil((Eg + V - 1) / V) > 6) V <<= 1;
-    const bool vec = Eg % V == 0 && row_stride % V == 0 && (reinterpret_cast<uintptr_t>(logits) % (size_t)(V * esize)) == 0;
+    const bool vec = route_vec(logits, V, esize, row_stride, Eg);
     a.lg_Lg = lg2_ceil((Eg + V - 1) / V);
     a.lg_L = lg_G + a.lg_Lg;
     const bool wide = bias || (top_groups < n_groups && group_top == 2);
@@ -468,12 +589,10 @@ int nsx_expert_route_bwd(const void* logits, int dtype, int64_t T, int E, int64_
     if (T == 0) return NSX_OK;
     NSX_REQUIRE(logits && weights && experts && dweights && dlogits, "nsx_expert_route_bwd: NULL pointer");
     RouteArgs a{logits, row_stride, T, E, nullptr, nullptr, top_k, 1, 1, 1, sigmoid, renormalise, scale,
-                const_cast<float*>(weights), const_cast<int32_t*>(experts), n_device, 0, 0};
+                const_cast<float*>(weights), const_cast<int32_t*>(experts), n_device, 0, 0, fast_div(top_k)};
     const int esize = dtype == NSX_DTYPE_F32 ? 4 : 2;
-    int V = dtype == NSX_DTYPE_F32 ? (E <= 256 ? 4 : 8) : 8;
-    if (dtype != NSX_DTYPE_F32 && E % 8 && E <= 256) V = 4;
-    const bool vec = E % V == 0 && row_stride % V == 0 && (reinterpret_cast<uintptr_t>(logits) % (size_t)(V * esize)) == 0 &&
-                     (reinterpret_cast<uintptr_t>(dlogits) % (size_t)(V * esize)) == 0;
+    const int V = E % 8 && E <= 256 ? 4 : 8;
+    const bool vec = route_vec(logits, V, esize, row_stride, E) && route_vec(dlogits, V, esize, E, E);
     a.lg_L = lg2_ceil((E + V - 1) / V);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype * 32 + V) {
@@ -505,12 +624,14 @@ int nsx_expert_plan(const int32_t* experts, int64_t T, int top_k, int E, int32_t
     const int n = (int)(T * top_k), blocks = plan_blocks(n);
     NSX_REQUIRE(n == 0 || (experts && rows && positions), "nsx_expert_plan: NULL pointer");
     int64_t per = ((int64_t)n + blocks - 1) / blocks;
-    per = (per + PLAN_THREADS - 1) / PLAN_THREADS * PLAN_THREADS;
+    per = (per + PLAN_WAVES * PLAN_PIECE - 1) / (PLAN_WAVES * PLAN_PIECE) * (PLAN_WAVES * PLAN_PIECE);
     hipStream_t st = (hipStream_t)stream;
-    plan_count_kernel<<<blocks, PLAN_THREADS, 0, st>>>(experts, n, top_k, E, (int)per, (int32_t*)workspace, n_device);
-    NSX_LAUNCH_CHECK("nsx_expert_plan");
-    plan_place_kernel<<<blocks, PLAN_THREADS, 0, st>>>(experts, n, top_k, E, (int)per, (const int32_t*)workspace, offsets, rows,
-                                                       positions, n_device);
+    if (blocks > 1) {
+        plan_count_kernel<<<blocks, PLAN_THREADS, 0, st>>>(experts, n, top_k, E, (int)per, (int32_t*)workspace, n_device);
+        NSX_LAUNCH_CHECK("nsx_expert_plan");
+    }
+    plan_place_kernel<<<blocks, PLAN_THREADS, 0, st>>>(experts, n, top_k, E, lg2_ceil(E), (int)per, (const int32_t*)workspace, offsets,
+                                                       rows, positions, n_device);
     NSX_LAUNCH_CHECK("nsx_expert_plan");
     return NSX_OK;
 }
