@@ -121,13 +121,15 @@ __device__ __forceinline__ bool lin_order(int tiles, int m_tiles, int block, int
     tile = group * LIN_GROUP + rest - m * n;
     return true;
 }
-// dW: an XCD takes blocks of 4 x 4 tiles of one segment (or chunk of one) in turn with the others
+// dW: an XCD takes blocks of up to 4 x 4 tiles of one segment (or chunk of one) in turn with the others.  (No workgroups for
+// tiles that are not there: of blocks of 16 with one tile each, the working ones fell on two of an XCD's 32 CUs.)
+__host__ __device__ __forceinline__ int lin_group_dw(int tiles) { return tiles < 4 ? tiles : 4; }
 __device__ __forceinline__ bool lin_order_dw(const LinArgs& g, int block, int& s, int& m, int& c) {
-    const int gm = (g.m_tiles + 3) / 4, gc = (g.c_tiles + 3) / 4;
-    const int local = block >> 3, within = local & 15;
-    int group = (local >> 4) * 8 + (block & 7);
-    m = group % gm * 4 + (within & 3); group /= gm;
-    c = group % gc * 4 + (within >> 2);
+    const int wm = lin_group_dw(g.m_tiles), wc = lin_group_dw(g.c_tiles), gm = (g.m_tiles + wm - 1) / wm, gc = (g.c_tiles + wc - 1) / wc;
+    const int local = block >> 3, within = local % (wm * wc);
+    int group = local / (wm * wc) * 8 + (block & 7);
+    m = group % gm * wm + within % wm; group /= gm;
+    c = group % gc * wc + within / wm;
     s = group / gc;
     return m < g.m_tiles && c < g.c_tiles;
 }
@@ -356,30 +358,34 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
     }
 }
 
-// dW of an expert = the sum of its chunks, in their order.  16 chunks at a time side by side, 16 x 4 values per workgroup.
+// dW of an expert = the sum of its chunks, in their order: 16 of them side by side and 16 x 4 values per workgroup, or (few
+// chunks) 256 x 4 values.
 template <typename T>
 __global__ __launch_bounds__(256) void expert_sum_chunks_kernel(LinArgs g, T* __restrict__ d) {
     __shared__ f32x4 part[16][16];
-    const int e = blockIdx.y, lane = threadIdx.x & 63, who = threadIdx.x >> 4, at = threadIdx.x & 15;
+    const int e = blockIdx.y, lane = threadIdx.x & 63;
     int first = 0, a, b;
     for (int q = lane; q < e; q += kWave) { segment(g.offsets, q, g.R, a, b); first += (b - a + g.chunk - 1) / g.chunk; }
     for (int o = 1; o < kWave; o <<= 1) first += __shfl_xor(first, o);
     segment(g.offsets, e, g.R, a, b);
-    const int n = min((b - a + g.chunk - 1) / g.chunk, g.R / g.chunk + g.E - first);
+    const int n = min((b - a + g.chunk - 1) / g.chunk, g.R / g.chunk + g.E - first), ways = n > 8 ? 16 : 1;
+    const int who = ways > 1 ? threadIdx.x >> 4 : 0, at = ways > 1 ? threadIdx.x & 15 : threadIdx.x, step = 1024 / ways;
     const int64_t size = (int64_t)g.C * g.M;
-    for (int64_t i0 = (int64_t)blockIdx.x * 64; i0 < size; i0 += (int64_t)gridDim.x * 64) {
+    for (int64_t i0 = (int64_t)blockIdx.x * step; i0 < size; i0 += (int64_t)gridDim.x * step) {
         const int64_t i = i0 + at * 4;
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
         if (i < size)
-            for (int q = who; q < n; q += 16) s += *reinterpret_cast<const f32x4*>(g.partial + (first + q) * size + i);
-        part[who][at] = s;
-        __syncthreads();
-        if (who == 0 && i < size) {
-            for (int q = 1; q < 16; ++q) s += part[q][at];
+            for (int q = who; q < n; q += ways) s += *reinterpret_cast<const f32x4*>(g.partial + (first + q) * size + i);
+        if (ways > 1) {
+            part[who][at] = s;
+            __syncthreads();
+            if (who == 0)
+                for (int q = 1; q < 16; ++q) s += part[q][at];
+            __syncthreads();
+        }
+        if (who == 0 && i < size)
 #pragma unroll
             for (int r = 0; r < 4; ++r) d[(int64_t)e * size + i + r] = (T)s[r];
-        }
-        __syncthreads();
     }
 }
 
@@ -404,14 +410,16 @@ static int lin_launch_tile(LinArgs g, hipStream_t st) {
     g.c_tiles = (g.C + TC - 1) / TC;
     int64_t blocks;
     if (MODE == LIN_DW) {
-        const int64_t groups = (g.chunk > 0 ? g.R / g.chunk + g.E : g.E) * (int64_t)((g.m_tiles + 3) / 4) * ((g.c_tiles + 3) / 4);
-        blocks = (groups + 7) / 8 * 128;
+        const int wm = lin_group_dw(g.m_tiles), wc = lin_group_dw(g.c_tiles);
+        const int64_t groups = (g.chunk > 0 ? g.R / g.chunk + g.E : g.E) * (int64_t)((g.m_tiles + wm - 1) / wm) * ((g.c_tiles + wc - 1) / wc);
+        blocks = (groups + 7) / 8 * 8 * wm * wc;
     } else {
         blocks = ((int64_t)g.R / TC + g.E + 1) * g.m_tiles;
         blocks = (blocks + 7) / 8 * 8;
     }
     NSX_REQUIRE(blocks <= 0x7fffffff, "expert_linear: %lld tiles", (long long)blocks);
-    if (g.mask) expert_linear_kernel<T, MODE, TM, TC, WM, WC, true, F32><<<(unsigned)blocks, WM * WC * kWave, lds, st>>>(g);
+    constexpr bool MAY_MASK = MODE != LIN_FWD && TM * TC <= 128 * 128;
+    if (MAY_MASK && g.mask) expert_linear_kernel<T, MODE, TM, TC, WM, WC, MAY_MASK, F32><<<(unsigned)blocks, WM * WC * kWave, lds, st>>>(g);
     else expert_linear_kernel<T, MODE, TM, TC, WM, WC, false, F32><<<(unsigned)blocks, WM * WC * kWave, lds, st>>>(g);
     return NSX_OK;
 }
@@ -428,24 +436,35 @@ static bool small_tiles(const LinArgs& g) {
     return g.M <= 64 || g.R < 16 * (int64_t)g.E || rows * ((g.M + 127) / 128) < num_cus();
 }
 // dW, chunk (0: none) and tile.  us with chunks of 256 | 512 | 1024 | 2048 rows:
-//   262144 x 2 of 16,  32 ->  64   64 x 64 tiles  75 | 63 | 63 | 70     128 x 128 tiles 174 | 143 | 135 | 143
-//    65536 x 2 of 16, 128 -> 128   64 x 64 tiles  47 | 43 | 45 | 67     128 x 128 tiles  70 |  59 |  63 |  67
-//    65536 x 2 of 16, 256 -> 256   64 x 64 tiles 119 | 84 | 82 | 85     128 x 128 tiles 164 | 109 | 104 | 114
-//     5003 x 3 of 23, 176 -> 136   64 x 64 tiles  25 | 28 | 35 | 40     128 x 128 tiles  31 |  31 |  42 |  46
-// Short chunks fill the card, long ones keep the partial sums small beside what is read: about two and a half workgroups per CU.
+//   262144 x 2 of 16,  32 ->  64   64 x 64 tiles  45 | 40 | 39 | 50     128 x 128 tiles  63 |  54 |  58 |  61
+//    65536 x 2 of 16, 128 -> 128   64 x 64 tiles  36 | 31 | 38 | 52     128 x 128 tiles  40 |  33 |  37 |  55
+//    65536 x 2 of 16, 256 -> 256   64 x 64 tiles 118 | 81 | 80 | 84     128 x 128 tiles 110 |  79 |  79 |  80
+//     5003 x 3 of 23, 176 -> 136   64 x 64 tiles  24 | 26 | 32 | 37     128 x 128 tiles  25 |  27 |  36 |  43
+// Short chunks fill the card, long ones keep the partial sums small beside what is read: about four workgroups per CU.
 // Without chunks (the matrices have tiles enough) the larger tiles are faster: 16384 x 2 of 16, 1024 -> 2048: 570 | 180.
 struct DwPlan { int chunk; bool small; };
 static DwPlan dw_plan(int64_t R, int E, int n_in, int n_out) {
     const int64_t large = (int64_t)((n_in + 127) / 128) * ((n_out + 127) / 128), small = (int64_t)((n_in + 63) / 64) * ((n_out + 63) / 64);
     if (large * E >= 2 * (int64_t)num_cus()) return {0, false};
     if (small * E >= 4 * (int64_t)num_cus() || R < 8 * (int64_t)LIN_BQ) return {0, true};
-    int64_t chunk = R * small * 2 / (5 * (int64_t)num_cus());
+    int64_t chunk = R * small / (4 * (int64_t)num_cus());
     chunk = (chunk + LIN_BQ - 1) / LIN_BQ * LIN_BQ;
     return {(int)std::min<int64_t>(std::max<int64_t>(chunk, 4 * LIN_BQ), 1024), true};
 }
 
+// The largest products: a wave's tile of 128 x 64 needs three quarters of the LDS reads.  us with 128 x 128 | 256 x 128 | 128 x 256:
+//   16384 x 2 of 16, 1024 -> 2048   forward 172 | 162 | 173   dx 158 | 152 | 158   dW 177 | 178 | 166
+//   16384 x 2 of 8,  2048 -> 2048   forward 322 | 292 | 306   dx 304 | 287 | 289   dW 328 | 318 | 303
+//    8192 x 2 of 16, 1024 -> 1024   forward  52 |  56 |  58   dx  48 |  51 |  51   dW  59 |  62 |  57
+static bool large_tiles(int64_t tiles128) { return tiles128 >= 6 * (int64_t)num_cus(); }
+
 template <typename T, int MODE, bool F32>
 static int lin_launch(const LinArgs& g, bool small, hipStream_t st) {
+    if (!g.mask && !F32) {              // (with a mask to apply they do not fit the registers)
+        const int64_t tm = (g.M + 127) / 128;
+        if (MODE != LIN_DW && g.M > 128 && large_tiles((g.R / 128 + std::min(g.E, g.R)) * tm)) return lin_launch_tile<T, MODE, 256, 128, 2, 2, F32>(g, st);
+        if (MODE == LIN_DW && g.C > 128 && large_tiles(g.E * tm * ((g.C + 127) / 128))) return lin_launch_tile<T, MODE, 128, 256, 1, 4, F32>(g, st);
+    }
     if (small) return lin_launch_tile<T, MODE, 64, 64, 1, 2, F32>(g, st);
     return lin_launch_tile<T, MODE, 128, 128, 2, 2, F32>(g, st);
 }
@@ -529,7 +548,8 @@ int nsx_expert_linear_bwd_w(const void* x, int dtype, int64_t x_stride, int64_t 
     if (rc != NSX_OK) return rc;
     NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_w");
     if (g.chunk > 0) {
-        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)n_in * n_out + 63) / 64, 4096), E);
+        const int64_t step = R / g.chunk > 8 * (int64_t)E ? 64 : 1024;
+        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)n_in * n_out + step - 1) / step, 4096), E);
         if (dw_f32) expert_sum_chunks_kernel<float><<<grid, 256, 0, st>>>(g, (float*)dw);
         else if (dtype == NSX_DTYPE_F16) expert_sum_chunks_kernel<half_t><<<grid, 256, 0, st>>>(g, (half_t*)dw);
         else expert_sum_chunks_kernel<bf16_t><<<grid, 256, 0, st>>>(g, (bf16_t*)dw);

@@ -80,11 +80,10 @@ __device__ __forceinline__ float sigmoid_over(float x, float m) {
 }
 
 // One pass of the choice over the wave's rows: values c (taken from it as they are chosen) -> entries of `out`, k + 1 of them
-// if `more` (the one that just missed).  out: per row top_k + 1 of {value, logit, expert}.
-template <typename K> struct Chosen { K c; float x; int32_t e; };
+// if `more` (the one that just missed).  out: per row top_k + 1 of {value, expert}.
+template <typename K> struct Chosen { K c; int32_t e; };
 template <typename K, int V>
-__device__ __forceinline__ void choose(const RouteArgs& a, K (&c)[V], const float (&x)[V], int e0, int r, int sub, int rounds,
-                                       Chosen<K>* __restrict__ out) {
+__device__ __forceinline__ void choose(const RouteArgs& a, K (&c)[V], int e0, int r, int sub, int rounds, Chosen<K>* __restrict__ out) {
     const int L = 1 << a.lg_L;
     for (int j = 0; j < rounds; ++j) {
         K best = c[0];
@@ -96,13 +95,9 @@ __device__ __forceinline__ void choose(const RouteArgs& a, K (&c)[V], const floa
             int at = V - 1;
 #pragma unroll
             for (int i = V - 2; i >= 0; --i) at = c[i] == top ? i : at;
-            float xv = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                xv = i == at ? x[i] : xv;
-                c[i] = i == at ? (K)-INFINITY : c[i];
-            }
-            out[j] = Chosen<K>{top, xv, top > (K)-INFINITY ? e0 + at : -1};
+            for (int i = 0; i < V; ++i) c[i] = i == at ? (K)-INFINITY : c[i];
+            out[j] = Chosen<K>{top, top > (K)-INFINITY ? e0 + at : -1};
         }
     }
     wave_lds_fence();
@@ -162,8 +157,9 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
     const int Eg = a.E / a.G, g = sub >> a.lg_Lg, lg = sub & (Lg - 1);
     const int e0 = g * Eg + lg * V;
     const int nv = (on && g < a.G) ? min(max(Eg - lg * V, 0), V) : 0;
+    const T* row = reinterpret_cast<const T*>(a.x) + (on ? t : 0) * a.stride;
     float x[V];
-    load_logits<T, V, VEC>(reinterpret_cast<const T*>(a.x) + (on ? t : 0) * a.stride + (nv > 0 ? e0 : 0), nv, x);
+    load_logits<T, V, VEC>(row + (nv > 0 ? e0 : 0), nv, x);
     bool odd = false;                                          // a logit that leaves the row without a choice to speak of
 #pragma unroll
     for (int i = 0; i < V; ++i) odd |= (x[i] != x[i]) || (!a.sigmoid && x[i] == INFINITY);
@@ -189,7 +185,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
         for (int i = 0; i < V; ++i) c[i] = bad ? -INFINITY : x[i];
         float lowest;
         if (a.top_groups < a.G) keep_groups(a, c, r, g, lowest);
-        choose(a, c, x, e0, r, sub, a.k, out);
+        choose(a, c, e0, r, sub, a.k, out);
     } else {
         float bias[V];
 #pragma unroll
@@ -204,13 +200,13 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
             const float gap = keep_groups(a, c, r, g, lowest);                      // (of sums of up to two)
             again = !(gap > 2.f * unsure(lowest, a.sigmoid)) && !bad;
         }
-        choose(a, c, x, e0, r, sub, a.k + 1, out);
+        choose(a, c, e0, r, sub, a.k + 1, out);
         for (int j = sub; j < a.k; j += L) {
             const Chosen<float> p = out[j], q = out[j + 1];
             // (equal logits and biases are equal in 64 bits as well -- unless a third that is not may come between the last
             // that is chosen and the first that is not)
             if (q.e >= 0 && !(p.c - q.c > unsure(p.c, a.sigmoid)))
-                again |= j == a.k - 1 || !(p.x == q.x && (!a.bias || a.bias[p.e] == a.bias[q.e]));
+                again |= j == a.k - 1 || !((float)row[p.e] == (float)row[q.e] && (!a.bias || a.bias[p.e] == a.bias[q.e]));
         }
         wave_lds_fence();
         if (__ballot(again && on) != 0) {
@@ -235,10 +231,10 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
             }
             double lowest;
             if (a.top_groups < a.G) keep_groups(a, d, r, g, lowest);
-            choose(a, d, x, e0, r, sub, a.k, wide);
+            choose(a, d, e0, r, sub, a.k, wide);
             // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from)
             if (sub == 0)
-                for (int j = 0; j < a.k; ++j) { const Chosen<double> w = wide[j]; out[j] = Chosen<float>{(float)w.c, w.x, w.e}; }
+                for (int j = 0; j < a.k; ++j) { const Chosen<double> w = wide[j]; out[j] = Chosen<float>{(float)w.c, w.e}; }
             wave_lds_fence();
         }
     }
@@ -246,17 +242,17 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
     float m = 0.f, S = 1.f;
     if (a.renorm) {
         m = -INFINITY; S = 0.f;
-        for (int j = 0; j < a.k; ++j) if (out[j].e >= 0) m = fmaxf(m, out[j].x);
+        for (int j = 0; j < a.k; ++j) if (out[j].e >= 0) m = fmaxf(m, (float)row[out[j].e]);
         if (a.sigmoid) m = fminf(m, 0.f);
         for (int j = 0; j < a.k; ++j)
-            if (out[j].e >= 0) S += a.sigmoid ? sigmoid_over(out[j].x, m) : expf(out[j].x - m);
+            if (out[j].e >= 0) S += a.sigmoid ? sigmoid_over((float)row[out[j].e], m) : expf((float)row[out[j].e] - m);
     } else if (!a.sigmoid) {
         m = xmax; S = Z;
     }
     for (int j = sub; j < a.k; j += L) {
         int e = out[j].e;
         float w = 0.f;
-        if (e >= 0) w = a.scale * ((a.sigmoid ? sigmoid_over(out[j].x, m) : expf(out[j].x - m)) / S);
+        if (e >= 0) w = a.scale * ((a.sigmoid ? sigmoid_over((float)row[e], m) : expf((float)row[e] - m)) / S);
         if (!on) e = -1;
         else if (bad) { e = j; w = __builtin_nanf(""); }
         a.w[t * a.k + j] = w;
@@ -554,8 +550,9 @@ int nsx_expert_route_fwd(const void* logits, int dtype, int64_t T, int E, int64_
     const int Eg = E / n_groups, lg_G = lg2_ceil(n_groups);
     RouteArgs a{logits, row_stride, T, E, bias, selector, top_k, n_groups, top_groups, group_top, sigmoid, renormalise, scale,
                 weights, experts, n_device, 0, 0, fast_div(top_k)};
-    // 16 bytes per lane where the groups are whole numbers of them, else as few values per lane as 64 lanes allow
-    int V = 8;
+    // Values per lane: 16 leave the fewest exchanges and instructions per row, 4 the shortest chain for few rows.  us with 4 | 8 | 16:
+    // 2^20 x 32 fp32 top 2  64 | 41 | 38;  2^20 x 8 fp16 top 2  17 | 13 | 13;  65536 x 256 bf16 top 8  74 | 47 | 35;  1 x 64  5.3 | 5.6 | 6.9
+    int V = T <= 1024 ? 4 : Eg >= 32 ? 16 : 8;
     const int esize = dtype == NSX_DTYPE_F32 ? 4 : 2;
     while (V > 4 && Eg % V) V >>= 1;
     while (lg_G + lg2_ceil((Eg + V - 1) / V) > 6) V <<= 1;
