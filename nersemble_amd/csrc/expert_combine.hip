@@ -19,7 +19,8 @@ __device__ __forceinline__ int64_t valid_rows(int64_t T, const int64_t* n_dev) {
     return n < T ? (n < 0 ? 0 : n) : T;
 }
 
-template <typename T>
+// A thread makes 8 columns of a row; the KU choices of a round are read side by side, added in their order.
+template <typename T, int KU>
 __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __restrict__ out) {
     typedef typename Elem<T>::x8 x8;
     const int64_t total = valid_rows(a.T, a.n_dev) * a.chunks;
@@ -29,13 +30,24 @@ __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __re
         float s[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) s[q] = 0.f;
-        for (int j = 0; j < a.k; ++j) {
-            const int p = a.positions[t * a.k + j];
-            if ((unsigned)p >= (unsigned)a.R) continue;
-            const float w = a.w ? a.w[t * a.k + j] : 1.f;
-            const x8 v = *reinterpret_cast<const x8*>(reinterpret_cast<const T*>(a.y) + (int64_t)p * a.y_stride + c * 8);
+        for (int j = 0; j < a.k; j += KU) {
+            int p[KU];
+            float w[KU];
+            x8 v[KU];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) s[q] += w * (float)v[q];
+            for (int u = 0; u < KU; ++u) {
+                const bool in = KU <= 2 || j + u < a.k;
+                p[u] = in ? a.positions[t * a.k + j + u] : -1;
+                w[u] = in && a.w ? a.w[t * a.k + j + u] : 1.f;
+            }
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+                if ((unsigned)p[u] < (unsigned)a.R) v[u] = *reinterpret_cast<const x8*>(reinterpret_cast<const T*>(a.y) + (int64_t)p[u] * a.y_stride + c * 8);
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+                if ((unsigned)p[u] < (unsigned)a.R)
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) s[q] += w[u] * (float)v[u][q];
         }
         x8 o;
 #pragma unroll
@@ -81,6 +93,13 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(CombineArgs a, const T
         *reinterpret_cast<x8*>(dy + i * 8) = z;
 }
 
+template <typename T>
+static void combine_fwd_launch(const CombineArgs& a, T* out, unsigned grid, hipStream_t st) {
+    if (a.k == 1) combine_fwd_kernel<T, 1><<<grid, 256, 0, st>>>(a, out);
+    else if (a.k == 2) combine_fwd_kernel<T, 2><<<grid, 256, 0, st>>>(a, out);
+    else combine_fwd_kernel<T, 4><<<grid, 256, 0, st>>>(a, out);
+}
+
 }  // namespace nsx
 
 extern "C" {
@@ -108,8 +127,8 @@ int nsx_expert_combine_fwd(const void* y, int dtype, int64_t y_stride, int64_t R
     const int64_t blocks = (items + 255) / 256, most = (int64_t)num_cus() * 32;
     const unsigned grid = (unsigned)(blocks < most ? blocks : most);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == NSX_DTYPE_F16) combine_fwd_kernel<half_t><<<grid, 256, 0, st>>>(a, (half_t*)out);
-    else combine_fwd_kernel<bf16_t><<<grid, 256, 0, st>>>(a, (bf16_t*)out);
+    if (dtype == NSX_DTYPE_F16) combine_fwd_launch(a, (half_t*)out, grid, st);
+    else combine_fwd_launch(a, (bf16_t*)out, grid, st);
     NSX_LAUNCH_CHECK("nsx_expert_combine_fwd");
     return NSX_OK;
 }

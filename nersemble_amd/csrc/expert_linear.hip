@@ -389,6 +389,126 @@ __global__ __launch_bounds__(256) void expert_sum_chunks_kernel(LinArgs g, T* __
     }
 }
 
+// ---- narrow layers: at most 64 m and 64 q ------------------------------------------------------------------------------
+// Bound by memory: 32 -> 64 over 2^19 ordered rows reads 17 MB (from the caches, gathered) and writes 67.  No LDS and no barrier:
+// a wave keeps the whole matrix of its expert as fragments, reads 64 rows straight into the other operand's and stores whole
+// rows.  v_mfma_f32_16x16x32, D[m][c]: lane = row c of 16, four consecutive m per tile; the rows of P are dealt to the tiles so
+// that a lane's 4 MT values are consecutive (m = (lane / 16) 4 MT + 4 t + r).
+// us, tiles of 64 x 64 through LDS | this, 262144 rows x 2 of 16 experts, bf16 (dx with the ReLU's mask):
+//   forward  32 -> 64  30.2 | 23.7   64 -> 64  30.1 | 29.1   64 -> 16  26.1 | 16.0   (100000 x 2 of 61: 128 -> 64  18.6 | 24.2)
+//   dx       32 -> 64  35.9 | 27.7   64 -> 64  39.1 | 43.1   64 -> 16  28.7 | 22.8   16 -> 64  32.7 | 24.8
+// (dx gathers its matrix's fragments 2 bytes at a time, and with the mask's they leave fewer waves: up to 2048 weights.)
+constexpr int NARROW_ROWS = 256;      // ordered rows per workgroup of 4 waves
+
+template <typename T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mfma16<half_t>(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(Elem<half_t>::x8, a), __builtin_bit_cast(Elem<half_t>::x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mfma16<bf16_t>(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Elem<bf16_t>::x8, a), __builtin_bit_cast(Elem<bf16_t>::x8, b), c, 0, 0, 0);
+}
+
+template <typename T, int MODE, int MT, int QS, bool MASK>
+__global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, piece = lane >> 4;
+    int e, a, b;
+    if (!find_tile(g.offsets, g.E, g.R, NARROW_ROWS, blockIdx.x, e, a, b)) return;
+    a += wave * 64;
+    if (a >= b) return;
+    const bool nothing = e == g.E;
+    // rows of this wave, one to a lane
+    int row = min(a + lane, b - 1);
+    if (MODE == LIN_FWD && g.rows) { row = g.rows[row]; row = row >= 0 ? g.top_k(row) : -1; }
+    if (nothing || (MODE == LIN_FWD && row >= g.x_rows)) row = -1;
+    const char* Q = reinterpret_cast<const char*>(g.q);
+    const char* Y = reinterpret_cast<const char*>(g.mask);
+    u32x4 q[4][QS], y[MASK ? 4 : 1][MASK ? QS : 1];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int r = __shfl(row, u * 16 + c);
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const int at = s * 32 + piece * 8;
+            const bool in = r >= 0 && at < g.K;
+            q[u][s] = load16(in ? Q + ((int64_t)r * g.ldq + at) * 2 : zero_row());
+            if (MASK) y[u][s] = load16(in ? Y + ((int64_t)r * g.ldmask + at) * 2 : zero_row());
+        }
+    }
+    // the expert's matrix
+    u32x4 p[MT][QS];
+    const T* P = reinterpret_cast<const T*>(g.p) + (nothing ? 0 : e * g.p_expert);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = min((c >> 2) * (4 * MT) + t * 4 + (c & 3), g.M - 1);
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const int at = s * 32 + piece * 8;
+            if (MODE == LIN_FWD) p[t][s] = load16(at < g.K ? reinterpret_cast<const char*>(P + (int64_t)m * g.ldp + at) : zero_row());
+            else {
+                const uint16_t* w = reinterpret_cast<const uint16_t*>(P) + (int64_t)min(at, g.K - 8) * g.ldp + m;
+                // (q behind the end: whatever is here meets zeros of the other operand -- unless it is not finite: cleared)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const uint32_t v = (uint32_t)w[(2 * h) * g.ldp] | (uint32_t)w[(2 * h + 1) * g.ldp] << 16;
+                    p[t][s][h] = at < g.K ? v : 0u;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        if (a + u * 16 >= b) break;
+        f32x4 acc[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            if (MASK)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) q[u][s][w] = keep_where(q[u][s][w], y[u][s][w]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = mfma16<T>(p[t][s], q[u][s], acc[t]);
+        }
+        const int at = a + u * 16 + c, m = piece * (4 * MT);
+        if (at >= b) continue;
+        T out[4 * MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = acc[t][r];
+                if (MODE == LIN_FWD && g.relu) v = v <= 0.f ? 0.f : v;                  // (NaN stays)
+                out[t * 4 + r] = (T)v;
+            }
+        T* d = reinterpret_cast<T*>(g.d) + (int64_t)at * g.ldd + m;
+        if (MT == 1) {
+            if (m < g.M) *reinterpret_cast<u32x2*>(d) = *reinterpret_cast<const u32x2*>(out);
+        } else
+#pragma unroll
+            for (int h = 0; h < MT / 2; ++h)
+                if (m + h * 8 < g.M) *reinterpret_cast<u32x4*>(d + h * 8) = *reinterpret_cast<const u32x4*>(out + h * 8);
+    }
+}
+
+template <typename T, int MODE, int MT, int QS>
+static void narrow_launch_tile(const LinArgs& g, hipStream_t st) {
+    const unsigned blocks = (unsigned)(g.R / NARROW_ROWS + g.E + 1);
+    constexpr bool MAY_MASK = MODE != LIN_FWD;
+    if (MAY_MASK && g.mask) expert_narrow_kernel<T, MODE, MT, QS, MAY_MASK><<<blocks, 4 * kWave, 0, st>>>(g);
+    else expert_narrow_kernel<T, MODE, MT, QS, false><<<blocks, 4 * kWave, 0, st>>>(g);
+}
+template <typename T, int MODE, int MT>
+static void narrow_launch_m(const LinArgs& g, hipStream_t st) {
+    if (g.K <= 32) narrow_launch_tile<T, MODE, MT, 1>(g, st);
+    else narrow_launch_tile<T, MODE, MT, 2>(g, st);
+}
+template <typename T, int MODE>
+static void narrow_launch(const LinArgs& g, hipStream_t st) {
+    if (g.M <= 16) narrow_launch_m<T, MODE, 1>(g, st);
+    else if (g.M <= 32) narrow_launch_m<T, MODE, 2>(g, st);
+    else narrow_launch_m<T, MODE, 4>(g, st);
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------
 static int lin_check(const char* what, int dtype, int n_in, int n_out, int E, int64_t R, int top_k, const int32_t* offsets) {
     NSX_REQUIRE(dtype == NSX_DTYPE_F16 || dtype == NSX_DTYPE_BF16, "%s: dtype %d is not a 16-bit float", what, dtype);
@@ -460,6 +580,8 @@ static bool large_tiles(int64_t tiles128) { return tiles128 >= 6 * (int64_t)num_
 
 template <typename T, int MODE, bool F32>
 static int lin_launch(const LinArgs& g, bool small, hipStream_t st) {
+    if constexpr (MODE != LIN_DW)
+        if (g.M <= 64 && g.K <= 64 && (MODE == LIN_FWD || g.M * g.K <= 2048)) { narrow_launch<T, MODE>(g, st); return NSX_OK; }
     if (!g.mask && !F32) {              // (with a mask to apply they do not fit the registers)
         const int64_t tm = (g.M + 127) / 128;
         if (MODE != LIN_DW && g.M > 128 && large_tiles((g.R / 128 + std::min(g.E, g.R)) * tm)) return lin_launch_tile<T, MODE, 256, 128, 2, 2, F32>(g, st);
