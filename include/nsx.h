@@ -1059,16 +1059,15 @@ int nsx_expert_plan(const int32_t* experts, int64_t T, int top_k, int E, int32_t
 int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, int top_k,
                           const void* weight, int n_in, int n_out, int E, const int32_t* offsets, int64_t R, int relu, void* y,
                           void* stream);
-/* dx [R][n_in] in the plan's order (nsx_expert_combine_fwd without weights brings it to the rows).  y: the forward's result if
- * it had the ReLU (dy counts where y is not 0), else NULL. */
-int nsx_expert_linear_bwd_x(const void* dy, int dtype, int64_t dy_stride, const void* y, int64_t y_stride, const void* weight,
-                            int n_in, int n_out, int E, const int32_t* offsets, int64_t R, void* dx, void* stream);
-/* dw [E][n_out][n_in], of x's dtype or (dw_f32) in 32 bits; 0 for an expert without rows.  workspace:
- * nsx_expert_linear_bwd_w_workspace bytes (0: none). */
-int64_t nsx_expert_linear_bwd_w_workspace(int64_t R, int E, int n_in, int n_out);
-int nsx_expert_linear_bwd_w(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, int top_k,
-                            const void* dy, int64_t dy_stride, const void* y, int64_t y_stride, int n_in, int n_out, int E,
-                            const int32_t* offsets, int64_t R, int dw_f32, void* dw, void* workspace, void* stream);
+/* Gradients of the above.  dx (or NULL): [R][n_in] where x holds ordered rows (rows NULL), else [x_rows][n_in], a row's choices
+ * summed (rows without choices: 0).  dw (or NULL): [E][n_out][n_in], of x's dtype or (dw_f32) in 32 bits, 0 for an expert without
+ * rows.  y: the forward's result if it had the ReLU (dy counts where y is not 0), else NULL.  weight is read for dx, x for dw.
+ * workspace: nsx_expert_linear_bwd_workspace bytes (0: none). */
+int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int gather, int want_dw);
+int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, const int32_t* positions,
+                          int top_k, const void* weight, const void* dy, int64_t dy_stride, const void* y, int64_t y_stride, int n_in,
+                          int n_out, int E, const int32_t* offsets, int64_t R, void* dx, int dw_f32, void* dw, void* workspace,
+                          void* stream);
 /* out [T][n] = sum_j weights[t][j] * y[positions[t][j]] (weights NULL: 1); choices without a position count nothing.  Rows of
  * out behind n_device are not written. */
 int nsx_expert_combine_fwd(const void* y, int dtype, int64_t y_stride, int64_t R, int n, const float* weights,

@@ -617,65 +617,74 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
     return NSX_OK;
 }
 
-int nsx_expert_linear_bwd_x(const void* dy, int dtype, int64_t dy_stride, const void* y, int64_t y_stride, const void* weight,
-                            int n_in, int n_out, int E, const int32_t* offsets, int64_t R, void* dx, void* stream) {
-    using namespace nsx;
-    int rc = lin_check("nsx_expert_linear_bwd_x", dtype, n_in, n_out, E, R, 1, offsets);
-    if (rc != NSX_OK) return rc;
-    if (R == 0) return NSX_OK;
-    NSX_REQUIRE(dy && weight && dx && aligned16(dy) && aligned16(y) && aligned16(weight) && aligned16(dx) && lin_stride(dy_stride, n_out) &&
-                    (!y || lin_stride(y_stride, n_out)),
-                "nsx_expert_linear_bwd_x: NULL or unaligned pointer or row stride");
-    LinArgs g{};
-    g.p = weight; g.q = dy; g.mask = y; g.d = dx; g.ldp = n_in; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in;
-    g.p_expert = (int64_t)n_in * n_out; g.offsets = offsets; g.E = E; g.R = (int)R; g.x_rows = (int)R;
-    g.M = n_in; g.K = n_out;
-    rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(g, small_tiles(g), (hipStream_t)stream)
-                                 : lin_launch<bf16_t, LIN_DX, false>(g, small_tiles(g), (hipStream_t)stream);
-    if (rc != NSX_OK) return rc;
-    NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_x");
-    return NSX_OK;
-}
-
-int64_t nsx_expert_linear_bwd_w_workspace(int64_t R, int E, int n_in, int n_out) {
-    using namespace nsx;
-    int32_t some = 0;
-    const int rc = lin_check("nsx_expert_linear_bwd_w_workspace", NSX_DTYPE_F16, n_in, n_out, E, R, 1, &some);
-    if (rc != NSX_OK) return rc;
-    const int chunk = dw_plan(R, E, n_in, n_out).chunk;
+// workspace: dx in the plan's order (16-byte steps), then dW's partial sums
+static int64_t bwd_dx_bytes(int64_t R, int n_in, bool gather) { return gather ? R * n_in * 2 : 0; }
+static int64_t bwd_dw_bytes(int64_t R, int E, int n_in, int n_out) {
+    const int chunk = nsx::dw_plan(R, E, n_in, n_out).chunk;
     return chunk > 0 ? (R / chunk + E) * n_in * n_out * 4 : 0;
 }
 
-int nsx_expert_linear_bwd_w(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, int top_k,
-                            const void* dy, int64_t dy_stride, const void* y, int64_t y_stride, int n_in, int n_out, int E,
-                            const int32_t* offsets, int64_t R, int dw_f32, void* dw, void* workspace, void* stream) {
+int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int gather, int want_dw) {
     using namespace nsx;
-    int rc = lin_check("nsx_expert_linear_bwd_w", dtype, n_in, n_out, E, R, top_k, offsets);
+    int32_t some = 0;
+    const int rc = lin_check("nsx_expert_linear_bwd_workspace", NSX_DTYPE_F16, n_in, n_out, E, R, 1, &some);
     if (rc != NSX_OK) return rc;
-    NSX_REQUIRE(dw && aligned16(dw) && (R == 0 || dy) && (x || x_rows == 0) && aligned16(x) && aligned16(dy) && aligned16(y) &&
-                    lin_stride(x_stride, n_in) && lin_stride(dy_stride, n_out) && (!y || lin_stride(y_stride, n_out)),
-                "nsx_expert_linear_bwd_w: NULL or unaligned pointer or row stride");
-    NSX_REQUIRE(x_rows >= 0 && x_rows <= NSX_MAX_EXPERT_ENTRIES && (rows || x_rows == R), "nsx_expert_linear_bwd_w: x has %lld rows", (long long)x_rows);
-    LinArgs g{};
-    const DwPlan how = dw_plan(R, E, n_in, n_out);
-    g.chunk = how.chunk;
-    NSX_REQUIRE(g.chunk == 0 || (workspace && aligned16(workspace)), "nsx_expert_linear_bwd_w: no workspace");
-    g.p = x; g.q = dy; g.mask = y; g.d = dw; g.ldp = x_stride; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in;
-    g.d_expert = (int64_t)n_in * n_out; g.offsets = offsets; g.rows = rows; g.top_k = fast_div(top_k); g.E = E; g.R = (int)R;
-    g.x_rows = (int)x_rows; g.M = n_in; g.C = n_out; g.partial = (float*)workspace;
+    return (want_dx ? bwd_dx_bytes(R, n_in, gather) : 0) + (want_dw ? bwd_dw_bytes(R, E, n_in, n_out) : 0);
+}
+
+int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, const int32_t* positions,
+                          int top_k, const void* weight, const void* dy, int64_t dy_stride, const void* y, int64_t y_stride, int n_in,
+                          int n_out, int E, const int32_t* offsets, int64_t R, void* dx, int dw_f32, void* dw, void* workspace,
+                          void* stream) {
+    using namespace nsx;
+    int rc = lin_check("nsx_expert_linear_bwd", dtype, n_in, n_out, E, R, top_k, offsets);
+    if (rc != NSX_OK) return rc;
+    NSX_REQUIRE(x_rows >= 0 && x_rows <= NSX_MAX_EXPERT_ENTRIES / top_k && (rows ? x_rows * top_k == R : x_rows == R),
+                "nsx_expert_linear_bwd: x has %lld rows", (long long)x_rows);
+    NSX_REQUIRE((R == 0 || dy) && aligned16(dy) && aligned16(y) && lin_stride(dy_stride, n_out) && (!y || lin_stride(y_stride, n_out)),
+                "nsx_expert_linear_bwd: NULL or unaligned dy or y, or their row strides");
+    NSX_REQUIRE(!dx || (aligned16(dx) && (R == 0 || (weight && aligned16(weight) && (!rows || positions)))),
+                "nsx_expert_linear_bwd: dx needs aligned pointers, weight and, for gathered rows, positions");
+    NSX_REQUIRE(!dw || (aligned16(dw) && (x || x_rows == 0) && aligned16(x) && lin_stride(x_stride, n_in)),
+                "nsx_expert_linear_bwd: dw needs aligned pointers and x (row stride %lld)", (long long)x_stride);
+    const int64_t dx_bytes = dx ? bwd_dx_bytes(R, n_in, rows) : 0;
+    NSX_REQUIRE(dx_bytes + (dw ? bwd_dw_bytes(R, E, n_in, n_out) : 0) == 0 || (workspace && aligned16(workspace)),
+                "nsx_expert_linear_bwd: no workspace");
     hipStream_t st = (hipStream_t)stream;
-    const bool f32 = dw_f32 || g.chunk > 0;
-    if (dtype == NSX_DTYPE_F16) rc = f32 ? lin_launch<half_t, LIN_DW, true>(g, how.small, st) : lin_launch<half_t, LIN_DW, false>(g, how.small, st);
-    else rc = f32 ? lin_launch<bf16_t, LIN_DW, true>(g, how.small, st) : lin_launch<bf16_t, LIN_DW, false>(g, how.small, st);
-    if (rc != NSX_OK) return rc;
-    NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_w");
-    if (g.chunk > 0) {
-        const int64_t step = R / g.chunk > 8 * (int64_t)E ? 64 : 1024;
-        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)n_in * n_out + step - 1) / step, 4096), E);
-        if (dw_f32) expert_sum_chunks_kernel<float><<<grid, 256, 0, st>>>(g, (float*)dw);
-        else if (dtype == NSX_DTYPE_F16) expert_sum_chunks_kernel<half_t><<<grid, 256, 0, st>>>(g, (half_t*)dw);
-        else expert_sum_chunks_kernel<bf16_t><<<grid, 256, 0, st>>>(g, (bf16_t*)dw);
-        NSX_LAUNCH_CHECK("nsx_expert_linear_bwd_w");
+    LinArgs g{};
+    g.q = dy; g.mask = y; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in; g.offsets = offsets; g.top_k = fast_div(top_k);
+    g.E = E; g.R = (int)R; g.M = n_in;
+    if (dx && R > 0) {
+        LinArgs h = g;
+        h.p = weight; h.ldp = n_in; h.p_expert = (int64_t)n_in * n_out; h.d = rows ? workspace : dx; h.x_rows = (int)R; h.K = n_out;
+        rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(h, small_tiles(h), st) : lin_launch<bf16_t, LIN_DX, false>(h, small_tiles(h), st);
+        if (rc != NSX_OK) return rc;
+        NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
+        // A row's choices are summed in 32 bits; their gradients lie in 16 bits between the two launches (in 32 they would be twice
+        // the traffic): off by at most half a step of each term beside the sum's own rounding.
+        if (rows) {
+            rc = nsx_expert_combine_fwd(workspace, dtype, n_in, R, n_in, nullptr, positions, x_rows, top_k, dx, nullptr, stream);
+            if (rc != NSX_OK) return rc;
+        }
+    }
+    if (dw) {
+        const DwPlan how = dw_plan(R, E, n_in, n_out);
+        g.chunk = how.chunk;
+        g.p = x; g.ldp = x_stride; g.d = dw; g.d_expert = (int64_t)n_in * n_out; g.rows = rows; g.x_rows = (int)x_rows; g.C = n_out;
+        g.partial = reinterpret_cast<float*>((char*)workspace + dx_bytes);
+        const bool f32 = dw_f32 || g.chunk > 0;
+        if (dtype == NSX_DTYPE_F16) rc = f32 ? lin_launch<half_t, LIN_DW, true>(g, how.small, st) : lin_launch<half_t, LIN_DW, false>(g, how.small, st);
+        else rc = f32 ? lin_launch<bf16_t, LIN_DW, true>(g, how.small, st) : lin_launch<bf16_t, LIN_DW, false>(g, how.small, st);
+        if (rc != NSX_OK) return rc;
+        NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
+        if (g.chunk > 0) {
+            const int64_t step = R / g.chunk > 8 * (int64_t)E ? 64 : 1024;
+            const dim3 grid((unsigned)std::min<int64_t>(((int64_t)n_in * n_out + step - 1) / step, 4096), E);
+            if (dw_f32) expert_sum_chunks_kernel<float><<<grid, 256, 0, st>>>(g, (float*)dw);
+            else if (dtype == NSX_DTYPE_F16) expert_sum_chunks_kernel<half_t><<<grid, 256, 0, st>>>(g, (half_t*)dw);
+            else expert_sum_chunks_kernel<bf16_t><<<grid, 256, 0, st>>>(g, (bf16_t*)dw);
+            NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
+        }
     }
     return NSX_OK;
 }

@@ -11,6 +11,7 @@ module built on these calls.)  All four launch on torch's current stream, keep n
 ``_lib.device_count`` rows behind the device-side count are not routed, and not written by ``route_experts`` and
 ``expert_combine``.  A plan's numbers are bounded inside the kernels; equal inputs give equal bits.
 """
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -166,6 +167,14 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
 # ------------------------------------------------------------------------------------------------
 # plan
 # ------------------------------------------------------------------------------------------------
+@lru_cache(maxsize=1024)
+def _plan_bytes(n_entries, n_experts):
+    n = lib().nsx_expert_plan_workspace(n_entries, n_experts)
+    if n < 0:
+        check(n, "nsx_expert_plan_workspace")
+    return n
+
+
 def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
     """The plan of ``chosen`` [T, top_k] int32 (``route_experts``): a stable sort of its entries by expert.  Entries outside
     [0, n_experts) are not routed."""
@@ -173,10 +182,8 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
         raise RuntimeError(f"expert_plan: chosen is [T, top_k] int32 (got {tuple(chosen.shape)} {chosen.dtype})")
     chosen = chosen.contiguous()
     T, k = chosen.shape
-    dev, n_experts = chosen.device, int(n_experts)
-    need = int(lib().nsx_expert_plan_workspace(T * k, n_experts))
-    if need < 0:
-        check(need, "nsx_expert_plan_workspace")
+    n_experts = int(n_experts)
+    need = _plan_bytes(T * k, n_experts)
     # one allocation: offsets | rows | positions | workspace (16-byte steps)
     o, r = -(-(n_experts + 1) // 4) * 4, -(-(T * k) // 4) * 4
     dev = _here(chosen)
@@ -200,32 +207,29 @@ def _linear(x, x_stride, w16, plan, gather, relu):
     return y
 
 
+@lru_cache(maxsize=1024)
+def _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w):
+    n = lib().nsx_expert_linear_bwd_workspace(R, E, K, N, need_x, gather, need_w)
+    if n < 0:
+        check(n, "nsx_expert_linear_bwd_workspace")
+    return n
+
+
 def _linear_bwd(ctx, dy):
     x, w16, y, offsets, rows, positions = ctx.saved_tensors
     x_stride, x_rows, (E, N, K), gather, w_dtype, need_x, need_w = ctx.cfg
     R, top_k = rows.shape[0], positions.shape[1]
     g, g_stride = _rows_of(dy, 8)
-    dev, code, L = _here(g), _DTYPE[g.dtype], lib()
-    stream = _raw_stream(dev)
-    g_at, o_at, y_at = g.data_ptr(), _at(offsets, dev), None if y is None else _at(y, dev)
-    dx = dw = None
-    if need_x:
-        dx = torch.empty((R, K), dtype=g.dtype, device=g.device)
-        check(L.nsx_expert_linear_bwd_x(g_at, code, g_stride, y_at, N, _at(w16, dev), K, N, E, o_at, R, dx.data_ptr(), stream),
-              "nsx_expert_linear_bwd_x")
-        if gather:
-            # a row's choices summed in 32 bits; their gradients lie in 16 bits between the two launches (twice the
-            # memory traffic otherwise): an error of at most half a step of each term beside the sum's own rounding
-            dx = _combine(dx, K, None, positions)
-    if need_w:
-        need = L.nsx_expert_linear_bwd_w_workspace(R, E, K, N)
-        if need < 0:
-            check(need, "nsx_expert_linear_bwd_w_workspace")
-        ws = torch.empty((need,), dtype=torch.uint8, device=g.device) if need else None
-        dw = torch.empty((E, N, K), dtype=w_dtype, device=g.device)
-        check(L.nsx_expert_linear_bwd_w(_at(x, dev), code, x_stride, x_rows, _at(rows, dev) if gather else None, top_k, g_at, g_stride,
-                                        y_at, N, K, N, E, o_at, R, w_dtype == _F32, dw.data_ptr(),
-                                        None if ws is None else ws.data_ptr(), stream), "nsx_expert_linear_bwd_w")
+    dev, place = _here(g), g.device
+    need = _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w)
+    ws = torch.empty((need,), dtype=torch.uint8, device=place) if need else None
+    dx = torch.empty((x_rows, K), dtype=g.dtype, device=place) if need_x else None
+    dw = torch.empty((E, N, K), dtype=w_dtype, device=place) if need_w else None
+    check(lib().nsx_expert_linear_bwd(
+        _at(x, dev) if need_w else None, _DTYPE[g.dtype], x_stride, x_rows, _at(rows, dev) if gather else None, _at(positions, dev), top_k,
+        _at(w16, dev) if need_x else None, g.data_ptr(), g_stride, None if y is None else _at(y, dev), N, K, N, E, _at(offsets, dev), R,
+        dx.data_ptr() if need_x else None, w_dtype == _F32, dw.data_ptr() if need_w else None, ws.data_ptr() if need else None,
+        _raw_stream(dev)), "nsx_expert_linear_bwd")
     return dx, dw, None, None, None, None
 
 

@@ -97,10 +97,10 @@ def test_c_abi_refuses_bad_arguments():
     _refused(route(scale=float("nan")), "scale")
     _refused(route(logits=None), "NULL")
     assert route(T=0) == 0
-    bwd = lambda **o: L.nsx_expert_route_bwd(o.get("x", P), 0, o.get("T", 4), 16, o.get("s", 16), 2, 0, 1, 1.0, P, P, o.get("g", P), P, None, None)  # noqa: E731
-    _refused(bwd(s=3), "stride")
-    _refused(bwd(g=None), "NULL")
-    assert bwd(T=0) == 0
+    rbwd = lambda **o: L.nsx_expert_route_bwd(o.get("x", P), 0, o.get("T", 4), 16, o.get("s", 16), 2, 0, 1, 1.0, P, P, o.get("g", P), P, None, None)  # noqa: E731
+    _refused(rbwd(s=3), "stride")
+    _refused(rbwd(g=None), "NULL")
+    assert rbwd(T=0) == 0
     _refused(L.nsx_expert_plan_workspace(-1, 4), "entries")
     _refused(L.nsx_expert_plan_workspace(4, 0), "n_experts")
     assert L.nsx_expert_plan_workspace(4096, 16) > 0
@@ -122,12 +122,29 @@ def test_c_abi_refuses_bad_arguments():
     _refused(lin(rows=None), "rows")
     _refused(lin(R=1 << 31), "ordered rows")
     assert lin(R=0) == 0
-    _refused(L.nsx_expert_linear_bwd_x(P, 1, 60, None, 0, P, 32, 64, 4, P, 16, P, None), "stride")
-    _refused(L.nsx_expert_linear_bwd_x(P, 1, 64, P, 8, P, 32, 64, 4, P, 16, P, None), "stride")
-    _refused(L.nsx_expert_linear_bwd_w(P, 1, 32, 8, None, 2, P, 64, None, 0, 32, 64, 4, P, 16, 0, P, None, None), "x has 8 rows")
-    _refused(L.nsx_expert_linear_bwd_w(P, 1, 32, 8, P, 2, P, 64, None, 0, 32, 64, 4, P, 16, 0, None, None, None), "NULL")
-    _refused(L.nsx_expert_linear_bwd_w(P, 1, 32, 1 << 20, P, 2, P, 64, None, 0, 32, 64, 4, P, 1 << 21, 0, P, None, None), "workspace")
-    _refused(L.nsx_expert_linear_bwd_w_workspace(16, 4, 33, 64), "multiples of 8")
+
+    def bwd(x=P, dtype=1, x_stride=32, x_rows=8, rows=P, positions=P, k=2, w=P, dy=P, dy_stride=64, y=None, y_stride=0, K=32, N=64, E=4,
+            R=16, dx=P, dw=P, ws=P):
+        return L.nsx_expert_linear_bwd(x, dtype, x_stride, x_rows, rows, positions, k, w, dy, dy_stride, y, y_stride, K, N, E, P, R, dx, 0,
+                                       dw, ws, None)
+    _refused(bwd(dtype=0), "16-bit")
+    _refused(bwd(dy_stride=60), "strides")
+    _refused(bwd(dy_stride=(1 << 20) + 8), "strides")
+    _refused(bwd(y=P, y_stride=8), "strides")
+    _refused(bwd(dy=None), "NULL")
+    _refused(bwd(x_rows=7), "x has 7 rows")
+    _refused(bwd(rows=None), "x has 8 rows")
+    _refused(bwd(positions=None), "positions")
+    _refused(bwd(w=None), "weight")
+    _refused(bwd(x=None), "dw needs")
+    _refused(bwd(x_stride=24), "dw needs")
+    _refused(bwd(dw=ctypes.c_void_p(8)), "dw needs")
+    _refused(bwd(ws=None), "workspace")
+    _refused(bwd(x_rows=1 << 20, R=1 << 21, dx=None, ws=None), "workspace")
+    assert bwd(R=0, x_rows=0, dw=None) == 0 and bwd(dx=None, dw=None) == 0
+    _refused(L.nsx_expert_linear_bwd_workspace(16, 4, 33, 64, 1, 1, 1), "multiples of 8")
+    assert L.nsx_expert_linear_bwd_workspace(16, 4, 32, 64, 1, 1, 0) == 16 * 32 * 2
+    assert L.nsx_expert_linear_bwd_workspace(16, 4, 32, 64, 1, 0, 0) == 0
     _refused(L.nsx_expert_combine_fwd(P, 1, 60, 16, 64, None, P, 8, 2, P, None, None), "stride")
     _refused(L.nsx_expert_combine_fwd(P, 0, 64, 16, 64, None, P, 8, 2, P, None, None), "16-bit")
     _refused(L.nsx_expert_combine_fwd(P, 1, 64, 16, 64, None, None, 8, 2, P, None, None), "NULL")
