@@ -121,6 +121,21 @@ __device__ __forceinline__ bool lin_order(int tiles, int m_tiles, int block, int
     tile = group * LIN_GROUP + rest - m * n;
     return true;
 }
+// The expert with the rank-th most rows (up to 64 experts; of more, simply the rank-th): the longest sums start first and do not
+// end alone.
+__device__ __forceinline__ int expert_by_size(const int32_t* __restrict__ offsets, int E, int R, int rank) {
+    if (E > kWave) return rank;
+    const int lane = threadIdx.x & 63;
+    int a = 0, b = 0;
+    if (lane < E) segment(offsets, lane, R, a, b);
+    const int n = b - a;
+    int before = 0;
+    for (int e = 0; e < E; ++e) {
+        const int other = __builtin_amdgcn_readlane(n, e);
+        before += (other > n || (other == n && e < lane)) ? 1 : 0;
+    }
+    return __ffsll((unsigned long long)__ballot(lane < E && before == rank)) - 1;
+}
 // dW: an XCD takes blocks of up to 4 x 4 tiles of one segment (or chunk of one) in turn with the others.  (No workgroups for
 // tiles that are not there: of blocks of 16 with one tile each, the working ones fell on two of an XCD's 32 CUs.)
 __host__ __device__ __forceinline__ int lin_group_dw(int tiles) { return tiles < 4 ? tiles : 4; }
@@ -151,7 +166,7 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
             if (chunk >= g.R / g.chunk + g.E || !find_tile(g.offsets, g.E, g.R, g.chunk, chunk, e, a, b) || e == g.E) return;
         } else {
             if (chunk >= g.E) return;
-            e = chunk;
+            e = expert_by_size(g.offsets, g.E, g.R, chunk);
             segment(g.offsets, e, g.R, a, b);
         }
     } else {
