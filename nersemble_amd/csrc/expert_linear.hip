@@ -552,7 +552,7 @@ static int lin_launch_tile(LinArgs g, hipStream_t st) {
         blocks = ((int64_t)g.R / TC + g.E + 1) * g.m_tiles;
         blocks = (blocks + 7) / 8 * 8;
     }
-    NSX_REQUIRE(blocks <= 0x7fffffff, "expert_linear: %lld tiles", (long long)blocks);
+    NSX_REQUIRE(blocks * (WM * WC * kWave) < ((int64_t)1 << 32), "expert_linear: %lld tiles are more than one launch", (long long)blocks);
     constexpr bool MAY_MASK = MODE != LIN_FWD && TM * TC <= 128 * 128;
     if (MAY_MASK && g.mask) expert_linear_kernel<T, MODE, TM, TC, WM, WC, MAY_MASK, F32><<<(unsigned)blocks, WM * WC * kWave, lds, st>>>(g);
     else expert_linear_kernel<T, MODE, TM, TC, WM, WC, false, F32><<<(unsigned)blocks, WM * WC * kWave, lds, st>>>(g);

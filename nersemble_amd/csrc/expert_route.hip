@@ -559,6 +559,8 @@ int nsx_expert_route_fwd(const void* logits, int dtype, int64_t T, int E, int64_
     const bool vec = route_vec(logits, V, esize, row_stride, Eg);
     a.lg_Lg = lg2_ceil((Eg + V - 1) / V);
     a.lg_L = lg_G + a.lg_Lg;
+    NSX_REQUIRE((T << a.lg_L) + 256 < ((int64_t)1 << 32), "nsx_expert_route_fwd: %lld rows of %d lanes are more than one launch",
+                (long long)T, 1 << a.lg_L);
     const bool wide = bias || (top_groups < n_groups && group_top == 2);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype * 32 + V) {
@@ -591,6 +593,8 @@ int nsx_expert_route_bwd(const void* logits, int dtype, int64_t T, int E, int64_
     const int V = E % 8 && E <= 256 ? 4 : 8;
     const bool vec = route_vec(logits, V, esize, row_stride, E) && route_vec(dlogits, V, esize, E, E);
     a.lg_L = lg2_ceil((E + V - 1) / V);
+    NSX_REQUIRE((T << a.lg_L) + 256 < ((int64_t)1 << 32), "nsx_expert_route_bwd: %lld rows of %d lanes are more than one launch",
+                (long long)T, 1 << a.lg_L);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype * 32 + V) {
         case 4: launch_route_bwd<float, 4>(a, vec, dweights, dlogits, st); break;

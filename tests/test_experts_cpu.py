@@ -96,6 +96,7 @@ def test_c_abi_refuses_bad_arguments():
     _refused(route(scale=0.0), "scale")
     _refused(route(scale=float("nan")), "scale")
     _refused(route(logits=None), "NULL")
+    _refused(route(T=1 << 27, E=512, stride=512), "one launch")
     assert route(T=0) == 0
     rbwd = lambda **o: L.nsx_expert_route_bwd(o.get("x", P), 0, o.get("T", 4), 16, o.get("s", 16), 2, 0, 1, 1.0, P, P, o.get("g", P), P, None, None)  # noqa: E731
     _refused(rbwd(s=3), "stride")

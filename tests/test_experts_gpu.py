@@ -570,3 +570,129 @@ def test_routed_network(n_in, n_out, n_hidden, routing, cuda):
     else:
         with pytest.raises(RuntimeError):
             net.rebalance()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# corners
+# ---------------------------------------------------------------------------------------------------------------------
+def test_no_rows_at_all(cuda):
+    """Zero rows: empty results, a weight gradient of zeros, through every call."""
+    from nersemble_amd import experts as X
+    E, K, N = 3, 32, 48
+    for k in (1, 2):
+        logits = torch.empty((0, E), device=cuda, requires_grad=True)
+        w, c = X.route_experts(logits, k)
+        plan = X.expert_plan(c, E)
+        x = torch.empty((0, K), dtype=torch.float16, device=cuda, requires_grad=True)
+        m = torch.randn((E, N, K), device=cuda).half().requires_grad_(True)
+        y = X.expert_linear(x, m, plan, relu=True)
+        out = X.expert_combine(y, w, plan)
+        assert w.shape == (0, k) and y.shape == (0, N) and out.shape == (0, N) and (plan.offsets == 0).all()
+        dl, dx, dm = torch.autograd.grad(out, [logits, x, m], torch.empty_like(out))
+        assert dl.shape == (0, E) and dx.shape == (0, K) and (dm == 0).all()
+
+
+def test_gradients_of_some_inputs_only(cuda):
+    """Each input's gradient alone is the one that is computed beside the others'."""
+    from nersemble_amd import experts as X
+    (x, logits, w1, w2), go = _mixture_inputs(150, 5, 32, 64, 16, 9, cuda)
+    full = torch.autograd.grad(_mixture(x, logits, w1, w2, 5, 2), [x, logits, w1, w2], go)
+    for n in range(4):
+        leaves = [v.detach().requires_grad_(i == n) for i, v in enumerate((x, logits, w1, w2))]
+        (g,) = torch.autograd.grad(_mixture(*leaves, 5, 2), [leaves[n]], go)
+        assert torch.equal(g, full[n])
+    # and a second differentiation is refused, not wrong
+    g = torch.autograd.grad(_mixture(x, logits, w1, w2, 5, 2), [w1], go, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.float().sum(), [x])
+
+
+def test_what_is_not_routed_is_not_read(cuda):
+    """Rows, gradients and outputs that no segment holds may be anything."""
+    from nersemble_amd import experts as X
+    nan = float("nan")
+    T, E, k = 300, 4, 2
+    (x, logits, w1, w2), go = _mixture_inputs(T, E, 32, 64, 16, 10, cuda)
+    sel = (torch.arange(T, device=cuda) % 3 > 0).to(torch.uint8)
+    off = sel == 0
+    want = _mixture(x, logits, w1, w2, E, k, sel)
+    wg = torch.autograd.grad(want, [x, logits, w1, w2], go)
+    x2, l2, go2 = x.detach().clone(), logits.detach().clone(), go.clone()
+    x2[off], l2[off], go2[off] = nan, nan, nan
+    leaves = [v.detach().requires_grad_(True) for v in (x2, l2, w1, w2)]
+    got = _mixture(*leaves, E, k, sel)
+    gg = torch.autograd.grad(got, leaves, go2)
+    assert torch.equal(got, want) and (got[off] == 0).all()
+    for a, b in zip(gg, wg):
+        assert torch.equal(a, b)
+    # the gradient of a product's rows behind the last segment
+    _, c = X.route_experts(l2, k, selector=sel)
+    plan = X.expert_plan(c, E)
+    xa, wa = x.detach().requires_grad_(True), w1.detach().requires_grad_(True)
+    y = X.expert_linear(xa, wa, plan)
+    n = int(plan.offsets[-1])
+    dy = torch.randn(y.shape, device=cuda).half()
+    a = torch.autograd.grad(y, [xa, wa], dy, retain_graph=True)
+    dy[n:] = nan
+    b = torch.autograd.grad(y, [xa, wa], dy)
+    assert n < y.shape[0] and (y[n:] == 0).all() and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_more_than_2_31_elements(cuda):
+    """Ordered rows whose elements pass 2^31 (and whose bytes pass 2^32): products, gradients and join at the far end."""
+    from nersemble_amd import experts as X
+    T, E, K, N = (1 << 20) + 5, 3, 8, 2056
+    g = torch.Generator(device=cuda).manual_seed(0)
+    c = torch.randint(0, E, (T, 1), generator=g, device=cuda, dtype=torch.int32)
+    plan = X.expert_plan(c, E)
+    x = torch.randn((T, K), generator=g, device=cuda).half().requires_grad_(True)
+    w = torch.randn((E, N, K), generator=g, device=cuda).half().requires_grad_(True)
+    y = X.expert_linear(x, w, plan)
+    assert y.numel() > 2 ** 31
+    last = plan.rows[-200:].long()
+    want = x.detach().float()[last] @ w.detach().float()[E - 1].t()
+    tol = 2.0 ** -11 * want.abs() + 2.0 ** -25 + (K + 2) * 2 * U * (x.detach().float().abs()[last] @ w.detach().float().abs()[E - 1].t())
+    assert ((y.detach()[-200:].float() - want).abs() <= tol).all()
+    wt = torch.ones((T, 1), device=cuda)
+    out = X.expert_combine(y.detach(), wt, plan)
+    assert torch.equal(out[last], y.detach()[-200:])
+    del out
+    # dx of the last rows alone: dy is zero before them (a sum over 2056 outputs), dW then is theirs as well
+    dy = torch.zeros_like(y)
+    dy[-200:] = torch.randn((200, N), generator=g, device=cuda).half()
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    far = dy[-200:].float()
+    want = far @ w.detach().float()[E - 1]
+    tol = 2 * (2.0 ** -11 * want.abs() + 2.0 ** -25) + (N + 2) * 2 * U * (far.abs() @ w.detach().float().abs()[E - 1])
+    assert ((dx[last].float() - want).abs() <= tol).all() and int((dx != 0).any(1).sum()) == 200
+    want = far.t() @ x.detach().float()[last]
+    tol = 2.0 ** -11 * want.abs() + 2.0 ** -25 + (200 + 66) * 2 * U * (far.abs().t() @ x.detach().float().abs()[last])
+    assert ((dw[E - 1].float() - want).abs() <= tol).all() and (dw[:E - 1] == 0).all()
+
+
+def test_route_choice_where_32_bits_do_not_tell(cuda):
+    """Scores plus a bias that lie closer than 32 bits resolve, and equal ones: the choice is that of 64 bits."""
+    from nersemble_amd import experts as X
+    rng = np.random.default_rng(4)
+    for E, G, tg, gt in ((64, 1, 1, 1), (64, 8, 3, 2), (256, 8, 4, 2)):
+        x = (rng.standard_normal((257, E)) * 0.5).astype(np.float32)
+        # neighbours one step of fp32 apart, in a shuffled order
+        for t in range(0, 257, 2):
+            base = np.float32(rng.standard_normal())
+            x[t] = base + np.float32(2.0 ** -22) * rng.permutation(E).astype(np.float32)
+        x[1::4] = np.round(x[1::4] * 4) / 4                                   # many equal
+        for bias in (np.zeros(E, np.float32), (rng.integers(0, 3, E) * 2.0 ** -20).astype(np.float32)):
+            for sc in ("sigmoid", "softmax"):
+                w, c = X.route_experts(torch.from_numpy(x).to(cuda), 6, scores=sc, bias=torch.from_numpy(bias).to(cuda), n_groups=G, top_groups=tg, group_top=gt)
+                s = ox.scores(x, sc == "sigmoid") + bias
+                _, wc = ox.route(x, 6, sc == "sigmoid", bias, G, tg, gt)
+                got = c.cpu().numpy()
+                # (64-bit sums of a softmax depend on their order by 1e-16: a row counts where no two values are that close but not equal)
+                v = np.sort(s, axis=1)
+                d = np.diff(v, axis=1)
+                clear = ~((d > 0) & (d < 1e-13)).any(1)
+                if G > 1:
+                    by = np.sort(np.sort(s.reshape(len(s), G, -1), axis=2)[:, :, -gt:].sum(2), axis=1)
+                    dg = np.diff(by, axis=1)
+                    clear &= ~((dg > 0) & (dg < 1e-13)).any(1)
+                assert clear.mean() > 0.5 and np.array_equal(got[clear], wc[clear]), (E, G, sc)
