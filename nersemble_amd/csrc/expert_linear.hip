@@ -484,9 +484,12 @@ __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t] = mfma16<T>(p[t][s], q[u][s], acc[t]);
         }
+        if (nothing)                                      // (the first expert's matrix may hold what is not finite)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int at = a + u * 16 + c, m = piece * (4 * MT);
         if (at >= b) continue;
-        T out[4 * MT];
+        alignas(16) T out[4 * MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -591,6 +594,8 @@ static DwPlan dw_plan(int64_t R, int E, int n_in, int n_out) {
 //   16384 x 2 of 16, 1024 -> 2048   forward 172 | 162 | 173   dx 158 | 152 | 158   dW 177 | 178 | 166
 //   16384 x 2 of 8,  2048 -> 2048   forward 322 | 292 | 306   dx 304 | 287 | 289   dW 328 | 318 | 303
 //    8192 x 2 of 16, 1024 -> 1024   forward  52 |  56 |  58   dx  48 |  51 |  51   dW  59 |  62 |  57
+//    2048 x 8 of 256, 2048 -> 1024  forward 221 | 208 |       dx 259 | 223     (64 x 64: 283, 282)
+// Where segments have a few rows the 64 x 64 tiles stay: 64 x 8 of 256, 1024 -> 2048: forward 147 | 163 (256 x 128), dx 144 | 149.
 static bool large_tiles(int64_t tiles128) { return tiles128 >= 6 * (int64_t)num_cus(); }
 
 template <typename T, int MODE, bool F32>
@@ -599,7 +604,7 @@ static int lin_launch(const LinArgs& g, bool small, hipStream_t st) {
         if (g.M <= 64 && g.K <= 64 && (MODE == LIN_FWD || g.M * g.K <= 2048)) { narrow_launch<T, MODE>(g, st); return NSX_OK; }
     if (!g.mask && !F32) {              // (with a mask to apply they do not fit the registers)
         const int64_t tm = (g.M + 127) / 128;
-        if (MODE != LIN_DW && g.M > 128 && large_tiles((g.R / 128 + std::min(g.E, g.R)) * tm)) return lin_launch_tile<T, MODE, 256, 128, 2, 2, F32>(g, st);
+        if (MODE != LIN_DW && !small && g.M > 128 && large_tiles((g.R / 128 + std::min(g.E, g.R)) * tm)) return lin_launch_tile<T, MODE, 256, 128, 2, 2, F32>(g, st);
         if (MODE == LIN_DW && g.C > 128 && large_tiles(g.E * tm * ((g.C + 127) / 128))) return lin_launch_tile<T, MODE, 128, 256, 1, 4, F32>(g, st);
     }
     if (small) return lin_launch_tile<T, MODE, 64, 64, 1, 2, F32>(g, st);

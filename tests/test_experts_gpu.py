@@ -297,6 +297,68 @@ def test_linear_row_of_infinities_stays_in_its_row(cuda):
     assert torch.isnan(X.expert_linear(x2, w, plan, relu=True)[plan.positions[11, 0].long()]).all()
 
 
+@pytest.mark.parametrize("K,N", [(32, 64), (64, 16), (16, 64), (128, 64), (64, 128), (256, 256)])
+def test_linear_rows_behind_the_last_segment_are_zero_whatever_the_weights(K, N, cuda):
+    from nersemble_amd import experts as X
+    T, E = 700, 3
+    c = torch.full((T, 2), -1, dtype=torch.int32, device=cuda)
+    c[::3, 1] = 1
+    plan = X.expert_plan(c, E)
+    n = int(plan.offsets[-1])
+    x = torch.randn((T, K), device=cuda).half().requires_grad_(True)
+    w = torch.randn((E, N, K), device=cuda).half()
+    w[0], w[2] = float("inf"), float("nan")
+    w.requires_grad_(True)
+    y = X.expert_linear(x, w, plan)
+    assert (y[n:] == 0).all() and torch.isfinite(y).all() and (y[:n] != 0).any()
+    dx, dw = torch.autograd.grad(y, [x, w], torch.ones_like(y))
+    off = (c < 0).all(1)
+    assert torch.isfinite(dx).all() and (dx[off] == 0).all() and (dw[[0, 2]] == 0).all() and torch.isfinite(dw).all()
+    dh, = torch.autograd.grad(X.expert_linear(x.detach().repeat(2, 1).requires_grad_(True), w, plan, gather=False).sum(), [w])
+    assert (dh[[0, 2]] == 0).all()
+
+
+@pytest.mark.parametrize("T,k,E,K,N", [(16384, 2, 17, 1000, 2056), (9000, 3, 70, 776, 776)])
+@pytest.mark.parametrize("dtype,relu,master", [("bf16", False, False), ("fp16", True, False), ("fp16", False, True)])
+def test_linear_largest_tiles(T, k, E, K, N, dtype, relu, master, cuda):
+    """Products of thousands of tiles, one expert with a third of the rows, against 64-bit products of each segment."""
+    from nersemble_amd import experts as X
+    g = torch.Generator(device=cuda).manual_seed(T)
+    dt, (h, tiny) = DT[dtype], HALF[DT[dtype]]
+    logits = torch.randn((T, E), generator=g, device=cuda)
+    logits[:, 3] += 2
+    _, c = X.route_experts(logits, k)
+    c[::10] = -1
+    plan = X.expert_plan(c, E)
+    x = torch.randn((T, K), generator=g, device=cuda).to(dt).requires_grad_(True)
+    wf = torch.randn((E, N, K), generator=g, device=cuda) / K ** 0.5
+    w = (wf if master else wf.to(dt)).requires_grad_(True)
+    y = X.expert_linear(x, w, plan, relu=relu)
+    dy = torch.randn(y.shape, generator=g, device=cuda).to(dt)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    off = plan.offsets.tolist()
+    assert (y[off[-1]:] == 0).all()
+    wx, tx = torch.zeros((T, K), dtype=torch.float64, device=cuda), torch.zeros((T, K), dtype=torch.float64, device=cuda)
+
+    def inside(got, want, tol, what):
+        assert ((got.double() - want).abs() <= tol).all(), what
+    for e in range(E):
+        a, b = off[e], off[e + 1]
+        r = (plan.rows[a:b] // k).long()
+        xe, we = x.detach()[r].double(), wf[e].to(dt).double()
+        want, mag = xe @ we.t(), xe.abs() @ we.t().abs()
+        if relu:
+            want = want.clamp(min=0)
+        inside(y[a:b], want, h * want.abs() + tiny + (K + 2) * 2 * U * mag, "y")
+        dz = dy[a:b].double() * (y[a:b] > 0) if relu else dy[a:b].double()
+        want, mag = dz.t() @ xe, dz.t().abs() @ xe.abs()
+        inside(dw[e], want, (b - a + 2) * 2 * U * mag + (0 if master else h * want.abs() + tiny), "dw")
+        want, mag = dz @ we, dz.abs() @ we.abs()
+        wx.index_add_(0, r, want)
+        tx.index_add_(0, r, h * want.abs() + tiny + (N + 2 + k) * 2 * U * mag)
+    inside(dx, wx, (tx + h * wx.abs() + h * tx + tiny) * (1 + 4 * U * k), "dx")
+
+
 def test_linear_layouts(cuda):
     """Strided, transposed and misaligned rows, gradients and weights give what their contiguous copies give."""
     from nersemble_amd import experts as X
@@ -696,3 +758,80 @@ def test_route_choice_where_32_bits_do_not_tell(cuda):
                     dg = np.diff(by, axis=1)
                     clear &= ~((dg > 0) & (dg < 1e-13)).any(1)
                 assert clear.mean() > 0.5 and np.array_equal(got[clear], wc[clear]), (E, G, sc)
+
+
+def test_the_same_expert_twice_for_a_row(cuda):
+    """Choices made by hand: a row that names one expert several times is several entries of it, gradients add up."""
+    from nersemble_amd import experts as X
+    T, E, K, N = 70, 3, 24, 40
+    g = torch.Generator(device=cuda).manual_seed(3)
+    c = torch.randint(0, E, (T, 1), generator=g, device=cuda, dtype=torch.int32)
+    x = torch.randn((T, K), generator=g, device=cuda).half().requires_grad_(True)
+    w = torch.randn((E, N, K), generator=g, device=cuda).half().requires_grad_(True)
+    go = torch.randn((T, N), generator=g, device=cuda).half()
+    one, three = X.expert_plan(c, E), X.expert_plan(c.expand(T, 3), E)
+    wt = torch.tensor([0.5, 0.25, 0.25], device=cuda).expand(T, 3)
+    a = X.expert_combine(X.expert_linear(x, w, one), torch.ones((T, 1), device=cuda), one)
+    b = X.expert_combine(X.expert_linear(x, w, three), wt, three)
+    assert torch.equal(a, b)                                         # (weights that are powers of two: nothing rounds)
+    ga, gb = torch.autograd.grad(a, [x, w], go), torch.autograd.grad(b, [x, w], go)
+    # dw: the same terms (scaled exactly) in another order; dx: three scaled copies of one gradient, each rounded
+    h, tiny = HALF[torch.float16]
+    x64, w64, g64 = x.detach().double(), w.detach().double(), go.double()
+    for e in range(E):
+        m = c[:, 0] == e
+        mag = g64[m].t().abs() @ x64[m].abs()
+        tol = 2 * (h * ga[1][e].double().abs() * 2 + tiny) + 2 * (3 * int(m.sum()) + 66) * 2 * U * mag
+        assert ((ga[1][e].double() - gb[1][e].double()).abs() <= tol).all()
+        mag = g64[m].abs() @ w64[e].abs()
+        tol = 2 * (2 * h * ga[0][m].double().abs() + 4 * tiny) + 2 * (N + 6) * 2 * U * mag + h * h * mag
+        assert ((ga[0][m].double() - gb[0][m].double()).abs() <= tol).all()
+
+
+def test_products_against_differences(cuda):
+    """Gradients of the products and of the join against differences: both are linear in each input, so a step of 1 in one
+    value changes the loss by the gradient, up to the roundings of the outputs."""
+    from nersemble_amd import experts as X
+    g = torch.Generator(device=cuda).manual_seed(8)
+    T, k, E, K, N = 9, 2, 3, 8, 16
+    _, c = X.route_experts(torch.randn((T, E), generator=g, device=cuda), k)
+    plan = X.expert_plan(c, E)
+    # small whole numbers: every product, sum and difference is exact in fp16 and fp32
+    x = torch.randint(-3, 4, (T, K), generator=g, device=cuda).half()
+    w = torch.randint(-3, 4, (E, N, K), generator=g, device=cuda).half()
+    wt = torch.randint(-2, 3, (T, k), generator=g, device=cuda).float()
+    go = torch.randint(-1, 2, (T, N), generator=g, device=cuda).half()
+
+    def loss(x, w, wt):
+        return (X.expert_combine(X.expert_linear(x, w, plan), wt, plan).double() * go.double()).sum()
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, wt)]
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    base = loss(x, w, wt)
+    for n, v in enumerate((x, w, wt)):
+        for i in range(0, v.numel(), 5):
+            args = [u.clone() for u in (x, w, wt)]
+            args[n].view(-1)[i] += 1
+            assert float(loss(*args) - base) == float(grads[n].reshape(-1)[i]), (n, i)
+
+
+def test_two_runs_at_once_on_two_streams(cuda):
+    """Two steps enqueued on two streams without waiting for each other give what they give alone."""
+    a, ga = _mixture_inputs(3000, 8, 64, 128, 32, 11, cuda)
+    b, gb = _mixture_inputs(2500, 5, 32, 64, 16, 12, cuda)
+
+    def step(v, go, E):
+        out = _mixture(*v, E, 2)
+        return [out] + list(torch.autograd.grad(out, v, go))
+    want = step(a, ga, 8), step(b, gb, 5)
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (v, go, E) in enumerate(((a, ga, 8), (b, gb, 5))):
+            with torch.cuda.stream(s[i]):
+                got[i].append(step(v, go, E))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for p, q in zip(r, want[i]):
+                assert torch.equal(p, q)
