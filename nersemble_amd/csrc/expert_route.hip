@@ -14,7 +14,10 @@
 //     exp(x_j - min(max, 0)) / (1 + exp(x_j)) -- neither underflows where all chosen scores are tiny.
 // A row is held by L lanes of a wave, V consecutive experts in each (64 / L rows per wave): a row is read once, 16 or 32 bytes
 // per lane.  A round of "largest value, lowest index" is log2(L) exchanges of the value within the lanes (DPP), a ballot of the
-// lanes that hold it, and the first of them takes its expert out.
+// lanes that hold it, and the first of them takes its expert out.  The entries lie in LDS, a lane each computes their weights.
+// Bound by memory where few are chosen: 2^20 x 32 fp32, top 2: 32 us (151 MB, 4.7 TB/s; a copy reaches 4.96).  By the rounds'
+// instructions where many are: 65536 x 256 bf16, top 8: 25 us (38 MB, 1.5 TB/s); with a bias 62 us in fp32, and 30011 rows of 8
+// groups 34 us, of which 10 are one wave that does its rows again in 64 bits at the end.
 #include "expert_common.h"
 #include <algorithm>
 
@@ -79,48 +82,70 @@ __device__ __forceinline__ float sigmoid_over(float x, float m) {
     return x <= 0.f ? expf(x - m) / (1.f + expf(x)) : 1.f / (1.f + expf(-x));
 }
 
-// One pass of the choice over the wave's rows: values c (taken from it as they are chosen) -> entries of `out`, k + 1 of them
-// if `more` (the one that just missed).  out: per row top_k + 1 of {value, expert}.
+// What is compared: 64-bit values as they are, 32-bit ones as integers of the same order (-0 as 0), whose largest of three is one
+// instruction.  Nothing that is compared is NaN.
+template <typename K> struct Order;
+template <> struct Order<float> {
+    typedef int32_t type;
+    static __device__ __forceinline__ int32_t of(float v) { const int32_t b = __builtin_bit_cast(int32_t, v + 0.f); return b ^ ((b >> 31) & 0x7fffffff); }
+    static __device__ __forceinline__ float value(int32_t k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
+    static __device__ __forceinline__ int32_t none() { return 0x807fffff; }                 // of(-inf)
+};
+template <> struct Order<double> {
+    typedef double type;
+    static __device__ __forceinline__ double of(double v) { return v; }
+    static __device__ __forceinline__ double value(double k) { return k; }
+    static __device__ __forceinline__ double none() { return -INFINITY; }
+};
+
+// One pass of the choice over the wave's rows: `rounds` entries of `out` per row, c of the chosen becomes none.
 template <typename K> struct Chosen { K c; int32_t e; };
 template <typename K, int V>
-__device__ __forceinline__ void choose(const RouteArgs& a, K (&c)[V], int e0, int r, int sub, int rounds, Chosen<K>* __restrict__ out) {
+__device__ __forceinline__ void choose(const RouteArgs& a, typename Order<K>::type (&c)[V], int e0, int r, int sub, int rounds, Chosen<K>* __restrict__ out) {
+    typedef Order<K> O;
     const int L = 1 << a.lg_L;
     for (int j = 0; j < rounds; ++j) {
-        K best = c[0];
+        auto best = c[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) best = c[i] > best ? c[i] : best;
-        const K top = row_all<TakeMax>(best, L);
+        const auto top = row_all<TakeMax>(best, L);
         const uint64_t holders = row_lanes(__ballot(best == top), r, a.lg_L);
         if (__ffsll((unsigned long long)holders) - 1 == sub) {
-            int at = V - 1;
+            int at = 0;
+            bool found = false;
 #pragma unroll
-            for (int i = V - 2; i >= 0; --i) at = c[i] == top ? i : at;
-#pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = i == at ? (K)-INFINITY : c[i];
-            out[j] = Chosen<K>{top, top > (K)-INFINITY ? e0 + at : -1};
+            for (int i = 0; i < V; ++i) {
+                const bool here = !found && c[i] == top;
+                at = here ? i : at;
+                c[i] = here ? O::none() : c[i];
+                found |= here;
+            }
+            out[j] = Chosen<K>{O::value(top), top > O::none() ? e0 + at : -1};
         }
     }
     wave_lds_fence();
 }
 
-// groups that stay: the values of the others become -inf.  Returns the distance between the last group that stays and the first
+// groups that stay: the values of the others become none.  Returns the distance between the last group that stays and the first
 // that does not, and the former's value.
 template <typename K, int V>
-__device__ __forceinline__ K keep_groups(const RouteArgs& a, K (&c)[V], int r, int g, K& lowest) {
-    K b1 = (K)-INFINITY, b2 = (K)-INFINITY;
+__device__ __forceinline__ K keep_groups(const RouteArgs& a, typename Order<K>::type (&c)[V], int r, int g, K& lowest) {
+    typedef Order<K> O;
+    auto b1 = O::none(), b2 = O::none();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        b2 = c[i] > b1 ? b1 : (c[i] > b2 ? c[i] : b2);
+        const auto lo = c[i] < b1 ? c[i] : b1;
+        b2 = lo > b2 ? lo : b2;
         b1 = c[i] > b1 ? c[i] : b1;
     }
     for (int o = 1; o < 1 << a.lg_Lg; o <<= 1) {
-        const K p1 = __shfl_xor(b1, o), p2 = __shfl_xor(b2, o);
-        const K lo = p1 < b1 ? p1 : b1;
+        const auto p1 = __shfl_xor(b1, o), p2 = __shfl_xor(b2, o);
+        const auto lo = p1 < b1 ? p1 : b1;
         b1 = p1 > b1 ? p1 : b1;
         b2 = p2 > b2 ? p2 : b2;
         b2 = lo > b2 ? lo : b2;
     }
-    const K mine = a.group_top == 2 ? b1 + b2 : b1;
+    const K mine = a.group_top == 2 ? O::value(b1) + O::value(b2) : O::value(b1);
     int before = 0;
     for (int h = 0; h < a.G; ++h) {
         const K other = __shfl(mine, (r << a.lg_L) + (h << a.lg_Lg));
@@ -129,7 +154,7 @@ __device__ __forceinline__ K keep_groups(const RouteArgs& a, K (&c)[V], int r, i
     const bool stays = before < a.top_groups && g < a.G;
     if (!stays)
 #pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = (K)-INFINITY;
+        for (int i = 0; i < V; ++i) c[i] = O::none();
     lowest = -row_all<TakeMax>(stays ? -mine : (K)-INFINITY, 1 << a.lg_L);
     const K highest = row_all<TakeMax>(stays || g >= a.G ? (K)-INFINITY : mine, 1 << a.lg_L);
     return lowest - highest;
@@ -178,29 +203,37 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
         for (int i = 0; i < V; ++i) z += x[i] > -INFINITY ? expf(x[i] - xmax) : 0.f;
         Z = row_all<TakeSum>(z, L);
     }
-    float c[V];
+    int32_t c[V];
     bool again = false;
     if (!SCORES) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = bad ? -INFINITY : x[i];
+        for (int i = 0; i < V; ++i) c[i] = bad ? Order<float>::none() : Order<float>::of(x[i]);
         float lowest;
-        if (a.top_groups < a.G) keep_groups(a, c, r, g, lowest);
-        choose(a, c, e0, r, sub, a.k, out);
+        if (a.top_groups < a.G) keep_groups<float>(a, c, r, g, lowest);
+        choose<float>(a, c, e0, r, sub, a.k, out);
     } else {
         float bias[V];
 #pragma unroll
+        for (int i = 0; i < V; ++i) bias[i] = 0.f;
+        if (a.bias) {
+            if (VEC) { if (nv > 0) __builtin_memcpy(bias, a.bias + e0, V * sizeof(float)); }
+            else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) if (i < nv) bias[i] = a.bias[e0 + i];
+            }
+        }
+#pragma unroll
         for (int i = 0; i < V; ++i) {
-            bias[i] = (a.bias && i < nv) ? a.bias[e0 + i] : 0.f;
             const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-x[i])) : expf(x[i] - xmax) * (1.f / Z);
             const float v = s + bias[i];
-            c[i] = (!bad && x[i] > -INFINITY && v == v) ? v : -INFINITY;
+            c[i] = (!bad && x[i] > -INFINITY && v == v) ? Order<float>::of(v) : Order<float>::none();
         }
         if (a.top_groups < a.G) {
             float lowest;
-            const float gap = keep_groups(a, c, r, g, lowest);                      // (of sums of up to two)
+            const float gap = keep_groups<float>(a, c, r, g, lowest);                      // (of sums of up to two)
             again = !(gap > 2.f * unsure(lowest, a.sigmoid)) && !bad;
         }
-        choose(a, c, e0, r, sub, a.k + 1, out);
+        choose<float>(a, c, e0, r, sub, a.k + 1, out);
         for (int j = sub; j < a.k; j += L) {
             const Chosen<float> p = out[j], q = out[j + 1];
             // (equal logits and biases are equal in 64 bits as well -- unless a third that is not may come between the last
@@ -230,29 +263,36 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
                 d[i] = (!bad && x[i] > -INFINITY && v == v) ? v : -INFINITY;
             }
             double lowest;
-            if (a.top_groups < a.G) keep_groups(a, d, r, g, lowest);
-            choose(a, d, e0, r, sub, a.k, wide);
+            if (a.top_groups < a.G) keep_groups<double>(a, d, r, g, lowest);
+            choose<double>(a, d, e0, r, sub, a.k, wide);
             // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from)
             if (sub == 0)
                 for (int j = 0; j < a.k; ++j) { const Chosen<double> w = wide[j]; out[j] = Chosen<float>{(float)w.c, w.e}; }
             wave_lds_fence();
         }
     }
-    if (t >= T_) return;
-    float m = 0.f, S = 1.f;
-    if (a.renorm) {
-        m = -INFINITY; S = 0.f;
-        for (int j = 0; j < a.k; ++j) if (out[j].e >= 0) m = fmaxf(m, (float)row[out[j].e]);
-        if (a.sigmoid) m = fminf(m, 0.f);
-        for (int j = 0; j < a.k; ++j)
-            if (out[j].e >= 0) S += a.sigmoid ? sigmoid_over((float)row[out[j].e], m) : expf((float)row[out[j].e] - m);
-    } else if (!a.sigmoid) {
-        m = xmax; S = Z;
+    // the weights: an entry to a lane, which keeps its logit in c's place
+    float m = -INFINITY, S = 0.f;
+    for (int j = sub; j < a.k; j += L) {
+        const float v = out[j].e >= 0 ? (float)row[out[j].e] : -INFINITY;
+        out[j].c = v;
+        m = fmaxf(m, v);
     }
+    if (a.renorm) {
+        m = row_all<TakeMax>(m, L);
+        if (a.sigmoid) m = fminf(m, 0.f);
+        for (int j = sub; j < a.k; j += L)
+            if (out[j].e >= 0) S += a.sigmoid ? sigmoid_over(out[j].c, m) : expf(out[j].c - m);
+        S = row_all<TakeSum>(S, L);
+    } else {
+        m = a.sigmoid ? 0.f : xmax;
+        S = Z;
+    }
+    if (t >= T_) return;
     for (int j = sub; j < a.k; j += L) {
         int e = out[j].e;
         float w = 0.f;
-        if (e >= 0) w = a.scale * ((a.sigmoid ? sigmoid_over((float)row[e], m) : expf((float)row[e] - m)) / S);
+        if (e >= 0) w = a.scale * ((a.sigmoid ? sigmoid_over(out[j].c, m) : expf(out[j].c - m)) / S);
         if (!on) e = -1;
         else if (bad) { e = j; w = __builtin_nanf(""); }
         a.w[t * a.k + j] = w;
@@ -550,9 +590,12 @@ int nsx_expert_route_fwd(const void* logits, int dtype, int64_t T, int E, int64_
     const int Eg = E / n_groups, lg_G = lg2_ceil(n_groups);
     RouteArgs a{logits, row_stride, T, E, bias, selector, top_k, n_groups, top_groups, group_top, sigmoid, renormalise, scale,
                 weights, experts, n_device, 0, 0, fast_div(top_k)};
-    // Values per lane: 16 leave the fewest exchanges and instructions per row, 4 the shortest chain for few rows.  us with 4 | 8 | 16:
-    // 2^20 x 32 fp32 top 2  64 | 41 | 38;  2^20 x 8 fp16 top 2  17 | 13 | 13;  65536 x 256 bf16 top 8  74 | 47 | 35;  1 x 64  5.3 | 5.6 | 6.9
-    int V = T <= 1024 ? 4 : Eg >= 32 ? 16 : 8;
+    // Values per lane: 16 leave the fewest exchanges and instructions per row, 4 the shortest chain where few waves hide it.  us with
+    // 4 | 8 | 16 (groups: 8 with a bias, the best 2 of each counting, 4 of them stay):
+    //   2^20 x 32 fp32 top 2      62 | 38 | 32     16384 x 64 fp32 top 6           6.0 |  5.5 |  6.8    30011 x 256 bf16 top 8, groups  50 | 35 | 34
+    //   65536 x 256 bf16 top 8    58 | 35 | 25      4096 x 64 fp32 top 6           4.5 |  5.0 |  6.7     2^20 x 8 fp16 top 2            17 | 13 | 13
+    //   2^18 x 64 fp32 top 6      46 | 33 | 30      4096 x 256 bf16 top 8, groups 14.7 | 15.7 | 20.2     1 x 64 fp32 top 6             4.5 | 4.3 | 5.7
+    int V = T * E <= 1 << 19 ? 4 : T * E <= 1 << 22 || Eg < 32 ? 8 : 16;
     const int esize = dtype == NSX_DTYPE_F32 ? 4 : 2;
     while (V > 4 && Eg % V) V >>= 1;
     while (lg_G + lg2_ceil((Eg + V - 1) / V) > 6) V <<= 1;
