@@ -306,6 +306,9 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
 // softmax  dx_e = [e chosen] w_e g_e - s_e sum_i g_i w_i.  Only the last one reads whole rows of logits again.
 // A wave's rows lie in LDS as 32-bit values: cleared, the chosen places written by one lane per entry, read back and stored
 // whole -- the entries are read once and no lane compares its experts with them.
+// Bound by memory: 2^20 x 32 fp32, top 2 renormalised: 26 us for 159 MB (the caches take part of them; a copy: 32); the whole
+// softmax, which reads the logits as well, 68 for 293 (59).  fp32 rows leave 16 bytes per lane side by side (32 per lane: 29 us).
+// Stores past the caches (nontemporal) took 21 us, but what they gain the next reader of the gradient pays: together 81 | 82 us.
 template <typename T, int V, bool VEC>
 __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a, const float* __restrict__ dw, T* __restrict__ dx) {
     extern __shared__ __attribute__((aligned(16))) char route_lds[];
@@ -366,6 +369,16 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a, const float
         if (any)
 #pragma unroll
             for (int i = 0; i < V; ++i) o[i] -= s[i] / z * A;
+    }
+    if (sizeof(T) == 4 && VEC && a.E == L * V) {               // the wave's rows are one stretch of memory: 16 bytes per lane, side by side
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) own[i] = f32x4{o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]};
+            wave_lds_fence();
+        }
+        for (int i = lane * 4; i < rows * a.E; i += kWave * 4)
+            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(dx) + t0 * (int64_t)a.E + i) = *reinterpret_cast<const f32x4*>(d + i);
+        return;
     }
     if (nv == 0) return;
     T* p = dx + t * (int64_t)a.E + e0;
