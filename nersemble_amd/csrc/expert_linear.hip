@@ -38,6 +38,7 @@ struct LinArgs {
     int m_tiles, c_tiles, relu;
     int chunk;                       // dW: rows per partial sum (0: a whole segment, no partial sums)
     float* partial;                  // [chunk][C][M]
+    const void* x; int64_t ldx;      // narrow layers: both gradients at once
 };
 
 template <typename T> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
@@ -423,6 +424,52 @@ template <> __device__ __forceinline__ f32x4 mfma16<bf16_t>(u32x4 a, u32x4 b, f3
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Elem<bf16_t>::x8, a), __builtin_bit_cast(Elem<bf16_t>::x8, b), c, 0, 0, 0);
 }
 
+// An expert's matrix as fragments of P
+template <typename T, int MODE, int MT, int QS>
+__device__ __forceinline__ void narrow_matrix(const LinArgs& g, int e, u32x4 (&p)[MT][QS]) {
+    const int lane = threadIdx.x & 63, c = lane & 15, piece = lane >> 4;
+    const T* P = reinterpret_cast<const T*>(g.p) + e * g.p_expert;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = min((c >> 2) * (4 * MT) + t * 4 + (c & 3), g.M - 1);
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const int at = s * 32 + piece * 8;
+            if (MODE == LIN_FWD) p[t][s] = load16(at < g.K ? reinterpret_cast<const char*>(P + (int64_t)m * g.ldp + at) : zero_row());
+            else {
+                const uint16_t* w = reinterpret_cast<const uint16_t*>(P) + (int64_t)min(at, g.K - 8) * g.ldp + m;
+                // (q behind the end: whatever is here meets zeros of the other operand -- unless it is not finite: cleared)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const uint32_t v = (uint32_t)w[(2 * h) * g.ldp] | (uint32_t)w[(2 * h + 1) * g.ldp] << 16;
+                    p[t][s][h] = at < g.K ? v : 0u;
+                }
+            }
+        }
+    }
+}
+// 4 MT consecutive values of row `at`, from m on
+template <typename T, int MT>
+__device__ __forceinline__ void narrow_store(const LinArgs& g, int at, const f32x4 (&acc)[MT], bool relu) {
+    const int m = ((threadIdx.x & 63) >> 4) * (4 * MT);
+    alignas(16) T out[4 * MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float v = acc[t][r];
+            if (relu) v = v <= 0.f ? 0.f : v;                  // (NaN stays)
+            out[t * 4 + r] = (T)v;
+        }
+    T* d = reinterpret_cast<T*>(g.d) + (int64_t)at * g.ldd + m;
+    if (MT == 1) {
+        if (m < g.M) *reinterpret_cast<u32x2*>(d) = *reinterpret_cast<const u32x2*>(out);
+    } else
+#pragma unroll
+        for (int h = 0; h < MT / 2; ++h)
+            if (m + h * 8 < g.M) *reinterpret_cast<u32x4*>(d + h * 8) = *reinterpret_cast<const u32x4*>(out + h * 8);
+}
+
 template <typename T, int MODE, int MT, int QS, bool MASK>
 __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, piece = lane >> 4;
@@ -449,27 +496,8 @@ __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
             if (MASK) y[u][s] = load16(in ? Y + ((int64_t)r * g.ldmask + at) * 2 : zero_row());
         }
     }
-    // the expert's matrix
     u32x4 p[MT][QS];
-    const T* P = reinterpret_cast<const T*>(g.p) + (nothing ? 0 : e * g.p_expert);
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = min((c >> 2) * (4 * MT) + t * 4 + (c & 3), g.M - 1);
-#pragma unroll
-        for (int s = 0; s < QS; ++s) {
-            const int at = s * 32 + piece * 8;
-            if (MODE == LIN_FWD) p[t][s] = load16(at < g.K ? reinterpret_cast<const char*>(P + (int64_t)m * g.ldp + at) : zero_row());
-            else {
-                const uint16_t* w = reinterpret_cast<const uint16_t*>(P) + (int64_t)min(at, g.K - 8) * g.ldp + m;
-                // (q behind the end: whatever is here meets zeros of the other operand -- unless it is not finite: cleared)
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const uint32_t v = (uint32_t)w[(2 * h) * g.ldp] | (uint32_t)w[(2 * h + 1) * g.ldp] << 16;
-                    p[t][s][h] = at < g.K ? v : 0u;
-                }
-            }
-        }
-    }
+    narrow_matrix<T, MODE, MT, QS>(g, nothing ? 0 : e, p);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         if (a + u * 16 >= b) break;
@@ -487,25 +515,158 @@ __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
         if (nothing)                                      // (the first expert's matrix may hold what is not finite)
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int at = a + u * 16 + c, m = piece * (4 * MT);
-        if (at >= b) continue;
-        alignas(16) T out[4 * MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float v = acc[t][r];
-                if (MODE == LIN_FWD && g.relu) v = v <= 0.f ? 0.f : v;                  // (NaN stays)
-                out[t * 4 + r] = (T)v;
-            }
-        T* d = reinterpret_cast<T*>(g.d) + (int64_t)at * g.ldd + m;
-        if (MT == 1) {
-            if (m < g.M) *reinterpret_cast<u32x2*>(d) = *reinterpret_cast<const u32x2*>(out);
-        } else
-#pragma unroll
-            for (int h = 0; h < MT / 2; ++h)
-                if (m + h * 8 < g.M) *reinterpret_cast<u32x4*>(d + h * 8) = *reinterpret_cast<const u32x4*>(out + h * 8);
+        if (a + u * 16 + c < b) narrow_store<T, MT>(g, a + u * 16 + c, acc, MODE == LIN_FWD && g.relu);
     }
+}
+
+// Both gradients of a narrow layer in one pass over dy, y and x.  A wave takes 64 rows at a time: dz as fragments straight from
+// memory, as in the kernel above, makes dx; for dW the rows are the sum's index, so dz and x go through LDS (a region of the wave's
+// own) turned: a lane holds the same 8 features of the rows c, 16 + c, 32 + c and 48 + c, which it stores side by side -- the
+// order of a sum over rows is free as long as both operands have it.  dW's 32-bit sums stay in registers for a whole chunk of a
+// segment, the four waves' are added in their order at its end; expert_sum_chunks_kernel adds the chunks.
+// Feature f's row of 128 bytes lies at f with the lowest bit turned by bit 3, its 16-byte pieces permuted by f / 2: neither the
+// stores (features 8 apart) nor the fragment reads (16 features) meet on a bank.
+__device__ __forceinline__ uint32_t turned_at(int f, int piece) { return (f ^ (f >> 3 & 1)) * 128 + ((piece ^ (f >> 1)) & 7) * 16; }
+template <int S>
+__device__ __forceinline__ void put_turned(char* lds, const u32x4 (&v)[4][S], int features) {
+    const int lane = threadIdx.x & 63, c = lane & 15, piece = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        if (s * 32 + piece * 8 >= features) continue;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t sel = h ? 0x07060302u : 0x05040100u;
+                const u32x2 o = {__builtin_amdgcn_perm(v[1][s][w], v[0][s][w], sel), __builtin_amdgcn_perm(v[3][s][w], v[2][s][w], sel)};
+                *reinterpret_cast<u32x2*>(lds + turned_at(s * 32 + piece * 8 + w * 2 + h, c >> 1) + (c & 1) * 8) = o;
+            }
+    }
+}
+
+template <typename T, int MT, int QS, bool MASK>
+__global__ __launch_bounds__(4 * kWave, 3) void expert_narrow_bwd_kernel(LinArgs g) {
+    constexpr int XS = (MT + 1) / 2, CT = 2 * QS, MINE = (16 * MT + 32 * QS) * 128;
+    static_assert(MT * CT * 1024 <= MINE, "the sums fit where the rows were");
+    __shared__ __attribute__((aligned(16))) char turned[4][MINE];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, piece = lane >> 4;
+    int e, a, b;
+    if (!find_tile(g.offsets, g.E, g.R, g.chunk, blockIdx.x, e, a, b)) return;
+    if (e == g.E) {                                            // rows behind the last segment
+        const int m8 = g.M / 8;
+        for (int i = threadIdx.x; i < (b - a) * m8; i += 4 * kWave)
+            *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(g.d) + (int64_t)(a + i / m8) * g.ldd + i % m8 * 8) = u32x4{0, 0, 0, 0};
+        return;
+    }
+    char* zt = turned[wave];
+    char* xt = zt + 32 * QS * 128;
+    u32x4 p[MT][QS];
+    narrow_matrix<T, LIN_DX, MT, QS>(g, e, p);
+    f32x4 sum[MT][CT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int v = 0; v < CT; ++v) sum[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const char* Q = reinterpret_cast<const char*>(g.q);
+    const char* Y = reinterpret_cast<const char*>(g.mask);
+    const char* X = reinterpret_cast<const char*>(g.x);
+    for (int r0 = a + wave * 64; r0 < b; r0 += 4 * 64) {
+        int row = min(r0 + lane, b - 1);                       // of x, one to a lane
+        if (g.rows) { row = g.rows[row]; row = row >= 0 ? g.top_k(row) : -1; }
+        if (r0 + lane >= b || row >= g.x_rows) row = -1;
+        u32x4 q[4][QS], y[MASK ? 4 : 1][MASK ? QS : 1], x[4][XS];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = r0 + u * 16 + c;
+#pragma unroll
+            for (int s = 0; s < QS; ++s) {
+                const int at = s * 32 + piece * 8;
+                const bool in = r < b && at < g.K;
+                q[u][s] = load16(in ? Q + ((int64_t)r * g.ldq + at) * 2 : zero_row());
+                if (MASK) y[u][s] = load16(in ? Y + ((int64_t)r * g.ldmask + at) * 2 : zero_row());
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = __shfl(row, u * 16 + c);
+#pragma unroll
+            for (int s = 0; s < XS; ++s) {
+                const int at = s * 32 + piece * 8;
+                x[u][s] = load16(r >= 0 && at < g.M ? X + ((int64_t)r * g.ldx + at) * 2 : zero_row());
+            }
+        }
+        if (MASK)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int s = 0; s < QS; ++s)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) q[u][s][w] = keep_where(q[u][s][w], y[u][s][w]);
+        put_turned<QS>(zt, q, 32 * QS);
+        put_turned<XS>(xt, x, 16 * MT);
+        wave_lds_fence();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            f32x4 acc[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < QS; ++s)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[t] = mfma16<T>(p[t][s], q[u][s], acc[t]);
+            if (r0 + u * 16 + c < b) narrow_store<T, MT>(g, r0 + u * 16 + c, acc, false);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 fx[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) fx[t] = *reinterpret_cast<const u32x4*>(xt + turned_at(t * 16 + c, s * 4 + piece));
+#pragma unroll
+            for (int v = 0; v < CT; ++v) {
+                const u32x4 fz = *reinterpret_cast<const u32x4*>(zt + turned_at(v * 16 + c, s * 4 + piece));
+#pragma unroll
+                for (int t = 0; t < MT; ++t) sum[t][v] = mfma16<T>(fx[t], fz, sum[t][v]);
+            }
+        }
+        wave_lds_fence();
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int v = 0; v < CT; ++v) *reinterpret_cast<f32x4*>(zt + (t * CT + v) * 1024 + lane * 16) = sum[t][v];
+    __syncthreads();
+    if ((int)blockIdx.x >= g.R / g.chunk + g.E) return;        // (never, of a plan's offsets)
+    for (int i = wave; i < MT * CT; i += 4) {
+        f32x4 s = *reinterpret_cast<const f32x4*>(turned[0] + i * 1024 + lane * 16);
+#pragma unroll
+        for (int w = 1; w < 4; ++w) s += *reinterpret_cast<const f32x4*>(turned[w] + i * 1024 + lane * 16);
+        const int m = i / CT * 16 + piece * 4, o = i % CT * 16 + c;
+        if (m < g.M && o < g.K) *reinterpret_cast<f32x4*>(g.partial + ((int64_t)blockIdx.x * g.K + o) * g.M + m) = s;
+    }
+}
+
+template <typename T, int MT, int QS>
+static void narrow_bwd_tile(const LinArgs& g, hipStream_t st) {
+    const unsigned blocks = (unsigned)(g.R / g.chunk + g.E + 1);
+    if (g.mask) expert_narrow_bwd_kernel<T, MT, QS, true><<<blocks, 4 * kWave, 0, st>>>(g);
+    else expert_narrow_bwd_kernel<T, MT, QS, false><<<blocks, 4 * kWave, 0, st>>>(g);
+}
+template <typename T, int MT>
+static void narrow_bwd_m(const LinArgs& g, hipStream_t st) {
+    if (g.K <= 32) narrow_bwd_tile<T, MT, 1>(g, st);
+    else narrow_bwd_tile<T, MT, 2>(g, st);
+}
+template <typename T>
+static void narrow_bwd(const LinArgs& g, hipStream_t st) {
+    if (g.M <= 16) narrow_bwd_m<T, 1>(g, st);
+    else if (g.M <= 32) narrow_bwd_m<T, 2>(g, st);
+    else narrow_bwd_m<T, 4>(g, st);
+}
+// rows per chunk where both gradients of a layer are made at once (0: they are not): a round of three workgroups per CU
+static int narrow_bwd_chunk(int64_t R, int n_in, int n_out) {
+    if (n_in > 64 || n_out > 64 || R < 8 * NARROW_ROWS) return 0;
+    const int64_t chunk = (R / (3 * (int64_t)num_cus()) + NARROW_ROWS) / NARROW_ROWS * NARROW_ROWS;
+    return (int)std::min<int64_t>(chunk, 1 << 20);
 }
 
 template <typename T, int MODE, int MT, int QS>
@@ -639,8 +800,9 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
 
 // workspace: dx in the plan's order (16-byte steps), then dW's partial sums
 static int64_t bwd_dx_bytes(int64_t R, int n_in, bool gather) { return gather ? R * n_in * 2 : 0; }
-static int64_t bwd_dw_bytes(int64_t R, int E, int n_in, int n_out) {
-    const int chunk = nsx::dw_plan(R, E, n_in, n_out).chunk;
+static int64_t bwd_dw_bytes(int64_t R, int E, int n_in, int n_out, bool with_dx) {
+    int chunk = with_dx ? nsx::narrow_bwd_chunk(R, n_in, n_out) : 0;
+    if (chunk == 0) chunk = nsx::dw_plan(R, E, n_in, n_out).chunk;
     return chunk > 0 ? (R / chunk + E) * n_in * n_out * 4 : 0;
 }
 
@@ -649,7 +811,7 @@ int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, i
     int32_t some = 0;
     const int rc = lin_check("nsx_expert_linear_bwd_workspace", NSX_DTYPE_F16, n_in, n_out, E, R, 1, &some);
     if (rc != NSX_OK) return rc;
-    return (want_dx ? bwd_dx_bytes(R, n_in, gather) : 0) + (want_dw ? bwd_dw_bytes(R, E, n_in, n_out) : 0);
+    return (want_dx ? bwd_dx_bytes(R, n_in, gather) : 0) + (want_dw ? bwd_dw_bytes(R, E, n_in, n_out, want_dx) : 0);
 }
 
 int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, const int32_t* positions,
@@ -668,17 +830,27 @@ int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_
     NSX_REQUIRE(!dw || (aligned16(dw) && (x || x_rows == 0) && aligned16(x) && lin_stride(x_stride, n_in)),
                 "nsx_expert_linear_bwd: dw needs aligned pointers and x (row stride %lld)", (long long)x_stride);
     const int64_t dx_bytes = dx ? bwd_dx_bytes(R, n_in, rows) : 0;
-    NSX_REQUIRE(dx_bytes + (dw ? bwd_dw_bytes(R, E, n_in, n_out) : 0) == 0 || (workspace && aligned16(workspace)),
+    NSX_REQUIRE(dx_bytes + (dw ? bwd_dw_bytes(R, E, n_in, n_out, dx != nullptr) : 0) == 0 || (workspace && aligned16(workspace)),
                 "nsx_expert_linear_bwd: no workspace");
     hipStream_t st = (hipStream_t)stream;
     LinArgs g{};
     g.q = dy; g.mask = y; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in; g.offsets = offsets; g.top_k = fast_div(top_k);
     g.E = E; g.R = (int)R; g.M = n_in;
+    g.rows = rows; g.x_rows = (int)x_rows; g.C = n_out;
+    g.partial = reinterpret_cast<float*>((char*)workspace + dx_bytes);
+    const int at_once = dx && dw ? narrow_bwd_chunk(R, n_in, n_out) : 0;
     if (dx && R > 0) {
         LinArgs h = g;
-        h.p = weight; h.ldp = n_in; h.p_expert = (int64_t)n_in * n_out; h.d = rows ? workspace : dx; h.x_rows = (int)R; h.K = n_out;
-        rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(h, small_tiles(h), st) : lin_launch<bf16_t, LIN_DX, false>(h, small_tiles(h), st);
-        if (rc != NSX_OK) return rc;
+        h.p = weight; h.ldp = n_in; h.p_expert = (int64_t)n_in * n_out; h.d = rows ? workspace : dx; h.K = n_out;
+        if (at_once) {
+            h.x = x; h.ldx = x_stride; h.chunk = at_once;
+            if (dtype == NSX_DTYPE_F16) narrow_bwd<half_t>(h, st);
+            else narrow_bwd<bf16_t>(h, st);
+        } else {
+            h.rows = nullptr; h.x_rows = (int)R;
+            rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(h, small_tiles(h), st) : lin_launch<bf16_t, LIN_DX, false>(h, small_tiles(h), st);
+            if (rc != NSX_OK) return rc;
+        }
         NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
         // A row's choices are summed in 32 bits; their gradients lie in 16 bits between the two launches (in 32 they would be twice
         // the traffic): off by at most half a step of each term beside the sum's own rounding.
@@ -689,14 +861,16 @@ int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_
     }
     if (dw) {
         const DwPlan how = dw_plan(R, E, n_in, n_out);
-        g.chunk = how.chunk;
-        g.p = x; g.ldp = x_stride; g.d = dw; g.d_expert = (int64_t)n_in * n_out; g.rows = rows; g.x_rows = (int)x_rows; g.C = n_out;
-        g.partial = reinterpret_cast<float*>((char*)workspace + dx_bytes);
-        const bool f32 = dw_f32 || g.chunk > 0;
-        if (dtype == NSX_DTYPE_F16) rc = f32 ? lin_launch<half_t, LIN_DW, true>(g, how.small, st) : lin_launch<half_t, LIN_DW, false>(g, how.small, st);
-        else rc = f32 ? lin_launch<bf16_t, LIN_DW, true>(g, how.small, st) : lin_launch<bf16_t, LIN_DW, false>(g, how.small, st);
-        if (rc != NSX_OK) return rc;
-        NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
+        g.chunk = at_once ? at_once : how.chunk;
+        g.d = dw; g.d_expert = (int64_t)n_in * n_out;
+        if (!at_once) {
+            const bool f32 = dw_f32 || g.chunk > 0;
+            g.p = x; g.ldp = x_stride;
+            if (dtype == NSX_DTYPE_F16) rc = f32 ? lin_launch<half_t, LIN_DW, true>(g, how.small, st) : lin_launch<half_t, LIN_DW, false>(g, how.small, st);
+            else rc = f32 ? lin_launch<bf16_t, LIN_DW, true>(g, how.small, st) : lin_launch<bf16_t, LIN_DW, false>(g, how.small, st);
+            if (rc != NSX_OK) return rc;
+            NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
+        }
         if (g.chunk > 0) {
             const int64_t step = R / g.chunk > 8 * (int64_t)E ? 64 : 1024;
             const dim3 grid((unsigned)std::min<int64_t>(((int64_t)n_in * n_out + step - 1) / step, 4096), E);

@@ -272,6 +272,14 @@ def test_linear_larger(K, N, T, k, E, cuda):
     _linear_case(cuda, T, k, E, K, N, "fp16", False, True, False, 0.0)
 
 
+@pytest.mark.parametrize("K,N", [(8, 8), (8, 64), (16, 32), (32, 64), (64, 16), (64, 32), (40, 24), (24, 48), (64, 64)])
+@pytest.mark.parametrize("gather,relu,master", [(True, True, False), (True, False, True), (False, True, True), (False, False, False)])
+def test_linear_narrow_layers(K, N, gather, relu, master, cuda):
+    """Rows enough that both gradients of a narrow layer are made at once; segments of other lengths than its steps."""
+    _linear_case(cuda, 2501, 2, 7, K, N, "fp16", gather, relu, master, 0.2, seed=3)
+    _linear_case(cuda, 9001, 3, 3, K, N, "bf16", gather, relu, master, 0.0, 3, seed=4)
+
+
 def test_linear_row_of_infinities_stays_in_its_row(cuda):
     """What is not finite in one row (or in one expert's weights) reaches that row (those rows) alone."""
     from nersemble_amd import experts as X
