@@ -396,8 +396,12 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a, const float
 // ---- plan: a stable counting sort of the entries by expert ------------------------------------------------------------
 // Entry i = row * top_k + choice.  An entry whose expert is not in [0, E), or whose row lies behind the device-side count, is
 // in no segment: its position is -1.  Blocks own consecutive stretches of entries, the waves of a block consecutive parts of
-// them; what a wave counts in order lands in order, so equal inputs give equal plans.
-constexpr int PLAN_WAVES = 16, PLAN_THREADS = PLAN_WAVES * kWave, PLAN_MAX_BLOCKS = 256;
+// them; what a wave counts in order lands in order, so equal inputs give equal plans.  A first launch counts every block's entries
+// per expert; in the second a block knows from all counts where its own begin, and places them 64 at a time: lanes of one expert
+// find each other by ballots of the expert's bits.
+// Bound by the chain of steps: 2^20 rows x 2 of 16 experts, 25 MB: 18 us, 1.4 TB/s (a copy would take 5); 4096 x 2: 8 us, of which
+// one launch is 3.  8 entries per lane are loaded ahead; one at a time took 111 us.
+constexpr int PLAN_MAX_BLOCKS = 256;
 constexpr int PLAN_LANE = 8, PLAN_PIECE = PLAN_LANE * kWave;      // entries that a lane, a wave loads at a time
 
 __device__ __forceinline__ void plan_load(const int32_t* __restrict__ experts, int i0, int end, int E, int (&e)[PLAN_LANE]) {
@@ -416,13 +420,15 @@ __device__ __forceinline__ int plan_end(int n, int k, const int64_t* __restrict_
 }
 
 // entries per expert of each block
-__global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(const int32_t* __restrict__ experts, int n, int k, int E, int per_block,
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void plan_count_kernel(const int32_t* __restrict__ experts, int n, int k, int E, int per_block,
                                                                   int32_t* __restrict__ counts, const int64_t* __restrict__ n_dev) {
+    constexpr int PLAN_THREADS = WAVES * kWave;
     __shared__ int32_t hist[NSX_MAX_EXPERTS];
     for (int e = threadIdx.x; e < E; e += PLAN_THREADS) hist[e] = 0;
     __syncthreads();
     const int wave = threadIdx.x >> 6, a = blockIdx.x * per_block, b = min(a + per_block, plan_end(n, k, n_dev));
-    for (int i = a + wave * PLAN_PIECE; i < b; i += PLAN_WAVES * PLAN_PIECE) {
+    for (int i = a + wave * PLAN_PIECE; i < b; i += WAVES * PLAN_PIECE) {
         int e[PLAN_LANE];
         plan_load(experts, i, b, E, e);
 #pragma unroll
@@ -432,21 +438,23 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(const int32_t*
     for (int e = threadIdx.x; e < E; e += PLAN_THREADS) counts[(int64_t)blockIdx.x * E + e] = hist[e];
 }
 
-// bits: of an expert's number; lg_E: threads per column sum of the blocks' counts, as a power of two >= E
-__global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(const int32_t* __restrict__ experts, int n, int k, int E, int bits, int per_block,
+// bits: of an expert's number; 1 << bits <= the threads: the blocks' counts are summed column by column, several threads to a column
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void plan_place_kernel(const int32_t* __restrict__ experts, int n, int k, int E, int bits, int per_block,
                                                                   const int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
                                                                   int32_t* __restrict__ rows, int32_t* __restrict__ positions,
                                                                   const int64_t* __restrict__ n_dev) {
-    __shared__ int32_t cursor[PLAN_WAVES][NSX_MAX_EXPERTS];     // next free place of the wave's part, per expert
+    constexpr int PLAN_THREADS = WAVES * kWave, MAX_E = WAVES == 16 ? NSX_MAX_EXPERTS : WAVES == 8 ? 256 : 32;
+    __shared__ int32_t cursor[WAVES][MAX_E];                    // next free place of the wave's part, per expert
     __shared__ int32_t part_all[PLAN_THREADS], part_before[PLAN_THREADS];
-    __shared__ int32_t all[NSX_MAX_EXPERTS], first[NSX_MAX_EXPERTS];
+    __shared__ int32_t all[MAX_E], first[MAX_E];
     __shared__ int32_t routed;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blocks = gridDim.x;
     const int end = plan_end(n, k, n_dev);
-    for (int w = 0; w < PLAN_WAVES; ++w)
+    for (int w = 0; w < WAVES; ++w)
         for (int e = threadIdx.x; e < E; e += PLAN_THREADS) cursor[w][e] = 0;
     __syncthreads();
-    const int a0 = blockIdx.x * per_block, b0 = min(a0 + per_block, n), part = per_block / PLAN_WAVES;
+    const int a0 = blockIdx.x * per_block, b0 = min(a0 + per_block, n), part = per_block / WAVES;
     const int a = min(a0 + wave * part, b0), b = min(a + part, b0), live = min(b, end);
     int e[PLAN_LANE];
     for (int i = a; i < live; i += PLAN_PIECE) {
@@ -475,7 +483,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(const int32_t*
         if (blocks > 1) {
             for (int h = x; h < PLAN_THREADS; h += 1 << bits) { sum += part_all[h]; before += part_before[h]; }
         } else {
-            for (int w = 0; w < PLAN_WAVES; ++w) sum += cursor[w][x];
+            for (int w = 0; w < WAVES; ++w) sum += cursor[w][x];
         }
         all[x] = sum;
         first[x] = before;
@@ -506,7 +514,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(const int32_t*
     __syncthreads();
     for (int x = threadIdx.x; x < E; x += PLAN_THREADS) {
         int p = first[x];
-        for (int w = 0; w < PLAN_WAVES; ++w) { const int v = cursor[w][x]; cursor[w][x] = p; p += v; }
+        for (int w = 0; w < WAVES; ++w) { const int v = cursor[w][x]; cursor[w][x] = p; p += v; }
     }
     __syncthreads();
     const bool kept = b - a <= PLAN_PIECE;                        // (the entries are still in registers)
@@ -538,9 +546,23 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(const int32_t*
 // ---- host ---------------------------------------------------------------------------------------------------------
 static int lg2_ceil(int v) { int l = 0; while ((1 << l) < v) ++l; return l; }
 
-static int plan_blocks(int64_t n) {
-    const int64_t b = (n + PLAN_WAVES * PLAN_PIECE - 1) / (PLAN_WAVES * PLAN_PIECE);
+// Waves per block: one launch of 16 does up to 8192 entries; of more, short blocks spread the work over the CUs while every block
+// reads every other's counts.  us with 4 | 8 | 16:  524288 entries of 16 experts  10.9 | 12.5 | 14.9;  of 64  13.1 | 11.7 | 13.9;
+// of 256  23.9 | 14.8 | 15.0;  131072 of 256  13.2 | 11.8 | 14.1;  2^20 of 64  19.1 | 13.8 | 15.2;  2^21 of 16  24.0 | 18.5 | 18.4
+static int plan_waves(int64_t n, int E) {
+    if (n <= 16 * PLAN_PIECE || E > 256 || n > PLAN_MAX_BLOCKS * 8 * PLAN_PIECE) return 16;
+    return E <= 32 && n <= PLAN_MAX_BLOCKS * 4 * PLAN_PIECE ? 4 : 8;
+}
+static int plan_blocks(int64_t n, int E) {
+    const int64_t piece = (int64_t)plan_waves(n, E) * PLAN_PIECE, b = (n + piece - 1) / piece;
     return (int)(b < 1 ? 1 : b > PLAN_MAX_BLOCKS ? PLAN_MAX_BLOCKS : b);
+}
+
+template <int WAVES>
+static void launch_plan(int blocks, const int32_t* experts, int n, int k, int E, int per, int32_t* counts, int32_t* offsets, int32_t* rows,
+                        int32_t* positions, const int64_t* n_dev, hipStream_t st) {
+    if (blocks > 1) plan_count_kernel<WAVES><<<blocks, WAVES * kWave, 0, st>>>(experts, n, k, E, per, counts, n_dev);
+    plan_place_kernel<WAVES><<<blocks, WAVES * kWave, 0, st>>>(experts, n, k, E, lg2_ceil(E), per, counts, offsets, rows, positions, n_dev);
 }
 
 template <typename T, int V>
@@ -668,7 +690,7 @@ int64_t nsx_expert_plan_workspace(int64_t n_entries, int E) {
     using namespace nsx;
     NSX_REQUIRE(n_entries >= 0 && n_entries <= NSX_MAX_EXPERT_ENTRIES, "nsx_expert_plan_workspace: %lld entries", (long long)n_entries);
     NSX_REQUIRE(E >= 1 && E <= NSX_MAX_EXPERTS, "nsx_expert_plan_workspace: n_experts %d not in [1,%d]", E, NSX_MAX_EXPERTS);
-    return (int64_t)plan_blocks(n_entries) * E * 4;
+    return (int64_t)plan_blocks(n_entries, E) * E * 4;
 }
 
 int nsx_expert_plan(const int32_t* experts, int64_t T, int top_k, int E, int32_t* offsets, int32_t* rows, int32_t* positions,
@@ -678,17 +700,14 @@ int nsx_expert_plan(const int32_t* experts, int64_t T, int top_k, int E, int32_t
     NSX_REQUIRE(top_k >= 1 && top_k <= NSX_MAX_TOP_K, "nsx_expert_plan: top_k %d not in [1,%d]", top_k, NSX_MAX_TOP_K);
     NSX_REQUIRE(T >= 0 && T <= NSX_MAX_EXPERT_ENTRIES / top_k, "nsx_expert_plan: %lld rows of %d choices are too many", (long long)T, top_k);
     NSX_REQUIRE(offsets && workspace, "nsx_expert_plan: NULL pointer");
-    const int n = (int)(T * top_k), blocks = plan_blocks(n);
+    const int n = (int)(T * top_k), waves = plan_waves(n, E), blocks = plan_blocks(n, E);
     NSX_REQUIRE(n == 0 || (experts && rows && positions), "nsx_expert_plan: NULL pointer");
-    int64_t per = ((int64_t)n + blocks - 1) / blocks;
-    per = (per + PLAN_WAVES * PLAN_PIECE - 1) / (PLAN_WAVES * PLAN_PIECE) * (PLAN_WAVES * PLAN_PIECE);
+    const int64_t piece = (int64_t)waves * PLAN_PIECE, per = (((int64_t)n + blocks - 1) / blocks + piece - 1) / piece * piece;
     hipStream_t st = (hipStream_t)stream;
-    if (blocks > 1) {
-        plan_count_kernel<<<blocks, PLAN_THREADS, 0, st>>>(experts, n, top_k, E, (int)per, (int32_t*)workspace, n_device);
-        NSX_LAUNCH_CHECK("nsx_expert_plan");
-    }
-    plan_place_kernel<<<blocks, PLAN_THREADS, 0, st>>>(experts, n, top_k, E, lg2_ceil(E), (int)per, (const int32_t*)workspace, offsets,
-                                                       rows, positions, n_device);
+    int32_t* counts = (int32_t*)workspace;
+    if (waves == 16) launch_plan<16>(blocks, experts, n, top_k, E, (int)per, counts, offsets, rows, positions, n_device, st);
+    else if (waves == 8) launch_plan<8>(blocks, experts, n, top_k, E, (int)per, counts, offsets, rows, positions, n_device, st);
+    else launch_plan<4>(blocks, experts, n, top_k, E, (int)per, counts, offsets, rows, positions, n_device, st);
     NSX_LAUNCH_CHECK("nsx_expert_plan");
     return NSX_OK;
 }

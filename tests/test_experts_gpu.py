@@ -180,7 +180,7 @@ def _check_plan(plan, want):
 
 
 @pytest.mark.parametrize("T,k,E", [(0, 2, 4), (1, 1, 1), (1, 8, 64), (63, 1, 3), (257, 3, 512), (1000, 2, 16), (4096, 2, 16),
-                                   (3001, 7, 61), (20000, 8, 256), (300001, 2, 33)])
+                                   (3001, 7, 61), (20000, 8, 256), (300001, 2, 33), (150001, 3, 30), (100000, 8, 200), (1200000, 2, 7)])
 def test_plan(T, k, E, cuda):
     from nersemble_amd import experts as X
     rng = np.random.default_rng(T + E)
