@@ -1,6 +1,11 @@
 // expert_combine.hip -- routed experts: the weighted join of a row's expert outputs, and its gradients.
 //
-// out_t = sum_j w_tj y_pos(t,j);  dy_pos(t,j) = w_tj dout_t;  dw_tj = <dout_t, y_pos(t,j)>.  Sums in 32 bits.
+// out_t = sum_j w_tj y_pos(t,j);  dy_pos(t,j) = w_tj dout_t;  dw_tj = <dout_t, y_pos(t,j)>.  Sums in 32 bits; each result is rounded
+// to 16 bits once (dy: one product, rounded).
+// Bound by memory: y is read once, by rows of the plan's order, out or dy written once.  us and bytes / time:
+//   262144 rows x 2 choices, 64 columns fp16     forward 19.6 (105 MB, 5.4 TB/s)   backward 35.7 (174 MB, 4.9 TB/s)
+//   8192 x 8, 1024 columns bf16                  forward 30.4 (151 MB, 5.0 TB/s)   backward 65 (286 MB, 4.4 TB/s; a copy 4.96)
+// Stores past the caches (nontemporal) took 17, 32, 28.6 and 60 us, but the next reader of the result pays what they gain.
 #include "expert_common.h"
 
 namespace nsx {
@@ -19,7 +24,8 @@ __device__ __forceinline__ int64_t valid_rows(int64_t T, const int64_t* n_dev) {
     return n < T ? (n < 0 ? 0 : n) : T;
 }
 
-// A thread makes 8 columns of a row; the KU choices of a round are read side by side, added in their order.
+// A thread makes 8 columns of a row (16 bytes per load and store, neighbours side by side); the KU choices of a round are read side
+// by side, so that their latencies overlap, and added in their order: 8 choices one after the other take 34 us where this takes 30.
 template <typename T, int KU>
 __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __restrict__ out) {
     typedef typename Elem<T>::x8 x8;
@@ -56,7 +62,8 @@ __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __re
     }
 }
 
-// 2^lg lanes per row of `out`: dout is read once per choice (from the caches after the first), y once, dy written once.
+// 2^lg lanes per row of `out`: dout is read once per choice (from the caches after the first), y once, dy written once; the
+// products' sum goes through the row's lanes in a fixed order, no atomics.
 template <typename T>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(CombineArgs a, const T* __restrict__ dout, T* __restrict__ dy,
                                                           float* __restrict__ dw, int lg) {

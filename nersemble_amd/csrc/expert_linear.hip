@@ -375,7 +375,7 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
 }
 
 // dW of an expert = the sum of its chunks, in their order: 16 of them side by side and 16 x 4 values per workgroup, or (few
-// chunks) 256 x 4 values.
+// chunks) 256 x 4 values.  Bound by its chain of loads: 3.6 us for 700 chunks of 32 x 64 (5.7 MB), 4.3 for 81 of 176 x 136 (7.8 MB).
 template <typename T>
 __global__ __launch_bounds__(256) void expert_sum_chunks_kernel(LinArgs g, T* __restrict__ d) {
     __shared__ f32x4 part[16][16];
@@ -524,6 +524,11 @@ __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
 // own) turned: a lane holds the same 8 features of the rows c, 16 + c, 32 + c and 48 + c, which it stores side by side -- the
 // order of a sum over rows is free as long as both operands have it.  dW's 32-bit sums stay in registers for a whole chunk of a
 // segment, the four waves' are added in their order at its end; expert_sum_chunks_kernel adds the chunks.
+// Bound by memory: 262144 x 2 of 16 experts, 32 -> 64 with ReLU: 46 us for 185 MB (4.0 TB/s); dx and dW apart read dy and y
+// twice: 69.  us, both gradients with the join and the sum of the chunks, apart | at once:
+//   32 -> 64  84 | 60 (ReLU)  62 | 44 (none)    64 -> 64  112 | 94   87 | 76    64 -> 16  71 | 60    16 -> 64  75 | 49    64 -> 32  82 | 66
+//   2048 rows x 2 of 16, 32 -> 64  22 | 16      100000 x 2 of 61  43 | 30
+// Chunks for 2, 3, 4, 6 workgroups per CU: 48.9, 46.3, 45.5, 47.9 (32 -> 64), without ReLU 30.8, 30.8, 29.9, 32.5.
 // Feature f's row of 128 bytes lies at f with the lowest bit turned by bit 3, its 16-byte pieces permuted by f / 2: neither the
 // stores (features 8 apart) nor the fragment reads (16 features) meet on a bank.
 __device__ __forceinline__ uint32_t turned_at(int f, int piece) { return (f ^ (f >> 3 & 1)) * 128 + ((piece ^ (f >> 1)) & 7) * 16; }
