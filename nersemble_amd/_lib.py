@@ -101,7 +101,7 @@ SIGNATURES = {
     "nsx_expert_plan": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nsx_expert_linear_fwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p,
                                       c_int64, c_int, c_void_p, c_void_p]),
-    "nsx_expert_linear_bwd_workspace": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "nsx_expert_linear_bwd_workspace": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "nsx_expert_linear_bwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p,
                                       c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "nsx_expert_combine_fwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p,

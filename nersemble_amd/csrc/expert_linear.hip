@@ -280,6 +280,11 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
     };
     u32x4 fp[FM], fq[2][FC];
 
+    // Which of a SIMD's waves goes first: the one that multiplies, so that one workgroup's stores fall under another's products; for
+    // dx's large tiles (turning W takes longer) always the same one of two (its slot).  us without | so: 16384 x 2 of 16, 1024 -> 2048
+    // forward 183 | 174, dW 180 | 169, dx 170 | 163;  8192 x 2, 1024 -> 1024  forward 57 | 53, dW 62 | 57;  masked dx 288 | 302: without
+    constexpr int PRIO = MODE == LIN_DX && TM == 256 ? 2 : MODE == LIN_DX && MASK ? 0 : 1;
+    if (PRIO == 2 && (__builtin_amdgcn_s_getreg(4 | 3 << 11) & 1)) __builtin_amdgcn_s_setprio(3);      // HW_ID, bits 3:0: the slot
     if (q_begin < q_end) {
         locate(q_begin);
 #pragma unroll
@@ -288,6 +293,7 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
         for (int i = 0; i < NQ; ++i) load_q(q_begin, i);
         locate(q_begin + LIN_BQ);
         for (int q0 = q_begin; q0 < q_end; q0 += LIN_BQ) {
+            if (PRIO == 1) __builtin_amdgcn_s_setprio(0);
             if (q0 > q_begin) __syncthreads();
 #pragma unroll
             for (int i = 0; i < NP; ++i) put_p(i);
@@ -300,6 +306,7 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
             for (int i = 0; i < FM; ++i) fp[i] = frag(fr_p, wm * (TM / WM), 0, i);
 #pragma unroll
             for (int j = 0; j < FC; ++j) fq[0][j] = frag(fr_q, wc * (TC / WC), 0, j);
+            if (PRIO == 1) __builtin_amdgcn_s_setprio(1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < 4; ++s)
@@ -693,6 +700,21 @@ static void narrow_launch(const LinArgs& g, hipStream_t st) {
     else narrow_launch_m<T, MODE, 4>(g, st);
 }
 
+// dz of the routed rows, once: where many tiles would read y and mask dy again.  Bound by memory: 32768 x 2048, 403 MB: 83 us (4.8 TB/s).
+__global__ __launch_bounds__(256) void expert_mask_kernel(LinArgs g, u32x4* __restrict__ dz) {
+    const int pieces = g.K / 8;
+    const int64_t all = (int64_t)min(max(g.offsets[g.E], 0), g.R) * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / pieces;
+        const int at = (int)(i - r * pieces) * 16;
+        u32x4 v = load16(reinterpret_cast<const char*>(g.q) + r * g.ldq * 2 + at);
+        const u32x4 y = load16(reinterpret_cast<const char*>(g.mask) + r * g.ldmask * 2 + at);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v[w] = keep_where(v[w], y[w]);
+        dz[i] = v;
+    }
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------
 static int lin_check(const char* what, int dtype, int n_in, int n_out, int E, int64_t R, int top_k, const int32_t* offsets) {
     NSX_REQUIRE(dtype == NSX_DTYPE_F16 || dtype == NSX_DTYPE_BF16, "%s: dtype %d is not a 16-bit float", what, dtype);
@@ -764,6 +786,12 @@ static DwPlan dw_plan(int64_t R, int E, int n_in, int n_out) {
 // Where segments have a few rows the 64 x 64 tiles stay: 64 x 8 of 256, 1024 -> 2048: forward 147 | 163 (256 x 128), dx 144 | 149.
 static bool large_tiles(int64_t tiles128) { return tiles128 >= 6 * (int64_t)num_cus(); }
 
+// dz in a pass of its own (3 R n_out 16-bit values) or masked wherever dy is read (y once more per 128 input features in both
+// gradients, registers that large tiles do not have).  us, both gradients, masked in place | once:
+//   16384 x 2 of 16, 1024 -> 2048  616 | 455    2048 -> 1024  573 | 413    8192 x 2, 1024 -> 1024  165 | 143    64 x 8 of 64, 1024 -> 1024  106 | 83
+//   65536 x 2 of 16,  512 -> 128   215 | 183     256 -> 256   172 | 168    128 -> 128  66 | 71                  4096 x 2, 512 -> 512  42.4 | 43.9
+static bool mask_once(int64_t R, int n_in, int n_out) { return n_in >= 1024 || (n_in >= 256 && R * n_out >= 1 << 23); }
+
 template <typename T, int MODE, bool F32>
 static int lin_launch(const LinArgs& g, bool small, hipStream_t st) {
     if constexpr (MODE != LIN_DW)
@@ -803,20 +831,22 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
     return NSX_OK;
 }
 
-// workspace: dx in the plan's order (16-byte steps), then dW's partial sums
+// workspace: dx in the plan's order, dW's partial sums, masked dy (each a multiple of 16 bytes)
 static int64_t bwd_dx_bytes(int64_t R, int n_in, bool gather) { return gather ? R * n_in * 2 : 0; }
 static int64_t bwd_dw_bytes(int64_t R, int E, int n_in, int n_out, bool with_dx) {
     int chunk = with_dx ? nsx::narrow_bwd_chunk(R, n_in, n_out) : 0;
     if (chunk == 0) chunk = nsx::dw_plan(R, E, n_in, n_out).chunk;
     return chunk > 0 ? (R / chunk + E) * n_in * n_out * 4 : 0;
 }
+static int64_t bwd_dz_bytes(int64_t R, int n_in, int n_out) { return nsx::mask_once(R, n_in, n_out) ? R * n_out * 2 : 0; }
 
-int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int gather, int want_dw) {
+int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int gather, int want_dw, int masked) {
     using namespace nsx;
     int32_t some = 0;
     const int rc = lin_check("nsx_expert_linear_bwd_workspace", NSX_DTYPE_F16, n_in, n_out, E, R, 1, &some);
     if (rc != NSX_OK) return rc;
-    return (want_dx ? bwd_dx_bytes(R, n_in, gather) : 0) + (want_dw ? bwd_dw_bytes(R, E, n_in, n_out, want_dx) : 0);
+    return (want_dx ? bwd_dx_bytes(R, n_in, gather) : 0) + (want_dw ? bwd_dw_bytes(R, E, n_in, n_out, want_dx) : 0) +
+           (masked ? bwd_dz_bytes(R, n_in, n_out) : 0);
 }
 
 int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, const int32_t* positions,
@@ -834,15 +864,23 @@ int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_
                 "nsx_expert_linear_bwd: dx needs aligned pointers, weight and, for gathered rows, positions");
     NSX_REQUIRE(!dw || (aligned16(dw) && (x || x_rows == 0) && aligned16(x) && lin_stride(x_stride, n_in)),
                 "nsx_expert_linear_bwd: dw needs aligned pointers and x (row stride %lld)", (long long)x_stride);
-    const int64_t dx_bytes = dx ? bwd_dx_bytes(R, n_in, rows) : 0;
-    NSX_REQUIRE(dx_bytes + (dw ? bwd_dw_bytes(R, E, n_in, n_out, dx != nullptr) : 0) == 0 || (workspace && aligned16(workspace)),
-                "nsx_expert_linear_bwd: no workspace");
+    const int64_t dx_bytes = dx ? bwd_dx_bytes(R, n_in, rows) : 0, dw_bytes = dw ? bwd_dw_bytes(R, E, n_in, n_out, dx != nullptr) : 0;
+    const int64_t dz_bytes = y ? bwd_dz_bytes(R, n_in, n_out) : 0;
+    NSX_REQUIRE(dx_bytes + dw_bytes + dz_bytes == 0 || (workspace && aligned16(workspace)), "nsx_expert_linear_bwd: no workspace");
     hipStream_t st = (hipStream_t)stream;
     LinArgs g{};
     g.q = dy; g.mask = y; g.ldq = dy_stride; g.ldmask = y_stride; g.ldd = n_in; g.offsets = offsets; g.top_k = fast_div(top_k);
     g.E = E; g.R = (int)R; g.M = n_in;
     g.rows = rows; g.x_rows = (int)x_rows; g.C = n_out;
     g.partial = reinterpret_cast<float*>((char*)workspace + dx_bytes);
+    if (dz_bytes && (dx || dw)) {
+        g.K = n_out;
+        u32x4* dz = reinterpret_cast<u32x4*>((char*)workspace + dx_bytes + dw_bytes);
+        const int64_t blocks = (R * (n_out / 8) + 255) / 256;
+        expert_mask_kernel<<<(unsigned)std::min<int64_t>(blocks, 32 * (int64_t)num_cus()), 256, 0, st>>>(g, dz);
+        NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
+        g.q = dz; g.ldq = n_out; g.mask = nullptr;
+    }
     const int at_once = dx && dw ? narrow_bwd_chunk(R, n_in, n_out) : 0;
     if (dx && R > 0) {
         LinArgs h = g;

@@ -208,8 +208,8 @@ def _linear(x, x_stride, w16, plan, gather, relu):
 
 
 @lru_cache(maxsize=1024)
-def _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w):
-    n = lib().nsx_expert_linear_bwd_workspace(R, E, K, N, need_x, gather, need_w)
+def _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w, masked):
+    n = lib().nsx_expert_linear_bwd_workspace(R, E, K, N, need_x, gather, need_w, masked)
     if n < 0:
         check(n, "nsx_expert_linear_bwd_workspace")
     return n
@@ -221,7 +221,7 @@ def _linear_bwd(ctx, dy):
     R, top_k = rows.shape[0], positions.shape[1]
     g, g_stride = _rows_of(dy, 8)
     dev, place = _here(g), g.device
-    need = _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w)
+    need = _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w, y is not None)
     ws = torch.empty((need,), dtype=torch.uint8, device=place) if need else None
     dx = torch.empty((x_rows, K), dtype=g.dtype, device=place) if need_x else None
     dw = torch.empty((E, N, K), dtype=w_dtype, device=place) if need_w else None

@@ -143,9 +143,9 @@ def test_c_abi_refuses_bad_arguments():
     _refused(bwd(ws=None), "workspace")
     _refused(bwd(x_rows=1 << 20, R=1 << 21, dx=None, ws=None), "workspace")
     assert bwd(R=0, x_rows=0, dw=None) == 0 and bwd(dx=None, dw=None) == 0
-    _refused(L.nsx_expert_linear_bwd_workspace(16, 4, 33, 64, 1, 1, 1), "multiples of 8")
-    assert L.nsx_expert_linear_bwd_workspace(16, 4, 32, 64, 1, 1, 0) == 16 * 32 * 2
-    assert L.nsx_expert_linear_bwd_workspace(16, 4, 32, 64, 1, 0, 0) == 0
+    _refused(L.nsx_expert_linear_bwd_workspace(16, 4, 33, 64, 1, 1, 1, 0), "multiples of 8")
+    assert L.nsx_expert_linear_bwd_workspace(16, 4, 32, 64, 1, 1, 0, 1) == 16 * 32 * 2
+    assert L.nsx_expert_linear_bwd_workspace(16, 4, 32, 64, 1, 0, 0, 1) == 0
     _refused(L.nsx_expert_combine_fwd(P, 1, 60, 16, 64, None, P, 8, 2, P, None, None), "stride")
     _refused(L.nsx_expert_combine_fwd(P, 0, 64, 16, 64, None, P, 8, 2, P, None, None), "16-bit")
     _refused(L.nsx_expert_combine_fwd(P, 1, 64, 16, 64, None, None, 8, 2, P, None, None), "NULL")
