@@ -700,7 +700,7 @@ static void narrow_launch(const LinArgs& g, hipStream_t st) {
     else narrow_launch_m<T, MODE, 4>(g, st);
 }
 
-// dz of the routed rows, once: where many tiles would read y and mask dy again.  Bound by memory: 32768 x 2048, 403 MB: 83 us (4.8 TB/s).
+// dz of the routed rows, once: where many tiles would read y and mask dy again.  Bound by memory: 32768 x 2048, 403 MB: 68 us (5.9 TB/s, partly from the caches).
 __global__ __launch_bounds__(256) void expert_mask_kernel(LinArgs g, u32x4* __restrict__ dz) {
     const int pieces = g.K / 8;
     const int64_t all = (int64_t)min(max(g.offsets[g.E], 0), g.R) * pieces;
@@ -752,38 +752,51 @@ static int lin_launch_tile(LinArgs g, hipStream_t st) {
 
 // ---- which tile size ----------------------------------------------------------------------------------------------
 // Forward and dx, us by (rows x choices of experts, n_in -> n_out), bf16, 64 x 64 | 128 x 128 tiles:
-//   16384 x 2 of 16, 1024 -> 2048   339 | 177       4096 x 2 of 16, 1024 -> 1024    38 | 33       1024 x 2 of 16, 512 -> 512   9.5 | 11.0
-//   4 x 8 of 64, 1024 -> 1024      14.8 | 16.9      32 x 8 of 64, 1024 -> 1024    21.9 | 23.9     256 x 8 of 64, 1024 -> 1024 28.5 | 25.5
-//   262144 x 2 of 16, 32 -> 64     29.7 | 38.9      262144 x 2 of 16, 64 -> 16    26.3 | 35.1
+//   4096 x 2 of 16, 1024 -> 1024  39.8 | 34.5      1024 x 2 of 16, 512 -> 512  10.9 | 11.4       4 x 8 of 64, 1024 -> 1024  15.1 | 17.1
+//   32 x 8 of 64, 1024 -> 1024    26.7 | 28.4      256 x 8 of 64, 1024 -> 1024 35.9 | 34.8
+//   262144 x 2 of 16, 32 -> 64    30.2 | 38.4      262144 x 2 of 16, 64 -> 16  27.1 | 36.2
 // The small tile where the result is no wider than it, where a segment has but a few rows, or where the large ones are fewer
 // than the CUs.
 static bool small_tiles(const LinArgs& g) {
     const int64_t rows = g.R / 128 + std::min<int64_t>(g.E, g.R);
     return g.M <= 64 || g.R < 16 * (int64_t)g.E || rows * ((g.M + 127) / 128) < num_cus();
 }
-// dW, chunk (0: none) and tile.  us with chunks of 256 | 512 | 1024 | 2048 rows:
-//   262144 x 2 of 16,  32 ->  64   64 x 64 tiles  45 | 40 | 39 | 50     128 x 128 tiles  63 |  54 |  58 |  61
-//    65536 x 2 of 16, 128 -> 128   64 x 64 tiles  36 | 31 | 38 | 52     128 x 128 tiles  40 |  33 |  37 |  55
-//    65536 x 2 of 16, 256 -> 256   64 x 64 tiles 118 | 81 | 80 | 84     128 x 128 tiles 110 |  79 |  79 |  80
-//     5003 x 3 of 23, 176 -> 136   64 x 64 tiles  24 | 26 | 32 | 37     128 x 128 tiles  25 |  27 |  36 |  43
-// Short chunks fill the card, long ones keep the partial sums small beside what is read: about four workgroups per CU.
-// Without chunks (the matrices have tiles enough) the larger tiles are faster: 16384 x 2 of 16, 1024 -> 2048: 570 | 180.
+// dW, chunk (0: none) and tile.  us with chunks of 256 | 512 | 1024 | 2048 | 4096 rows, then without:
+//   262144 x 2 of 16,  32 ->   64   64 x 64 tiles   37 |  31 |  30 |  40                  128 x 128 tiles   47 |  40 |  39 |  46
+//    65536 x 2 of 16, 128 ->  128   64 x 64 tiles   31 |  27 |  30 |  42                  128 x 128 tiles   32 |  28 |  32 |  46
+//    65536 x 2 of 16, 256 ->  256   64 x 64 tiles  108 |  88 |  80 |  63 |  87;  247      128 x 128 tiles   93 |  76 |  65 |  60 |  92;  282
+//    65536 x 2 of 16, 512 ->  512   64 x 64 tiles    - | 316 | 224 | 199 | 204;  276      128 x 128 tiles    - | 259 | 160 | 141 | 146;  285
+//    65536 x 2 of 4, 1024 -> 1024   64 x 64 tiles    - | 998 | 787 | 690 | 646;  761      128 x 128 tiles    - | 834 | 585 | 466 | 402;  800
+//    16384 x 2 of 8,  768 ->  768   64 x 64 tiles  250 | 148 | 119 | 111 |   -;  116      128 x 128 tiles  278 | 164 | 129 | 115 |   -;  122
+//     8192 x 2 of 16, 512 ->  512   64 x 64 tiles   50 |  40 |  38 |  44 |   -;   35      128 x 128 tiles   46 |  37 |  36 |  44 |   -;   36
+//     5003 x 3 of 23, 176 ->  136   64 x 64 tiles   21 |  22 |  27 |  32                  128 x 128 tiles   22 |  24 |  30 |  36
+// Short chunks fill the card, long ones keep the partial sums small beside what is read: two workgroups per CU of the large tiles,
+// four of the small ones.  Without chunks where the matrices have tiles enough: 16384 x 2 of 16, 1024 -> 2048 then takes 570 | 180;
+// of small tiles only up to 8192 rows per expert.  (The lines above have segments of 0.4 to 1.5 of the mean.  Where they are nearly
+// equal, both gradients with chunks of large tiles | without chunks, small ones: 16384 x 2 of 8, 768 -> 768  203 | 168;  8192 x 2 of 16,
+// 512 -> 512  63 | 53;  65536 x 2 of 16, 512 -> 512  318 | 344;  of 4, 1024 -> 1024  898 | 1110.)
 struct DwPlan { int chunk; bool small; };
 static DwPlan dw_plan(int64_t R, int E, int n_in, int n_out) {
+    const int64_t cus = num_cus();
     const int64_t large = (int64_t)((n_in + 127) / 128) * ((n_out + 127) / 128), small = (int64_t)((n_in + 63) / 64) * ((n_out + 63) / 64);
-    if (large * E >= 2 * (int64_t)num_cus()) return {0, false};
-    if (small * E >= 4 * (int64_t)num_cus() || R < 8 * (int64_t)LIN_BQ) return {0, true};
-    int64_t chunk = R * small / (4 * (int64_t)num_cus());
-    chunk = (chunk + LIN_BQ - 1) / LIN_BQ * LIN_BQ;
-    return {(int)std::min<int64_t>(std::max<int64_t>(chunk, 4 * LIN_BQ), 1024), true};
+    if (large * E >= 2 * cus) return {0, false};
+    auto rows = [](int64_t n, int64_t least, int64_t most) { return (int)std::min(std::max((n + LIN_BQ - 1) / LIN_BQ * LIN_BQ, least), most); };
+    const bool enough = small * E >= 4 * cus;
+    if (n_in >= 256 && n_out >= 256 && R * large >= 512 * 2 * cus && (!enough || R >= 8192 * (int64_t)E)) return {rows(R * large / (2 * cus), 512, 4096), false};
+    if (enough || R < 8 * (int64_t)LIN_BQ) return {0, true};
+    return {rows(R * small / (4 * cus), 4 * LIN_BQ, 1024), true};
 }
 
 // The largest products: a wave's tile of 128 x 64 needs three quarters of the LDS reads.  us with 128 x 128 | 256 x 128 | 128 x 256:
-//   16384 x 2 of 16, 1024 -> 2048   forward 172 | 162 | 173   dx 158 | 152 | 158   dW 177 | 178 | 166
-//   16384 x 2 of 8,  2048 -> 2048   forward 322 | 292 | 306   dx 304 | 287 | 289   dW 328 | 318 | 303
-//    8192 x 2 of 16, 1024 -> 1024   forward  52 |  56 |  58   dx  48 |  51 |  51   dW  59 |  62 |  57
-//    2048 x 8 of 256, 2048 -> 1024  forward 221 | 208 |       dx 259 | 223     (64 x 64: 283, 282)
-// Where segments have a few rows the 64 x 64 tiles stay: 64 x 8 of 256, 1024 -> 2048: forward 147 | 163 (256 x 128), dx 144 | 149.
+//   16384 x 2 of 16, 1024 -> 2048   forward 196 | 181 | 186   dx 174 | 168 | 175   dW 190 | 190 | 168
+//   16384 x 2 of 8,  2048 -> 2048   forward 319 | 298 | 310   dx 305 | 309 | 305   dW 355 | 336 | 293
+//    8192 x 2 of 16, 1024 -> 1024   forward  52 |  58 |  63   dx  54 |  57 |  62   dW  56 |  65 |  55
+//    2048 x 8 of 256, 2048 -> 1024  forward 257 | 243 |       dx 253 | 233     (64 x 64: 269, 276)
+// All bound by LDS: 256 x 128 tiles read and write 36 KB of it per 16 of q, 288 cycles beside the products' 256.  As time = f + q s the
+// forward of the first line has f = 36 us (its result's bytes alone 27), s = 133 us per 1024 of q, 1030 TFLOP/s.  256 x 256 tiles with
+// 4 waves of 128 x 128 (LDS 192) have a workgroup per CU, whose start and stores nothing covers: f = 59, the same s; with loads
+// straight into LDS each step waits for its memory (1.3 us after the issue at the earliest; the products take 1.2).
+// Where segments have a few rows the 64 x 64 tiles stay: 64 x 8 of 256, 1024 -> 2048: forward 150 | 167 (256 x 128), dx 145 | 149.
 static bool large_tiles(int64_t tiles128) { return tiles128 >= 6 * (int64_t)num_cus(); }
 
 // dz in a pass of its own (3 R n_out 16-bit values) or masked wherever dy is read (y once more per 128 input features in both

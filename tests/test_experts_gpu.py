@@ -326,7 +326,7 @@ def test_linear_rows_behind_the_last_segment_are_zero_whatever_the_weights(K, N,
     assert (dh[[0, 2]] == 0).all()
 
 
-@pytest.mark.parametrize("T,k,E,K,N", [(16384, 2, 17, 1000, 2056), (9000, 3, 70, 776, 776)])
+@pytest.mark.parametrize("T,k,E,K,N", [(16384, 2, 17, 1000, 2056), (9000, 3, 70, 776, 776), (20000, 2, 5, 264, 520), (40001, 1, 3, 512, 256)])
 @pytest.mark.parametrize("dtype,relu,master", [("bf16", False, False), ("fp16", True, False), ("fp16", False, True)])
 def test_linear_largest_tiles(T, k, E, K, N, dtype, relu, master, cuda):
     """Products of thousands of tiles, one expert with a third of the rows, against 64-bit products of each segment."""
@@ -334,7 +334,7 @@ def test_linear_largest_tiles(T, k, E, K, N, dtype, relu, master, cuda):
     g = torch.Generator(device=cuda).manual_seed(T)
     dt, (h, tiny) = DT[dtype], HALF[DT[dtype]]
     logits = torch.randn((T, E), generator=g, device=cuda)
-    logits[:, 3] += 2
+    logits[:, min(3, E - 1)] += 2
     _, c = X.route_experts(logits, k)
     c[::10] = -1
     plan = X.expert_plan(c, E)
@@ -360,7 +360,7 @@ def test_linear_largest_tiles(T, k, E, K, N, dtype, relu, master, cuda):
         inside(y[a:b], want, h * want.abs() + tiny + (K + 2) * 2 * U * mag, "y")
         dz = dy[a:b].double() * (y[a:b] > 0) if relu else dy[a:b].double()
         want, mag = dz.t() @ xe, dz.t().abs() @ xe.abs()
-        inside(dw[e], want, (b - a + 2) * 2 * U * mag + (0 if master else h * want.abs() + tiny), "dw")
+        inside(dw[e], want, (b - a + 66) * 2 * U * mag + (0 if master else h * want.abs() + tiny), "dw")
         want, mag = dz @ we, dz.abs() @ we.abs()
         wx.index_add_(0, r, want)
         tx.index_add_(0, r, h * want.abs() + tiny + (N + 2 + k) * 2 * U * mag)
