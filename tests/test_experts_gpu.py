@@ -843,3 +843,29 @@ def test_two_runs_at_once_on_two_streams(cuda):
         for r in got[i]:
             for p, q in zip(r, want[i]):
                 assert torch.equal(p, q)
+
+
+def test_routed_network_rows_that_are_not_evaluated(cuda):
+    """What `selector` leaves out may hold anything: outputs 0, gradients as if the rows were not there; no rows at all work too."""
+    from nersemble_amd import tcnn
+    net = tcnn.RoutedNetwork(20, 5, {"n_neurons": 64, "n_hidden_layers": 2}, {"n_experts": 6, "top_k": 2}).to(cuda)
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn((300, 20), generator=g).to(cuda)
+    sel = (torch.arange(300, device=cuda) % 4 != 0).to(torch.uint8)
+    go = torch.randn((300, 5), generator=g).half().to(cuda)
+    grads = []
+    for fill in (0.0, float("nan"), float("inf")):
+        v = x.clone()
+        v[sel == 0] = fill
+        v.requires_grad_(True)
+        out = net(v, sel)
+        assert (out[sel == 0] == 0).all()
+        grads.append([out] + list(torch.autograd.grad(out, [v, net.params, net.gate], go)))
+    for other in grads[1:]:
+        for a, b in zip(grads[0], other):
+            assert torch.isfinite(b).all() and torch.equal(a, b)
+    assert (grads[0][1][sel == 0] == 0).all()
+    empty = net(x[:0].requires_grad_(True))
+    assert empty.shape == (0, 5)
+    (gp,) = torch.autograd.grad(empty.sum(), [net.params])
+    assert (gp == 0).all()
