@@ -7,7 +7,8 @@
     out = expert_combine(y, weights, plan)                    # [T, n]
 
 (The reference's only mixture is the dense blend of all hash grids, hash_ensemble.py:133-156; ``tcnn.RoutedNetwork`` is the
-module built on these calls.)  All four launch on torch's current stream, keep nothing between calls, never read the device from the host and can be captured into a graph.  Under
+module built on these calls.)  All four launch on torch's current stream, keep nothing between calls, never read the device from
+the host and can be captured into a graph.  Under
 ``_lib.device_count`` rows behind the device-side count are not routed, and not written by ``route_experts`` and
 ``expert_combine``.  A plan's numbers are bounded inside the kernels; equal inputs give equal bits.
 """
@@ -26,6 +27,24 @@ _DTYPE = {torch.float32: _lib.NSX_DTYPE_F32, torch.float16: _lib.NSX_DTYPE_F16, 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _F32, _I32 = torch.float32, torch.int32
 _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_profiler = _lib.profiler
+
+
+class _NotLoaded:
+    """The library before its first call (``_lib.lib`` says so where it is missing)."""
+
+    def __getattr__(self, name):
+        global _native
+        lib()
+        _native = _lib._lib._h
+        return getattr(_native, name)
+
+
+_native = _NotLoaded()
+
+
+def _libnsx():
+    return lib() if _profiler.enabled else _native
 
 
 class ExpertPlan:
@@ -33,7 +52,7 @@ class ExpertPlan:
 
     offsets [E + 1]: the ordered rows of expert e are offsets[e] .. offsets[e + 1]; rows [T * top_k]: entry of every ordered
     row, -1 behind the last segment; positions [T, top_k]: ordered row of every entry, -1 for an entry that is not routed."""
-    __slots__ = ("offsets", "rows", "positions", "n_experts", "n_rows", "top_k", "n_entries")
+    __slots__ = ("offsets", "rows", "positions", "n_experts", "n_rows", "top_k", "n_entries", "device")
 
     def __init__(self, offsets: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor):
         o, r, p = offsets.shape, rows.shape, positions.shape
@@ -41,11 +60,25 @@ class ExpertPlan:
                 or not offsets.dtype == rows.dtype == positions.dtype == _I32:
             raise RuntimeError(f"ExpertPlan: offsets [E + 1], rows [T * top_k] and positions [T, top_k] are int32 (got {tuple(o)} "
                                f"{offsets.dtype}, {tuple(r)} {rows.dtype}, {tuple(p)} {positions.dtype})")
+        self.device = offsets.get_device()
+        if not self.device == rows.get_device() == positions.get_device():
+            raise RuntimeError(f"ExpertPlan: offsets, rows and positions are on {offsets.device}, {rows.device} and {positions.device}")
         if not (offsets.is_contiguous() and rows.is_contiguous() and positions.is_contiguous()):
             offsets, rows, positions = offsets.contiguous(), rows.contiguous(), positions.contiguous()
         self.offsets, self.rows, self.positions = offsets, rows, positions
         self.n_experts, self.n_entries = o[0] - 1, r[0]
         self.n_rows, self.top_k = p
+
+    def _version(self):
+        return self.offsets._version + self.rows._version + self.positions._version
+
+
+def _plan_of(ctx) -> ExpertPlan:
+    """The plan of a forward pass, which has to be as it was then."""
+    plan, version = ctx.plan
+    if plan._version() != version:
+        raise RuntimeError("the plan that the forward pass used has been modified by an inplace operation")
+    return plan
 
 
 def _rows_of(t: torch.Tensor, align: int) -> Tuple[torch.Tensor, int]:
@@ -85,10 +118,12 @@ def _route(x, stride, bias, selector, top_k, sigmoid, n_groups, top_groups, grou
     dev = _here(x)
     weights = x.new_empty((T, top_k), dtype=_F32)
     chosen = x.new_empty((T, top_k), dtype=_I32)
-    check(lib().nsx_expert_route_fwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, None if bias is None else _at(bias, dev),
-                                     None if selector is None else _at(selector, dev), top_k, sigmoid, n_groups, top_groups, group_top,
-                                     renorm, scale, weights.data_ptr(), chosen.data_ptr(), ndev(T), _raw_stream(dev)),
-          "nsx_expert_route_fwd")
+    rc = _libnsx().nsx_expert_route_fwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, None if bias is None else _at(bias, dev),
+                                    None if selector is None else _at(selector, dev), top_k, sigmoid, n_groups, top_groups, group_top,
+                                    renorm, scale, weights.data_ptr(), chosen.data_ptr(),
+                                    None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
+    if rc:
+        check(rc, "nsx_expert_route_fwd")
     return weights, chosen
 
 
@@ -100,11 +135,13 @@ def _route_bwd(ctx, g, _):
     T, E = x.shape
     if g.dtype != _F32 or not g.is_contiguous():
         g = g.to(_F32).contiguous()
-    dev = _here(x)
-    d = torch.empty((T, E), dtype=x.dtype, device=x.device)
-    check(lib().nsx_expert_route_bwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, top_k, sigmoid, renorm, scale, weights.data_ptr(),
-                                     chosen.data_ptr(), _at(g, dev), d.data_ptr(), ndev(T), _raw_stream(dev)),
-          "nsx_expert_route_bwd")
+    dev = x.get_device()
+    d = torch.empty_like(x) if stride == E else x.new_empty((T, E))
+    rc = _libnsx().nsx_expert_route_bwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, top_k, sigmoid, renorm, scale, weights.data_ptr(),
+                                    chosen.data_ptr(), g.data_ptr(), d.data_ptr(),
+                                    None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
+    if rc:
+        check(rc, "nsx_expert_route_bwd")
     return d, None, None, None
 
 
@@ -147,7 +184,8 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
     if bias is not None:
         if bias.shape != (E,) or bias.dtype != _F32:
             raise RuntimeError(f"route_experts: bias is {tuple(bias.shape)} {bias.dtype}, not ({E},) fp32")
-        bias = bias.detach().contiguous()
+        if bias.requires_grad or not bias.is_contiguous():
+            bias = bias.detach().contiguous()
     if selector is not None:
         if selector.numel() != T:
             raise RuntimeError(f"route_experts: selector has {selector.numel()} entries for {T} rows")
@@ -189,9 +227,15 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
     dev = _here(chosen)
     buf = chosen.new_empty((o + 2 * r + need // 4,))
     base = buf.data_ptr()
-    check(lib().nsx_expert_plan(chosen.data_ptr(), T, k, n_experts, base, base + 4 * o, base + 4 * (o + r), base + 4 * (o + 2 * r), ndev(T),
-                                _raw_stream(dev)), "nsx_expert_plan")
-    return ExpertPlan(buf[:n_experts + 1], buf[o:o + T * k], buf[o + r:o + r + T * k].view(T, k))
+    rc = _libnsx().nsx_expert_plan(chosen.data_ptr(), T, k, n_experts, base, base + 4 * o, base + 4 * (o + r), base + 4 * (o + 2 * r),
+                                   None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
+    if rc:
+        check(rc, "nsx_expert_plan")
+    plan = ExpertPlan.__new__(ExpertPlan)
+    plan.offsets, plan.rows = buf.as_strided((n_experts + 1,), (1,), 0), buf.as_strided((T * k,), (1,), o)
+    plan.positions = buf.as_strided((T, k), (k, 1), o + r)
+    plan.n_experts, plan.n_entries, plan.n_rows, plan.top_k, plan.device = n_experts, T * k, T, k, dev
+    return plan
 
 
 # ------------------------------------------------------------------------------------------------
@@ -200,10 +244,15 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
 def _linear(x, x_stride, w16, plan, gather, relu):
     E, N, K = w16.shape
     dev = _here(x)
-    y = x.new_empty((plan.n_entries, N))
-    check(lib().nsx_expert_linear_fwd(x.data_ptr(), _DTYPE[x.dtype], x_stride, x.shape[0], _at(plan.rows, dev) if gather else None, plan.top_k,
-                                      _at(w16, dev), K, N, E, _at(plan.offsets, dev), plan.n_entries, relu, y.data_ptr(),
-                                      _raw_stream(dev)), "nsx_expert_linear_fwd")
+    if w16.get_device() != dev or plan.device != dev:
+        ptr(w16), ptr(plan.offsets)
+    n = plan.n_entries
+    y = x.new_empty((n, N))
+    rc = _libnsx().nsx_expert_linear_fwd(x.data_ptr(), _DTYPE[x.dtype], x_stride, x.shape[0], plan.rows.data_ptr() if gather else None,
+                                     plan.top_k, w16.data_ptr(), K, N, E, plan.offsets.data_ptr(), n, relu, y.data_ptr(),
+                                     _raw_stream(dev))
+    if rc:
+        check(rc, "nsx_expert_linear_fwd")
     return y
 
 
@@ -216,20 +265,26 @@ def _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w, masked):
 
 
 def _linear_bwd(ctx, dy):
-    x, w16, y, offsets, rows, positions = ctx.saved_tensors
+    x, w16, y = ctx.saved_tensors
     x_stride, x_rows, (E, N, K), gather, w_dtype, need_x, need_w = ctx.cfg
-    R, top_k = rows.shape[0], positions.shape[1]
-    g, g_stride = _rows_of(dy, 8)
-    dev, place = _here(g), g.device
+    plan = _plan_of(ctx)
+    R = plan.n_entries
+    if dy.is_contiguous() and dy.data_ptr() % 16 == 0:
+        g, g_stride = dy, N
+    else:
+        g, g_stride = _rows_of(dy, 8)
+    dev = _here(g)
     need = _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w, y is not None)
-    ws = torch.empty((need,), dtype=torch.uint8, device=place) if need else None
-    dx = torch.empty((x_rows, K), dtype=g.dtype, device=place) if need_x else None
-    dw = torch.empty((E, N, K), dtype=w_dtype, device=place) if need_w else None
-    check(lib().nsx_expert_linear_bwd(
-        _at(x, dev) if need_w else None, _DTYPE[g.dtype], x_stride, x_rows, _at(rows, dev) if gather else None, _at(positions, dev), top_k,
-        _at(w16, dev) if need_x else None, g.data_ptr(), g_stride, None if y is None else _at(y, dev), N, K, N, E, _at(offsets, dev), R,
-        dx.data_ptr() if need_x else None, w_dtype == _F32, dw.data_ptr() if need_w else None, ws.data_ptr() if need else None,
-        _raw_stream(dev)), "nsx_expert_linear_bwd")
+    ws = g.new_empty((need // 2,)) if need else None
+    dx = g.new_empty((x_rows, K)) if need_x else None
+    dw = None if not need_w else g.new_empty((E, N, K)) if w_dtype == g.dtype else g.new_empty((E, N, K), dtype=w_dtype)
+    rc = _libnsx().nsx_expert_linear_bwd(
+        x.data_ptr() if need_w else None, _DTYPE[g.dtype], x_stride, x_rows, plan.rows.data_ptr() if gather else None,
+        plan.positions.data_ptr(), plan.top_k, w16.data_ptr() if need_x else None, g.data_ptr(), g_stride,
+        None if y is None else y.data_ptr(), N, K, N, E, plan.offsets.data_ptr(), R, dx.data_ptr() if need_x else None,
+        w_dtype == _F32, dw.data_ptr() if need_w else None, ws.data_ptr() if need else None, _raw_stream(dev))
+    if rc:
+        check(rc, "nsx_expert_linear_bwd")
     return dx, dw, None, None, None, None
 
 
@@ -239,8 +294,8 @@ class _LinearFn(torch.autograd.Function):
         xr, x_stride = _rows_of(x, 8)
         y = _linear(xr, x_stride, w16, plan, gather, relu)
         need_x, need_w = ctx.needs_input_grad[:2]
-        ctx.save_for_backward(xr if need_w else None, w16 if need_x else None, y if relu else None,
-                              plan.offsets, plan.rows, plan.positions)
+        ctx.save_for_backward(xr if need_w else None, w16 if need_x else None, y if relu else None)
+        ctx.plan = plan, plan._version()
         ctx.cfg = (x_stride, x.shape[0], w16.shape, gather, weight.dtype, need_x, need_w)
         return y
 
@@ -270,16 +325,14 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gathe
     if xs[0] != (plan.n_rows if gather else plan.n_entries):
         raise RuntimeError(f"expert_linear: x has {xs[0]} rows for a plan of {plan.n_rows} x {plan.top_k} entries (gather={bool(gather)})")
     if w16 is None:
-        w16 = weight.detach() if wt == xt else weight.detach().to(xt)
+        w16 = weight if wt == xt else weight.detach().to(xt)
     elif w16.shape != ws or w16.dtype != xt:
         raise RuntimeError(f"expert_linear: w16 is {tuple(w16.shape)} {w16.dtype}, not {tuple(ws)} {xt}")
-    else:
-        w16 = w16.detach()
     if not w16.is_contiguous():
         w16 = w16.contiguous()
     if w16.data_ptr() % 16:
         w16 = w16.clone()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return _LinearFn.apply(x, weight, w16, plan, bool(gather), bool(relu))
     xr, x_stride = _rows_of(x, 8)
     return _linear(xr, x_stride, w16, plan, bool(gather), bool(relu))
@@ -288,31 +341,38 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gathe
 # ------------------------------------------------------------------------------------------------
 # join
 # ------------------------------------------------------------------------------------------------
-def _combine(y, y_stride, weights, positions):
-    T, k = positions.shape
+def _combine(y, y_stride, weights, plan):
     R, n = y.shape
+    T = plan.n_rows
     dev = _here(y)
+    if weights.get_device() != dev or plan.device != dev:
+        ptr(weights), ptr(plan.positions)
     out = y.new_empty((T, n))
-    check(lib().nsx_expert_combine_fwd(y.data_ptr(), _DTYPE[y.dtype], y_stride, R, n, None if weights is None else _at(weights, dev),
-                                       _at(positions, dev), T, k, out.data_ptr(), ndev(T), _raw_stream(dev)), "nsx_expert_combine_fwd")
+    rc = _libnsx().nsx_expert_combine_fwd(y.data_ptr(), _DTYPE[y.dtype], y_stride, R, n, weights.data_ptr(), plan.positions.data_ptr(), T,
+                                      plan.top_k, out.data_ptr(), None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
+    if rc:
+        check(rc, "nsx_expert_combine_fwd")
     return out
 
 
 def _combine_bwd(ctx, dout):
-    y, w, offsets, positions = ctx.saved_tensors
+    y, w = ctx.saved_tensors
     stride, w_dtype = ctx.cfg
-    T, k = positions.shape
+    plan = _plan_of(ctx)
+    T, k = plan.n_rows, plan.top_k
     R, n = y.shape
     if not dout.is_contiguous():
         dout = dout.contiguous()
     if dout.data_ptr() % 16:
         dout = dout.clone()
-    dev = _here(y)
-    dy = torch.empty((R, n), dtype=y.dtype, device=y.device)
-    dw = torch.empty((T, k), dtype=_F32, device=y.device)
-    check(lib().nsx_expert_combine_bwd(y.data_ptr(), _DTYPE[y.dtype], stride, R, n, _at(w, dev), _at(positions, dev),
-                                       _at(offsets, dev) + 4 * (offsets.shape[0] - 1), T, k, _at(dout, dev), dy.data_ptr(),
-                                       dw.data_ptr(), ndev(T), _raw_stream(dev)), "nsx_expert_combine_bwd")
+    dev = y.get_device()
+    dy = torch.empty_like(y) if stride == n else y.new_empty((R, n))
+    dw = torch.empty_like(w)
+    rc = _libnsx().nsx_expert_combine_bwd(y.data_ptr(), _DTYPE[y.dtype], stride, R, n, w.data_ptr(), plan.positions.data_ptr(),
+                                      plan.offsets.data_ptr() + 4 * plan.n_experts, T, k, dout.data_ptr(), dy.data_ptr(),
+                                      dw.data_ptr(), None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
+    if rc:
+        check(rc, "nsx_expert_combine_bwd")
     return dy, dw if w_dtype == _F32 else dw.to(w_dtype), None
 
 
@@ -321,9 +381,10 @@ class _CombineFn(torch.autograd.Function):
     def forward(ctx, y, weights, plan):
         yr, stride = _rows_of(y, 8)
         w = weights if weights.dtype == _F32 and weights.is_contiguous() else weights.to(_F32).contiguous()
-        ctx.save_for_backward(yr, w, plan.offsets, plan.positions)
+        ctx.save_for_backward(yr, w)
+        ctx.plan = plan, plan._version()
         ctx.cfg = (stride, weights.dtype)
-        return _combine(yr, stride, w, plan.positions)
+        return _combine(yr, stride, w, plan)
 
     @staticmethod
     def backward(ctx, dout):
@@ -339,9 +400,9 @@ def expert_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) -> 
     ys = y.shape
     if len(ys) != 2 or ys[0] != plan.n_entries or y.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"expert_combine: y is [{plan.n_entries}, n] in fp16 or bf16 (got {tuple(ys)} {y.dtype})")
-    if weights.shape != plan.positions.shape or not weights.is_floating_point():
-        raise RuntimeError(f"expert_combine: weights are {tuple(plan.positions.shape)} (got {tuple(weights.shape)} {weights.dtype})")
-    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
+    if weights.shape != (plan.n_rows, plan.top_k) or not weights.is_floating_point():
+        raise RuntimeError(f"expert_combine: weights are {(plan.n_rows, plan.top_k)} (got {tuple(weights.shape)} {weights.dtype})")
+    if (y.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
         return _CombineFn.apply(y, weights, plan)
     yr, stride = _rows_of(y, 8)
-    return _combine(yr, stride, weights.to(_F32).contiguous(), plan.positions)
+    return _combine(yr, stride, weights if weights.dtype == _F32 and weights.is_contiguous() else weights.to(_F32).contiguous(), plan)
