@@ -4,8 +4,9 @@
 // to 16 bits once (dy: one product, rounded).
 // Bound by memory: y is read once, by rows of the plan's order, out or dy written once.  us and bytes / time:
 //   262144 rows x 2 choices, 64 columns fp16     forward 19.6 (105 MB, 5.4 TB/s)   backward 35.7 (174 MB, 4.9 TB/s)
-//   8192 x 8, 1024 columns bf16                  forward 30.4 (151 MB, 5.0 TB/s)   backward 65 (286 MB, 4.4 TB/s; a copy 4.96)
-// Stores past the caches (nontemporal) took 17, 32, 28.6 and 60 us, but the next reader of the result pays what they gain.
+//   8192 x 8, 1024 columns bf16                  forward 30.4 (151 MB, 5.0 TB/s)   backward 63 (286 MB, 4.5 TB/s; a copy 4.96)
+//   524289 x 2, 16 columns fp16                                                    backward 22.8 (96 MB, 4.2 TB/s)
+// Stores past the caches (nontemporal) took 17, 32, 28.6 and 60 us (the first two lines), but the next reader of the result pays what they gain.
 #include "expert_common.h"
 
 namespace nsx {
@@ -62,9 +63,10 @@ __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __re
     }
 }
 
-// 2^lg lanes per row of `out`: dout is read once per choice (from the caches after the first), y once, dy written once; the
+// 2^lg lanes per row of `out`: y is read once, dy written once, dout once or (from the caches) once per choice; the
 // products' sum goes through the row's lanes in a fixed order, no atomics.
-template <typename T>
+// CP: pieces of a row that a lane keeps in registers (0: any number, dout read again for every choice); KU: choices side by side.
+template <typename T, int CP, int KU>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(CombineArgs a, const T* __restrict__ dout, T* __restrict__ dy,
                                                           float* __restrict__ dw, int lg) {
     typedef typename Elem<T>::x8 x8;
@@ -72,23 +74,50 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(CombineArgs a, const T
     const int64_t T_ = valid_rows(a.T, a.n_dev);
     const int64_t step = ((int64_t)gridDim.x * 256) >> lg;
     for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lg; t < T_; t += step) {
-        for (int j = 0; j < a.k; ++j) {
-            const int p = a.positions[t * a.k + j];
-            const bool there = (unsigned)p < (unsigned)a.R;
-            float dot = 0.f;
-            if (there) {
-                const float w = a.w[t * a.k + j];
-                for (int c = sub; c < a.chunks; c += lanes) {
-                    const x8 g = *reinterpret_cast<const x8*>(dout + (t * a.chunks + c) * 8);
-                    const x8 v = *reinterpret_cast<const x8*>(reinterpret_cast<const T*>(a.y) + (int64_t)p * a.y_stride + c * 8);
-                    x8 o;
+        x8 g[CP > 0 ? CP : 1];
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) { dot += (float)g[q] * (float)v[q]; o[q] = (T)(w * (float)g[q]); }
-                    *reinterpret_cast<x8*>(dy + ((int64_t)p * a.chunks + c) * 8) = o;
-                }
+        for (int i = 0; i < CP; ++i) {
+            const int c = sub + i * lanes;
+            if (c < a.chunks) g[i] = *reinterpret_cast<const x8*>(dout + (t * a.chunks + c) * 8);
+        }
+        for (int j = 0; j < a.k; j += KU) {
+            int p[KU];
+            float w[KU], dot[KU];
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+                const bool in = KU == 1 || j + u < a.k;
+                p[u] = in ? a.positions[t * a.k + j + u] : -1;
+                w[u] = in ? a.w[t * a.k + j + u] : 0.f;
+                dot[u] = 0.f;
             }
-            for (int o = 1; o < lanes; o <<= 1) dot += __shfl_xor(dot, o);
-            if (sub == 0) dw[t * a.k + j] = there ? dot : 0.f;
+            auto piece = [&](int u, int c, x8 g, x8 v) {
+                x8 o;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) { dot[u] += (float)g[q] * (float)v[q]; o[q] = (T)(w[u] * (float)g[q]); }
+                *reinterpret_cast<x8*>(dy + ((int64_t)p[u] * a.chunks + c) * 8) = o;
+            };
+            auto read = [&](int u, int c) { return *reinterpret_cast<const x8*>(reinterpret_cast<const T*>(a.y) + (int64_t)p[u] * a.y_stride + c * 8); };
+            if (CP > 0) {
+                x8 v[KU][CP > 0 ? CP : 1];
+#pragma unroll
+                for (int u = 0; u < KU; ++u)
+                    if ((unsigned)p[u] < (unsigned)a.R)
+#pragma unroll
+                        for (int i = 0; i < CP; ++i) if (sub + i * lanes < a.chunks) v[u][i] = read(u, sub + i * lanes);
+#pragma unroll
+                for (int u = 0; u < KU; ++u)
+                    if ((unsigned)p[u] < (unsigned)a.R)
+#pragma unroll
+                        for (int i = 0; i < CP; ++i) if (sub + i * lanes < a.chunks) piece(u, sub + i * lanes, g[i], v[u][i]);
+            } else if ((unsigned)p[0] < (unsigned)a.R) {
+                for (int c = sub; c < a.chunks; c += lanes)
+                    piece(0, c, *reinterpret_cast<const x8*>(dout + (t * a.chunks + c) * 8), read(0, c));
+            }
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+                for (int o = 1; o < lanes; o <<= 1) dot[u] += __shfl_xor(dot[u], o);
+                if (sub == 0 && j + u < a.k) dw[t * a.k + j + u] = (unsigned)p[u] < (unsigned)a.R ? dot[u] : 0.f;
+            }
         }
     }
     // rows of dy behind the last segment
@@ -100,6 +129,14 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(CombineArgs a, const T
         *reinterpret_cast<x8*>(dy + i * 8) = z;
 }
 
+template <typename T>
+static void combine_bwd_launch(const CombineArgs& a, const T* dout, T* dy, float* dw, int lg, unsigned grid, hipStream_t st) {
+    // us, dout read for every choice | kept, two choices at a time: rows of 16 columns, 524289 x 2  28.8 | 22.7, of 64, 262144 x 2
+    // 35.2 | 36.0, of 512, 4096 x 4  8.6 | 9.1, of 520, 20000 x 3  37.1 | 38.1, of 1024, 8192 x 8  65.5 | 63.1, of 2048, 16384 x 2  68.2 | 71.3
+    if (lg <= 2) combine_bwd_kernel<T, 1, 2><<<grid, 256, 0, st>>>(a, dout, dy, dw, lg);
+    else if (a.chunks > 96 && a.chunks <= 128) combine_bwd_kernel<T, 2, 2><<<grid, 256, 0, st>>>(a, dout, dy, dw, lg);
+    else combine_bwd_kernel<T, 0, 1><<<grid, 256, 0, st>>>(a, dout, dy, dw, lg);
+}
 template <typename T>
 static void combine_fwd_launch(const CombineArgs& a, T* out, unsigned grid, hipStream_t st) {
     if (a.k == 1) combine_fwd_kernel<T, 1><<<grid, 256, 0, st>>>(a, out);
@@ -156,9 +193,9 @@ int nsx_expert_combine_bwd(const void* y, int dtype, int64_t y_stride, int64_t R
     const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == NSX_DTYPE_F16)
-        combine_bwd_kernel<half_t><<<grid, 256, 0, st>>>(a, (const half_t*)dout, (half_t*)dy, dweights, lg);
+        combine_bwd_launch(a, (const half_t*)dout, (half_t*)dy, dweights, lg, grid, st);
     else
-        combine_bwd_kernel<bf16_t><<<grid, 256, 0, st>>>(a, (const bf16_t*)dout, (bf16_t*)dy, dweights, lg);
+        combine_bwd_launch(a, (const bf16_t*)dout, (bf16_t*)dy, dweights, lg, grid, st);
     NSX_LAUNCH_CHECK("nsx_expert_combine_bwd");
     return NSX_OK;
 }
