@@ -792,9 +792,10 @@ static DwPlan dw_plan(int64_t R, int E, int n_in, int n_out) {
 //   16384 x 2 of 8,  2048 -> 2048   forward 319 | 298 | 310   dx 305 | 309 | 305   dW 355 | 336 | 293
 //    8192 x 2 of 16, 1024 -> 1024   forward  52 |  58 |  63   dx  54 |  57 |  62   dW  56 |  65 |  55
 //    2048 x 8 of 256, 2048 -> 1024  forward 257 | 243 |       dx 253 | 233     (64 x 64: 269, 276)
-// All bound by LDS: 256 x 128 tiles read and write 36 KB of it per 16 of q, 288 cycles beside the products' 256.  As time = f + q s the
-// forward of the first line has f = 36 us (its result's bytes alone 27), s = 133 us per 1024 of q, 1030 TFLOP/s.  256 x 256 tiles with
-// 4 waves of 128 x 128 (LDS 192) have a workgroup per CU, whose start and stores nothing covers: f = 59, the same s; with loads
+// As time = f + q s the forward of the first line has f = 36 us (its result's bytes alone 27), s = 133 us per 1024 of q, 1030 TFLOP/s.
+// Matrix units busy 37 % of the cycles, LDS 32 %; the rest is the chain of a step (its loads, two barriers, stores, first fragments)
+// that two workgroups per CU cover in part: without loads it takes 22 us less, without stores into LDS 30 less again.  256 x 256
+// tiles with 4 waves of 128 x 128 have one workgroup per CU, whose start and stores nothing covers: f = 59, the same s; with loads
 // straight into LDS each step waits for its memory (1.3 us after the issue at the earliest; the products take 1.2).
 // Where segments have a few rows the 64 x 64 tiles stay: 64 x 8 of 256, 1024 -> 2048: forward 150 | 167 (256 x 128), dx 145 | 149.
 static bool large_tiles(int64_t tiles128) { return tiles128 >= 6 * (int64_t)num_cus(); }
