@@ -869,3 +869,44 @@ def test_routed_network_rows_that_are_not_evaluated(cuda):
     assert empty.shape == (0, 5)
     (gp,) = torch.autograd.grad(empty.sum(), [net.params])
     assert (gp == 0).all()
+
+
+def test_graph_of_a_wide_step_replays(cuda):
+    """Wide layers behind a ReLU (dy masked in a pass of its own, chunks of large tiles) captured and replayed: the eager result."""
+    T, E, shape = 6000, 3, (1024, 520, 264)
+
+    def step(leaves, go):
+        leaves = [v.detach().requires_grad_(True) for v in leaves]
+        out = _mixture(*leaves, E, 2)
+        return [out.detach()] + list(torch.autograd.grad(out, leaves, go))
+    leaves, go = _mixture_inputs(T, E, *shape, 21, cuda)
+    static = [v.detach().clone() for v in leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static, go)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(static, go)
+    for turn in range(3):
+        new, _ = _mixture_inputs(T, E, *shape, 30 + turn, cuda)
+        for s, v in zip(static, new):
+            s.copy_(v.detach())
+        graph.replay()
+        want = step(static, go)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want)), turn
+
+
+def test_a_plan_changed_before_the_backward_pass_is_refused(cuda):
+    from nersemble_amd import experts as X
+    (x, logits, w1, w2), go = _mixture_inputs(40, 4, 32, 64, 16, 5, cuda)
+    weights, chosen = X.route_experts(logits.detach(), 2)
+    plan = X.expert_plan(chosen, 4)
+    h = X.expert_linear(x, w1, plan, relu=True)
+    out = X.expert_combine(X.expert_linear(h, w2, plan, gather=False), weights, plan)
+    torch.autograd.grad(out, [x, w1], go, retain_graph=True)
+    plan.rows.add_(0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(out, [x, w1], go)
