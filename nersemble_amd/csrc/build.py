@@ -11,6 +11,7 @@ ROOT = os.path.dirname(os.path.dirname(HERE))
 INCLUDE = os.path.join(ROOT, "include")
 OBJ = os.path.join(HERE, "_obj")
 SO = os.path.join(HERE, "libnsx.so")
+BINDING = os.path.join(HERE, "_experts.so")
 ARCH = "gfx950"
 
 
@@ -68,7 +69,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
             list(ex.map(run, jobs))
     if force or jobs or _stale(SO, objs):
         run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", SO, *objs])
+    src = os.path.join(HERE, "experts_torch.cpp")
+    if force or _stale(BINDING, [src, os.path.join(INCLUDE, "nsx.h"), __file__]):
+        run(_binding(src))
     return SO
+
+
+def _binding(src):
+    """The one source that sees torch's headers: host code only, calls libnsx.so beside it."""
+    import sysconfig
+    import torch
+    root = os.path.join(os.path.dirname(torch.__file__))
+    inc = os.path.join(root, "include")
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE, "-I", inc,
+            "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"], "-I", "/opt/rocm/include",
+            src, "-o", BINDING, "-L", os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-ltorch_python",
+            "-L", HERE, "-lnsx", "-Wl,-rpath,$ORIGIN"]
 
 
 if __name__ == "__main__":

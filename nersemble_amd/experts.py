@@ -21,8 +21,6 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._lib import check, lib, ndev, ptr
 
-# (What is small here runs on the host in the time of one such call -- 10 to 40 us -- so the wrappers below read every tensor
-# property once, hand plain integers to the library and take the fast way where nothing has to be copied.)
 _DTYPE = {torch.float32: _lib.NSX_DTYPE_F32, torch.float16: _lib.NSX_DTYPE_F16, torch.bfloat16: _lib.NSX_DTYPE_BF16}
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _F32, _I32 = torch.float32, torch.int32
@@ -45,6 +43,26 @@ _native = _NotLoaded()
 
 def _libnsx():
     return lib() if _profiler.enabled else _native
+
+
+class _FastNotLoaded:
+    """csrc/experts_torch.cpp before its first call."""
+
+    def __getattr__(self, name):
+        global _fast
+        lib()
+        try:
+            from .csrc import _experts
+        except ImportError as e:
+            raise RuntimeError(f"nersemble_amd: the native binding csrc/_experts.so cannot be loaded ({e}). Build it with "
+                               f"`python -c 'import __graft_entry__ as g; g.build()'`.") from e
+        _fast = _experts
+        return getattr(_fast, name)
+
+
+# The calls whose arguments are plain (contiguous rows on the current device, no row count on the device, nobody profiling) run
+# natively from end to end; every other goes through the Functions below, which copy, refuse and record what there is.
+_fast = _FastNotLoaded()
 
 
 class ExpertPlan:
@@ -176,9 +194,16 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
     the chosen scores over their sum; times ``scale``.  A logit of -inf takes the expert out for its row.  ``selector`` uint8
     [T]: rows with 0 are not routed.  Where there is no expert to choose: chosen -1, weight 0.  A row with a NaN logit has NaN
     weights."""
+    sigmoid = _SCORES.get(scores)
+    groups = n_groups if top_groups is None else top_groups
+    if sigmoid is not None and _lib._COUNT_SCOPE is None and not _profiler.enabled:
+        out = _fast.route_experts(logits, int(top_k), sigmoid, bias, selector, int(n_groups), int(groups), int(group_top),
+                                  int(bool(renormalise)), float(scale))
+        if out is not None:
+            return out
     if logits.dim() != 2 or logits.dtype not in _DTYPE:
         raise RuntimeError(f"route_experts: logits are [T, E] in fp32, fp16 or bf16 (got {tuple(logits.shape)} {logits.dtype})")
-    if scores not in _SCORES:
+    if sigmoid is None:
         raise RuntimeError(f"route_experts: scores are 'softmax' or 'sigmoid' (got {scores!r})")
     T, E = logits.shape
     if bias is not None:
@@ -194,8 +219,7 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
             selector = selector.view(torch.uint8)
         if selector.dtype != torch.uint8:
             raise RuntimeError(f"route_experts: selector is uint8 or bool (got {selector.dtype})")
-    cfg = (int(top_k), _SCORES[scores], int(n_groups), int(n_groups if top_groups is None else top_groups), int(group_top),
-           int(bool(renormalise)), float(scale))
+    cfg = (int(top_k), sigmoid, int(n_groups), int(groups), int(group_top), int(bool(renormalise)), float(scale))
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteFn.apply(logits, bias, selector, cfg)
     x, stride = _rows_of(logits, 1)
@@ -216,6 +240,14 @@ def _plan_bytes(n_entries, n_experts):
 def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
     """The plan of ``chosen`` [T, top_k] int32 (``route_experts``): a stable sort of its entries by expert.  Entries outside
     [0, n_experts) are not routed."""
+    if _lib._COUNT_SCOPE is None and not _profiler.enabled:
+        out = _fast.plan(chosen, int(n_experts))
+        if out is not None:
+            plan = ExpertPlan.__new__(ExpertPlan)
+            plan.offsets, plan.rows, plan.positions = out
+            plan.n_rows, plan.top_k = chosen.shape
+            plan.n_experts, plan.n_entries, plan.device = int(n_experts), plan.n_rows * plan.top_k, chosen.get_device()
+            return plan
     if chosen.dim() != 2 or chosen.dtype != torch.int32:
         raise RuntimeError(f"expert_plan: chosen is [T, top_k] int32 (got {tuple(chosen.shape)} {chosen.dtype})")
     chosen = chosen.contiguous()
@@ -231,11 +263,7 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
                                    None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
     if rc:
         check(rc, "nsx_expert_plan")
-    plan = ExpertPlan.__new__(ExpertPlan)
-    plan.offsets, plan.rows = buf.as_strided((n_experts + 1,), (1,), 0), buf.as_strided((T * k,), (1,), o)
-    plan.positions = buf.as_strided((T, k), (k, 1), o + r)
-    plan.n_experts, plan.n_entries, plan.n_rows, plan.top_k, plan.device = n_experts, T * k, T, k, dev
-    return plan
+    return ExpertPlan(buf[:n_experts + 1], buf[o:o + T * k], buf[o + r:o + r + T * k].view(T, k))
 
 
 # ------------------------------------------------------------------------------------------------
@@ -315,6 +343,10 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gathe
     x: fp16 or bf16, [T, n_in] rows (``gather``) or [T * top_k, n_in] in the plan's order.  weight [E, n_out, n_in]: of x's
     dtype, or fp32 parameters whose copy in x's dtype is ``w16`` (made here if it is not given); the gradient has the dtype of
     ``weight``.  n_in and n_out are multiples of 8."""
+    if _lib._COUNT_SCOPE is None and not _profiler.enabled:
+        out = _fast.expert_linear(x, weight, w16, plan.offsets, plan.rows, plan.positions, bool(gather), bool(relu))
+        if out is not None:
+            return out
     xs, ws, xt, wt = x.shape, weight.shape, x.dtype, weight.dtype
     if len(xs) != 2 or xt not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"expert_linear: x is [rows, n_in] in fp16 or bf16 (got {tuple(xs)} {xt})")
@@ -397,6 +429,10 @@ _combine_bwd_once = once_differentiable(_combine_bwd)
 def expert_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """[T, n]: sum over a row's choices of ``weights[t, j] * y[plan.positions[t, j]]``, differentiable w.r.t. ``y`` [T * top_k,
     n] (fp16 or bf16, n a multiple of 8) and ``weights`` [T, top_k]; choices that are not routed count nothing."""
+    if _lib._COUNT_SCOPE is None and not _profiler.enabled:
+        out = _fast.expert_combine(y, weights, plan.offsets, plan.rows, plan.positions)
+        if out is not None:
+            return out
     ys = y.shape
     if len(ys) != 2 or ys[0] != plan.n_entries or y.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"expert_combine: y is [{plan.n_entries}, n] in fp16 or bf16 (got {tuple(ys)} {y.dtype})")

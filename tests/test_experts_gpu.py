@@ -11,6 +11,18 @@ from oracle import experts as ox
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True, params=["native", "functions"])
+def way(request, monkeypatch):
+    """Every test runs both ways through the host: the native nodes that plain arguments take, and the Functions for all others."""
+    from nersemble_amd import experts as X
+    if request.param == "functions":
+        class Never:
+            def __getattr__(self, name):
+                return lambda *args: None
+        monkeypatch.setattr(X, "_fast", Never())
+    return request.param
+
 U = 2.0 ** -24
 HALF = {torch.float16: (2.0 ** -11, 2.0 ** -25), torch.bfloat16: (2.0 ** -8, 2.0 ** -130)}
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
@@ -908,5 +920,38 @@ def test_a_plan_changed_before_the_backward_pass_is_refused(cuda):
     out = X.expert_combine(X.expert_linear(h, w2, plan, gather=False), weights, plan)
     torch.autograd.grad(out, [x, w1], go, retain_graph=True)
     plan.rows.add_(0)
-    with pytest.raises(RuntimeError, match="inplace"):
+    with pytest.raises(RuntimeError, match="inplace operation"):
         torch.autograd.grad(out, [x, w1], go)
+
+
+def test_plain_arguments_run_natively(cuda, way, monkeypatch):
+    """The native nodes are what runs where nothing stands against it; a row count on the device, a profiler or another layout do."""
+    from nersemble_amd import _lib
+    from nersemble_amd import experts as X
+    called = []
+    if way != "native":
+        return
+    X.expert_plan(torch.zeros((1, 1), dtype=torch.int32, device=cuda), 1)          # (loads it)
+    native = X._fast
+
+    class Watch:
+        def __getattr__(self, name):
+            def call(*args):
+                out = getattr(native, name)(*args)
+                called.append((name, out is not None))
+                return out
+            return call
+    monkeypatch.setattr(X, "_fast", Watch())
+    (x, logits, w1, w2), go = _mixture_inputs(50, 4, 32, 64, 16, 5, cuda)
+    out = _mixture(x, logits, w1, w2, 4, 2)
+    assert called == [("route_experts", True), ("plan", True), ("expert_linear", True), ("expert_linear", True), ("expert_combine", True)]
+    want = torch.autograd.grad(out, [x, logits, w1, w2], go)
+    called.clear()
+    strided = torch.randn((50, 48), device=cuda).half()[:, 8:40]
+    X.expert_linear(strided, w1, X.expert_plan(torch.zeros((50, 1), dtype=torch.int32, device=cuda), 4))
+    assert called == [("plan", True), ("expert_linear", False)]
+    called.clear()
+    with _lib.device_count(torch.tensor([50], device=cuda), 50):
+        again = _mixture(x, logits, w1, w2, 4, 2)
+        got = torch.autograd.grad(again, [x, logits, w1, w2], go)
+    assert not called and torch.equal(again, out) and all(torch.equal(a, b) for a, b in zip(got, want))
