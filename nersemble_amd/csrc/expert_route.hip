@@ -9,15 +9,16 @@
 //     compared as they are and no score is formed for experts that are not chosen.
 //   * Otherwise the choice is that of c in 64 bits: two experts whose 32-bit sums round to the same value, or change places,
 //     would make it depend on the order of the summation behind the softmax.  c is formed in 32 bits; only where neighbours in
-//     the order lie closer than its error is the wave's part done again in 64.
+//     the order lie closer than its error are they compared in 64.
 //   * Renormalised weights are ratios: of the softmax only exp(x_j - max over the chosen) is left, of the sigmoid
 //     exp(x_j - min(max, 0)) / (1 + exp(x_j)) -- neither underflows where all chosen scores are tiny.
 // A row is held by L lanes of a wave, V consecutive experts in each (64 / L rows per wave): a row is read once, 16 or 32 bytes
 // per lane.  A round of "largest value, lowest index" is log2(L) exchanges of the value within the lanes (DPP), a ballot of the
 // lanes that hold it, and the first of them takes its expert out.  The entries lie in LDS, a lane each computes their weights.
 // Bound by memory where few are chosen: 2^20 x 32 fp32, top 2: 32 us (151 MB, 4.7 TB/s; a copy reaches 4.96).  By the rounds'
-// instructions where many are: 65536 x 256 bf16, top 8: 25 us (38 MB, 1.5 TB/s); with a bias 62 us in fp32, and 30011 rows of 8
-// groups 34 us, of which 10 are one wave that does its rows again in 64 bits at the end.
+// instructions where many are: 65536 x 256 bf16, top 8: 25 us (38 MB, 1.5 TB/s); with a bias 55 us in fp32; 30011 rows of 8 groups
+// 27 us.  (With all experts of a wave in 64 bits wherever two entries were close these two took 62 and 35: the few waves that do
+// it end last.)
 #include "expert_common.h"
 #include <algorithm>
 
@@ -98,13 +99,13 @@ template <> struct Order<double> {
     static __device__ __forceinline__ double none() { return -INFINITY; }
 };
 
-// One pass of the choice over the wave's rows: `rounds` entries of `out` per row, c of the chosen becomes none.
+// Rounds first .. end of the choice over the wave's rows: an entry of `out` per row each, c of the chosen becomes none.
 template <typename K> struct Chosen { K c; int32_t e; };
 template <typename K, int V>
-__device__ __forceinline__ void choose(const RouteArgs& a, typename Order<K>::type (&c)[V], int e0, int r, int sub, int rounds, Chosen<K>* __restrict__ out) {
+__device__ __forceinline__ void choose(const RouteArgs& a, typename Order<K>::type (&c)[V], int e0, int r, int sub, int first, int end, Chosen<K>* __restrict__ out) {
     typedef Order<K> O;
     const int L = 1 << a.lg_L;
-    for (int j = 0; j < rounds; ++j) {
+    for (int j = first; j < end; ++j) {
         auto best = c[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) best = c[i] > best ? c[i] : best;
@@ -166,8 +167,8 @@ __device__ __forceinline__ K keep_groups(const RouteArgs& a, typename Order<K>::
 // 3e-6 relatively.  Adding the bias rounds once more.
 __device__ __forceinline__ float unsure(float v, int sigmoid) { return (sigmoid ? 1e-6f : 8e-6f) + 2.5e-7f * fabsf(v); }
 
-// SCORES: the choice goes by scores (32 bits first; rows in which neighbours of the choice lie closer than `unsure` are done
-// again in 64 bits), else by the logits themselves.
+// SCORES: the choice goes by scores, else by the logits themselves.  32 bits first; where neighbours of the choice lie closer than
+// `unsure`, the chosen and the one that just missed are compared in 64 bits, where more may have taken part all experts of the rows.
 template <typename T, int V, bool VEC, bool SCORES>
 __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArgs a) {
     extern __shared__ __attribute__((aligned(16))) char route_lds[];
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
     for (int i = 0; i < V; ++i) odd |= (x[i] != x[i]) || (!a.sigmoid && x[i] == INFINITY);
     const bool bad = row_lanes(__ballot(odd), r, a.lg_L) != 0;
 
-    const int slots = a.k + (SCORES ? 1 : 0);
+    const int slots = a.k + (SCORES ? 2 : 0);
     char* mine = route_lds + (size_t)(wave * rpw + r) * slots * (SCORES ? sizeof(Chosen<double>) : sizeof(Chosen<float>));
     Chosen<float>* out = reinterpret_cast<Chosen<float>*>(mine);
     float xmax = 0.f, Z = 1.f;                                 // softmax over the whole row, where it is asked for
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
         for (int i = 0; i < V; ++i) c[i] = bad ? Order<float>::none() : Order<float>::of(x[i]);
         float lowest;
         if (a.top_groups < a.G) keep_groups<float>(a, c, r, g, lowest);
-        choose<float>(a, c, e0, r, sub, a.k, out);
+        choose<float>(a, c, e0, r, sub, 0, a.k, out);
     } else {
         float bias[V];
 #pragma unroll
@@ -228,12 +229,13 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
             const float v = s + bias[i];
             c[i] = (!bad && x[i] > -INFINITY && v == v) ? Order<float>::of(v) : Order<float>::none();
         }
+        bool whole = false;                                    // the groups that stay, or more than one expert behind the choice, are in doubt
         if (a.top_groups < a.G) {
             float lowest;
-            const float gap = keep_groups<float>(a, c, r, g, lowest);                      // (of sums of up to two)
-            again = !(gap > 2.f * unsure(lowest, a.sigmoid)) && !bad;
+            const float gap = keep_groups<float>(a, c, r, g, lowest);                // (of sums of up to two)
+            whole = !(gap > 2.f * unsure(lowest, a.sigmoid)) && !bad;
         }
-        choose<float>(a, c, e0, r, sub, a.k + 1, out);
+        choose<float>(a, c, e0, r, sub, 0, a.k + 1, out);
         for (int j = sub; j < a.k; j += L) {
             const Chosen<float> p = out[j], q = out[j + 1];
             // (equal logits and biases are equal in 64 bits as well -- unless a third that is not may come between the last
@@ -242,32 +244,65 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
                 again |= j == a.k - 1 || !((float)row[p.e] == (float)row[q.e] && (!a.bias || a.bias[p.e] == a.bias[q.e]));
         }
         wave_lds_fence();
-        if (__ballot(again && on) != 0) {
-            Chosen<double>* wide = reinterpret_cast<Chosen<double>*>(mine);
+        if (__ballot((again || whole) && on) != 0) {
+            choose<float>(a, c, e0, r, sub, a.k + 1, a.k + 2, out);
+            const Chosen<float> last = out[a.k - 1], third = out[a.k + 1];
+            whole |= third.e >= 0 && !(last.c - third.c > unsure(last.c, a.sigmoid));
+            const bool all = __ballot(whole && on) != 0;
             double d[V], m = -INFINITY, z = 0.0;
-            if (!a.sigmoid) {
+            if (all || !a.sigmoid) {
+                if (!a.sigmoid) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) m = fmax(m, (double)x[i]);
-                m = row_all<TakeMax>(m, L);
-            }
+                    for (int i = 0; i < V; ++i) m = fmax(m, (double)x[i]);
+                    m = row_all<TakeMax>(m, L);
+                }
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double xi = (double)x[i];
-                d[i] = !(x[i] > -INFINITY) ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-xi)) : exp(xi - m);
-                z += d[i];
+                for (int i = 0; i < V; ++i) {
+                    const double xi = (double)x[i];
+                    d[i] = !(x[i] > -INFINITY) ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-xi)) : exp(xi - m);
+                    z += d[i];
+                }
+                if (!a.sigmoid) z = row_all<TakeSum>(z, L);
             }
-            if (!a.sigmoid) z = row_all<TakeSum>(z, L);
+            if (all) {
+                Chosen<double>* wide = reinterpret_cast<Chosen<double>*>(mine);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double v = (a.sigmoid ? d[i] : d[i] / z) + (double)bias[i];
-                d[i] = (!bad && x[i] > -INFINITY && v == v) ? v : -INFINITY;
+                for (int i = 0; i < V; ++i) {
+                    const double v = (a.sigmoid ? d[i] : d[i] / z) + (double)bias[i];
+                    d[i] = (!bad && x[i] > -INFINITY && v == v) ? v : -INFINITY;
+                }
+                double lowest;
+                if (a.top_groups < a.G) keep_groups<double>(a, d, r, g, lowest);
+                choose<double>(a, d, e0, r, sub, 0, a.k, wide);
+                // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from)
+                if (sub == 0)
+                    for (int j = 0; j < a.k; ++j) { const Chosen<double> w = wide[j]; out[j] = Chosen<float>{(float)w.c, w.e}; }
+            } else {
+                // The k + 1 candidates in 64 bits, an entry to a lane, then by their rank.
+                double* v = reinterpret_cast<double*>(mine + slots * sizeof(Chosen<float>));
+                int32_t* sorted = reinterpret_cast<int32_t*>(v);
+                for (int j = sub; j <= a.k; j += L) {
+                    const int e = out[j].e;
+                    const double xe = e >= 0 ? (double)(float)row[e] : 0.0;
+                    v[j] = e < 0 ? -INFINITY : (a.sigmoid ? 1.0 / (1.0 + exp(-xe)) : exp(xe - m) / z) + (a.bias ? (double)a.bias[e] : 0.0);
+                }
+                wave_lds_fence();
+                for (int j = sub; j <= a.k; j += L) {
+                    const int e = out[j].e;
+                    const double own = v[j];
+                    int rank = 0;
+                    for (int i = 0; i <= a.k; ++i) {
+                        const int f = out[i].e;
+                        const double other = v[i];
+                        rank += other > own || (other == own && (f < 0 || e < 0 ? i < j : f < e)) ? 1 : 0;
+                    }
+                    out[j].c = __builtin_bit_cast(float, rank);
+                }
+                wave_lds_fence();
+                for (int j = sub; j <= a.k; j += L) sorted[__builtin_bit_cast(int, out[j].c)] = out[j].e;
+                wave_lds_fence();
+                for (int j = sub; j < a.k; j += L) out[j].e = sorted[j];
             }
-            double lowest;
-            if (a.top_groups < a.G) keep_groups<double>(a, d, r, g, lowest);
-            choose<double>(a, d, e0, r, sub, a.k, wide);
-            // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from)
-            if (sub == 0)
-                for (int j = 0; j < a.k; ++j) { const Chosen<double> w = wide[j]; out[j] = Chosen<float>{(float)w.c, w.e}; }
             wave_lds_fence();
         }
     }
@@ -569,7 +604,7 @@ template <typename T, int V>
 static void launch_route(const RouteArgs& a, bool by_scores, bool vec, hipStream_t st) {
     const int rpw = kWave >> a.lg_L;
     const unsigned blocks = (unsigned)((a.T + (int64_t)rpw * ROUTE_WAVES - 1) / ((int64_t)rpw * ROUTE_WAVES));
-    const size_t lds = (size_t)ROUTE_WAVES * rpw * (by_scores ? (a.k + 1) * sizeof(Chosen<double>) : a.k * sizeof(Chosen<float>));
+    const size_t lds = (size_t)ROUTE_WAVES * rpw * (by_scores ? (a.k + 2) * sizeof(Chosen<double>) : a.k * sizeof(Chosen<float>));
     if (by_scores) {
         if (vec) route_fwd_kernel<T, V, true, true><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
         else route_fwd_kernel<T, V, false, true><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
@@ -627,7 +662,7 @@ int nsx_expert_route_fwd(const void* logits, int dtype, int64_t T, int E, int64_
                 weights, experts, n_device, 0, 0, fast_div(top_k)};
     // Values per lane: 16 leave the fewest exchanges and instructions per row, 4 the shortest chain where few waves hide it.  us with
     // 4 | 8 | 16 (groups: 8 with a bias, the best 2 of each counting, 4 of them stay):
-    //   2^20 x 32 fp32 top 2      62 | 38 | 32     16384 x 64 fp32 top 6           6.0 |  5.5 |  6.8    30011 x 256 bf16 top 8, groups  50 | 35 | 34
+    //   2^20 x 32 fp32 top 2      62 | 38 | 32     16384 x 64 fp32 top 6           6.0 |  5.5 |  6.8    30011 x 256 bf16 top 8, groups  48 | 31 | 27
     //   65536 x 256 bf16 top 8    58 | 35 | 25      4096 x 64 fp32 top 6           4.5 |  5.0 |  6.7     2^20 x 8 fp16 top 2            17 | 13 | 13
     //   2^18 x 64 fp32 top 6      46 | 33 | 30      4096 x 256 bf16 top 8, groups 14.7 | 15.7 | 20.2     1 x 64 fp32 top 6             4.5 | 4.3 | 5.7
     int V = T * E <= 1 << 19 ? 4 : T * E <= 1 << 22 || Eg < 32 ? 8 : 16;

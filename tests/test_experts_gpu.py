@@ -955,3 +955,36 @@ def test_plain_arguments_run_natively(cuda, way, monkeypatch):
         again = _mixture(x, logits, w1, w2, 4, 2)
         got = torch.autograd.grad(again, [x, logits, w1, w2], go)
     assert not called and torch.equal(again, out) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("E,k,G,tg,gt", [(64, 6, 1, 1, 1), (61, 8, 1, 1, 1), (256, 8, 8, 4, 2), (64, 64, 1, 1, 1), (9, 9, 1, 1, 1), (20, 1, 4, 2, 1)])
+@pytest.mark.parametrize("sc", ["sigmoid", "softmax"])
+def test_route_pairs_that_32_bits_do_not_tell(E, k, G, tg, gt, sc, cuda):
+    """Rows with one pair of sums a few 1e-9 apart, anywhere in the order: the choice is that of 64 bits."""
+    from nersemble_amd import experts as X
+    rng = np.random.default_rng(E + k)
+    T = 400
+    bias = (rng.standard_normal(E) * 0.1).astype(np.float32)
+    x = (rng.standard_normal((T, E)) * 1.5).astype(np.float32)
+    sig = sc == "sigmoid"
+    for t in range(T):
+        s = ox.scores(x[t:t + 1], sig)[0] + bias
+        order = np.argsort(-s)
+        a, b = order[t % min(E - 1, k + 1)], order[t % min(E - 1, k + 1) + 1]
+        if sig:                                                              # the logit that puts b beside a
+            p = s[a] - bias[b]
+            if 0 < p < 1:
+                x[t, b] = np.log(p / (1 - p))
+        else:
+            e, delta = np.exp(x[t].astype(np.float64)), np.float64(bias[a]) - np.float64(bias[b])
+            eb = (e[a] + delta * (e.sum() - e[b])) / (1 - delta)
+            if eb > 0:
+                x[t, b] = np.log(eb)
+    s = ox.scores(x, sig) + bias
+    gaps = np.diff(np.sort(s, axis=1), axis=1)
+    assert ((gaps > 0) & (gaps < 1e-7)).any(1).mean() > 0.2                  # (there are such pairs)
+    clear = ~((gaps > 0) & (gaps < 1e-13)).any(1)
+    w, c = X.route_experts(torch.from_numpy(x).to(cuda), k, scores=sc, bias=torch.from_numpy(bias).to(cuda), n_groups=G, top_groups=tg, group_top=gt)
+    ww, wc = ox.route(x, k, sig, bias, G, tg, gt)
+    assert clear.mean() > 0.9 and np.array_equal(c.cpu().numpy()[clear], wc[clear])
+    _close(w.cpu()[clear], ww[clear], _route_tol(x, ww, k)[clear], "weights")
