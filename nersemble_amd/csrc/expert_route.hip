@@ -434,8 +434,8 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a, const float
 // them; what a wave counts in order lands in order, so equal inputs give equal plans.  A first launch counts every block's entries
 // per expert; in the second a block knows from all counts where its own begin, and places them 64 at a time: lanes of one expert
 // find each other by ballots of the expert's bits.
-// Bound by the chain of steps: 2^20 rows x 2 of 16 experts, 25 MB: 18 us, 1.4 TB/s (a copy would take 5); 4096 x 2: 8 us, of which
-// one launch is 3.  8 entries per lane are loaded ahead; one at a time took 111 us.
+// Bound by the chain of steps: 2^20 rows x 2 of 16 experts, 25 MB: 16.6 us, 1.5 TB/s (a copy would take 5); 4096 x 2: 7.7 us, of
+// which one launch is 3.  8 entries per lane are loaded ahead; one at a time took 111 us.
 constexpr int PLAN_MAX_BLOCKS = 256;
 constexpr int PLAN_LANE = 8, PLAN_PIECE = PLAN_LANE * kWave;      // entries that a lane, a wave loads at a time
 
@@ -486,8 +486,7 @@ __global__ __launch_bounds__(WAVES * kWave) void plan_place_kernel(const int32_t
     __shared__ int32_t routed;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blocks = gridDim.x;
     const int end = plan_end(n, k, n_dev);
-    for (int w = 0; w < WAVES; ++w)
-        for (int e = threadIdx.x; e < E; e += PLAN_THREADS) cursor[w][e] = 0;
+    for (int x = lane; x < E; x += kWave) cursor[wave][x] = 0;
     __syncthreads();
     const int a0 = blockIdx.x * per_block, b0 = min(a0 + per_block, n), part = per_block / WAVES;
     const int a = min(a0 + wave * part, b0), b = min(a + part, b0), live = min(b, end);
@@ -516,8 +515,10 @@ __global__ __launch_bounds__(WAVES * kWave) void plan_place_kernel(const int32_t
     for (int x = threadIdx.x; x < E; x += PLAN_THREADS) {
         int sum = 0, before = 0;
         if (blocks > 1) {
+#pragma unroll 4
             for (int h = x; h < PLAN_THREADS; h += 1 << bits) { sum += part_all[h]; before += part_before[h]; }
         } else {
+#pragma unroll
             for (int w = 0; w < WAVES; ++w) sum += cursor[w][x];
         }
         all[x] = sum;
@@ -548,8 +549,11 @@ __global__ __launch_bounds__(WAVES * kWave) void plan_place_kernel(const int32_t
     }
     __syncthreads();
     for (int x = threadIdx.x; x < E; x += PLAN_THREADS) {
-        int p = first[x];
-        for (int w = 0; w < WAVES; ++w) { const int v = cursor[w][x]; cursor[w][x] = p; p += v; }
+        int p = first[x], v[WAVES];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v[w] = cursor[w][x];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) { cursor[w][x] = p; p += v[w]; }
     }
     __syncthreads();
     const bool kept = b - a <= PLAN_PIECE;                        // (the entries are still in registers)
