@@ -12,7 +12,6 @@ the host and can be captured into a graph.  Under
 ``_lib.device_count`` rows behind the device-side count are not routed, and not written by ``route_experts`` and
 ``expert_combine``.  A plan's numbers are bounded inside the kernels; equal inputs give equal bits.
 """
-from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -26,23 +25,6 @@ _SCORES = {"softmax": 0, "sigmoid": 1}
 _F32, _I32 = torch.float32, torch.int32
 _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _profiler = _lib.profiler
-
-
-class _NotLoaded:
-    """The library before its first call (``_lib.lib`` says so where it is missing)."""
-
-    def __getattr__(self, name):
-        global _native
-        lib()
-        _native = _lib._lib._h
-        return getattr(_native, name)
-
-
-_native = _NotLoaded()
-
-
-def _libnsx():
-    return lib() if _profiler.enabled else _native
 
 
 class _FastNotLoaded:
@@ -70,7 +52,10 @@ class ExpertPlan:
 
     offsets [E + 1]: the ordered rows of expert e are offsets[e] .. offsets[e + 1]; rows [T * top_k]: entry of every ordered
     row, -1 behind the last segment; positions [T, top_k]: ordered row of every entry, -1 for an entry that is not routed."""
-    __slots__ = ("offsets", "rows", "positions", "n_experts", "n_rows", "top_k", "n_entries", "device")
+    __slots__ = ("_offsets", "_rows", "_positions", "n_experts", "n_rows", "top_k", "n_entries", "device")
+    offsets = property(lambda self: self._offsets)
+    rows = property(lambda self: self._rows)
+    positions = property(lambda self: self._positions)
 
     def __init__(self, offsets: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor):
         o, r, p = offsets.shape, rows.shape, positions.shape
@@ -83,7 +68,7 @@ class ExpertPlan:
             raise RuntimeError(f"ExpertPlan: offsets, rows and positions are on {offsets.device}, {rows.device} and {positions.device}")
         if not (offsets.is_contiguous() and rows.is_contiguous() and positions.is_contiguous()):
             offsets, rows, positions = offsets.contiguous(), rows.contiguous(), positions.contiguous()
-        self.offsets, self.rows, self.positions = offsets, rows, positions
+        self._offsets, self._rows, self._positions = offsets, rows, positions
         self.n_experts, self.n_entries = o[0] - 1, r[0]
         self.n_rows, self.top_k = p
 
@@ -136,7 +121,7 @@ def _route(x, stride, bias, selector, top_k, sigmoid, n_groups, top_groups, grou
     dev = _here(x)
     weights = x.new_empty((T, top_k), dtype=_F32)
     chosen = x.new_empty((T, top_k), dtype=_I32)
-    rc = _libnsx().nsx_expert_route_fwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, None if bias is None else _at(bias, dev),
+    rc = lib().nsx_expert_route_fwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, None if bias is None else _at(bias, dev),
                                     None if selector is None else _at(selector, dev), top_k, sigmoid, n_groups, top_groups, group_top,
                                     renorm, scale, weights.data_ptr(), chosen.data_ptr(),
                                     None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
@@ -155,7 +140,7 @@ def _route_bwd(ctx, g, _):
         g = g.to(_F32).contiguous()
     dev = x.get_device()
     d = torch.empty_like(x) if stride == E else x.new_empty((T, E))
-    rc = _libnsx().nsx_expert_route_bwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, top_k, sigmoid, renorm, scale, weights.data_ptr(),
+    rc = lib().nsx_expert_route_bwd(x.data_ptr(), _DTYPE[x.dtype], T, E, stride, top_k, sigmoid, renorm, scale, weights.data_ptr(),
                                     chosen.data_ptr(), g.data_ptr(), d.data_ptr(),
                                     None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
     if rc:
@@ -229,7 +214,6 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
 # ------------------------------------------------------------------------------------------------
 # plan
 # ------------------------------------------------------------------------------------------------
-@lru_cache(maxsize=1024)
 def _plan_bytes(n_entries, n_experts):
     n = lib().nsx_expert_plan_workspace(n_entries, n_experts)
     if n < 0:
@@ -244,7 +228,7 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
         out = _fast.plan(chosen, int(n_experts))
         if out is not None:
             plan = ExpertPlan.__new__(ExpertPlan)
-            plan.offsets, plan.rows, plan.positions = out
+            plan._offsets, plan._rows, plan._positions = out
             plan.n_rows, plan.top_k = chosen.shape
             plan.n_experts, plan.n_entries, plan.device = int(n_experts), plan.n_rows * plan.top_k, chosen.get_device()
             return plan
@@ -259,7 +243,7 @@ def expert_plan(chosen: torch.Tensor, n_experts: int) -> ExpertPlan:
     dev = _here(chosen)
     buf = chosen.new_empty((o + 2 * r + need // 4,))
     base = buf.data_ptr()
-    rc = _libnsx().nsx_expert_plan(chosen.data_ptr(), T, k, n_experts, base, base + 4 * o, base + 4 * (o + r), base + 4 * (o + 2 * r),
+    rc = lib().nsx_expert_plan(chosen.data_ptr(), T, k, n_experts, base, base + 4 * o, base + 4 * (o + r), base + 4 * (o + 2 * r),
                                    None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
     if rc:
         check(rc, "nsx_expert_plan")
@@ -276,7 +260,7 @@ def _linear(x, x_stride, w16, plan, gather, relu):
         ptr(w16), ptr(plan.offsets)
     n = plan.n_entries
     y = x.new_empty((n, N))
-    rc = _libnsx().nsx_expert_linear_fwd(x.data_ptr(), _DTYPE[x.dtype], x_stride, x.shape[0], plan.rows.data_ptr() if gather else None,
+    rc = lib().nsx_expert_linear_fwd(x.data_ptr(), _DTYPE[x.dtype], x_stride, x.shape[0], plan.rows.data_ptr() if gather else None,
                                      plan.top_k, w16.data_ptr(), K, N, E, plan.offsets.data_ptr(), n, relu, y.data_ptr(),
                                      _raw_stream(dev))
     if rc:
@@ -284,7 +268,6 @@ def _linear(x, x_stride, w16, plan, gather, relu):
     return y
 
 
-@lru_cache(maxsize=1024)
 def _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w, masked):
     n = lib().nsx_expert_linear_bwd_workspace(R, E, K, N, need_x, gather, need_w, masked)
     if n < 0:
@@ -306,7 +289,7 @@ def _linear_bwd(ctx, dy):
     ws = g.new_empty((need // 2,)) if need else None
     dx = g.new_empty((x_rows, K)) if need_x else None
     dw = None if not need_w else g.new_empty((E, N, K)) if w_dtype == g.dtype else g.new_empty((E, N, K), dtype=w_dtype)
-    rc = _libnsx().nsx_expert_linear_bwd(
+    rc = lib().nsx_expert_linear_bwd(
         x.data_ptr() if need_w else None, _DTYPE[g.dtype], x_stride, x_rows, plan.rows.data_ptr() if gather else None,
         plan.positions.data_ptr(), plan.top_k, w16.data_ptr() if need_x else None, g.data_ptr(), g_stride,
         None if y is None else y.data_ptr(), N, K, N, E, plan.offsets.data_ptr(), R, dx.data_ptr() if need_x else None,
@@ -344,7 +327,7 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gathe
     dtype, or fp32 parameters whose copy in x's dtype is ``w16`` (made here if it is not given); the gradient has the dtype of
     ``weight``.  n_in and n_out are multiples of 8."""
     if _lib._COUNT_SCOPE is None and not _profiler.enabled:
-        out = _fast.expert_linear(x, weight, w16, plan.offsets, plan.rows, plan.positions, bool(gather), bool(relu))
+        out = _fast.expert_linear(x, weight, w16, plan._offsets, plan._rows, plan._positions, bool(gather), bool(relu))
         if out is not None:
             return out
     xs, ws, xt, wt = x.shape, weight.shape, x.dtype, weight.dtype
@@ -380,7 +363,7 @@ def _combine(y, y_stride, weights, plan):
     if weights.get_device() != dev or plan.device != dev:
         ptr(weights), ptr(plan.positions)
     out = y.new_empty((T, n))
-    rc = _libnsx().nsx_expert_combine_fwd(y.data_ptr(), _DTYPE[y.dtype], y_stride, R, n, weights.data_ptr(), plan.positions.data_ptr(), T,
+    rc = lib().nsx_expert_combine_fwd(y.data_ptr(), _DTYPE[y.dtype], y_stride, R, n, weights.data_ptr(), plan.positions.data_ptr(), T,
                                       plan.top_k, out.data_ptr(), None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
     if rc:
         check(rc, "nsx_expert_combine_fwd")
@@ -400,7 +383,7 @@ def _combine_bwd(ctx, dout):
     dev = y.get_device()
     dy = torch.empty_like(y) if stride == n else y.new_empty((R, n))
     dw = torch.empty_like(w)
-    rc = _libnsx().nsx_expert_combine_bwd(y.data_ptr(), _DTYPE[y.dtype], stride, R, n, w.data_ptr(), plan.positions.data_ptr(),
+    rc = lib().nsx_expert_combine_bwd(y.data_ptr(), _DTYPE[y.dtype], stride, R, n, w.data_ptr(), plan.positions.data_ptr(),
                                       plan.offsets.data_ptr() + 4 * plan.n_experts, T, k, dout.data_ptr(), dy.data_ptr(),
                                       dw.data_ptr(), None if _lib._COUNT_SCOPE is None else ndev(T), _raw_stream(dev))
     if rc:
@@ -430,7 +413,7 @@ def expert_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) -> 
     """[T, n]: sum over a row's choices of ``weights[t, j] * y[plan.positions[t, j]]``, differentiable w.r.t. ``y`` [T * top_k,
     n] (fp16 or bf16, n a multiple of 8) and ``weights`` [T, top_k]; choices that are not routed count nothing."""
     if _lib._COUNT_SCOPE is None and not _profiler.enabled:
-        out = _fast.expert_combine(y, weights, plan.offsets, plan.rows, plan.positions)
+        out = _fast.expert_combine(y, weights, plan._offsets, plan._rows, plan._positions)
         if out is not None:
             return out
     ys = y.shape

@@ -182,6 +182,8 @@ def test_python_layer_refuses_bad_arguments():
     for f in bad:
         with pytest.raises(RuntimeError):
             f()
+    with pytest.raises(AttributeError):                       # (checked once, in the constructor)
+        plan.rows = plan.rows[:1]
     for f in (lambda: X.route_experts(torch.zeros((4, 4)), 2), lambda: X.expert_plan(torch.zeros((4, 2), dtype=i32), 3),
               lambda: X.expert_linear(half(T, 8), half(E, 8, 8), plan), lambda: X.expert_combine(half(T * k, 8), torch.zeros((T, k)), plan)):
         with pytest.raises(RuntimeError, match="device tensors"):
