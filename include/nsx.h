@@ -32,7 +32,7 @@ extern "C" {
 #define NSX_MAX_SLOTS 64
 #define NSX_MAX_ADAM_SLOTS 192   /* gradient planes nsx_adam_hash_factored(_consume) reads (level-parallel runs: one per
                                    (source rank, code row), engine/level_parallel.py) */
-#define NSX_VERSION 129
+#define NSX_VERSION 130
 
 typedef uint16_t nsx_half;
 
@@ -1062,8 +1062,9 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
 /* Gradients of the above.  dx (or NULL): [R][n_in] where x holds ordered rows (rows NULL), else [x_rows][n_in], a row's choices
  * summed (rows without choices: 0).  dw (or NULL): [E][n_out][n_in], of x's dtype or (dw_f32) in 32 bits, 0 for an expert without
  * rows.  y: the forward's result if it had the ReLU (dy counts where y is not 0), else NULL.  weight is read for dx, x for dw.
- * workspace: nsx_expert_linear_bwd_workspace bytes (0: none), gather = rows are given, masked = y is. */
-int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int gather, int want_dw,
+ * workspace: nsx_expert_linear_bwd_workspace bytes (0: none), choices = top_k if rows are given, else 0 (the choices of a
+ * row are summed in 32 bits); masked = y is given. */
+int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int choices, int want_dw,
                                         int masked);
 int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, const int32_t* positions,
                           int top_k, const void* weight, const void* dy, int64_t dy_stride, const void* y, int64_t y_stride, int n_in,

@@ -27,9 +27,11 @@ __device__ __forceinline__ int64_t valid_rows(int64_t T, const int64_t* n_dev) {
 
 // A thread makes 8 columns of a row (16 bytes per load and store, neighbours side by side); the KU choices of a round are read side
 // by side, so that their latencies overlap, and added in their order: 8 choices one after the other take 34 us where this takes 30.
-template <typename T, int KU>
+// Y: what y lies in (the type of the result, or 32 bits).
+template <typename T, int KU, typename Y>
 __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __restrict__ out) {
     typedef typename Elem<T>::x8 x8;
+    typedef typename Elem<Y>::x8 y8;
     const int64_t total = valid_rows(a.T, a.n_dev) * a.chunks;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t t = i / a.chunks;
@@ -40,7 +42,7 @@ __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __re
         for (int j = 0; j < a.k; j += KU) {
             int p[KU];
             float w[KU];
-            x8 v[KU];
+            y8 v[KU];
 #pragma unroll
             for (int u = 0; u < KU; ++u) {
                 const bool in = KU <= 2 || j + u < a.k;
@@ -49,7 +51,7 @@ __global__ __launch_bounds__(256) void combine_fwd_kernel(CombineArgs a, T* __re
             }
 #pragma unroll
             for (int u = 0; u < KU; ++u)
-                if ((unsigned)p[u] < (unsigned)a.R) v[u] = *reinterpret_cast<const x8*>(reinterpret_cast<const T*>(a.y) + (int64_t)p[u] * a.y_stride + c * 8);
+                if ((unsigned)p[u] < (unsigned)a.R) v[u] = *reinterpret_cast<const y8*>(reinterpret_cast<const Y*>(a.y) + (int64_t)p[u] * a.y_stride + c * 8);
 #pragma unroll
             for (int u = 0; u < KU; ++u)
                 if ((unsigned)p[u] < (unsigned)a.R)
@@ -137,11 +139,22 @@ static void combine_bwd_launch(const CombineArgs& a, const T* dout, T* dy, float
     else if (a.chunks > 96 && a.chunks <= 128) combine_bwd_kernel<T, 2, 2><<<grid, 256, 0, st>>>(a, dout, dy, dw, lg);
     else combine_bwd_kernel<T, 0, 1><<<grid, 256, 0, st>>>(a, dout, dy, dw, lg);
 }
-template <typename T>
-static void combine_fwd_launch(const CombineArgs& a, T* out, unsigned grid, hipStream_t st) {
-    if (a.k == 1) combine_fwd_kernel<T, 1><<<grid, 256, 0, st>>>(a, out);
-    else if (a.k == 2) combine_fwd_kernel<T, 2><<<grid, 256, 0, st>>>(a, out);
-    else combine_fwd_kernel<T, 4><<<grid, 256, 0, st>>>(a, out);
+template <typename Y, typename T>
+static void combine_fwd_launch(const CombineArgs& a, T* out, hipStream_t st) {
+    const int64_t blocks = (a.T * a.chunks + 255) / 256, most = (int64_t)num_cus() * 32;
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    if (a.k == 1) combine_fwd_kernel<T, 1, Y><<<grid, 256, 0, st>>>(a, out);
+    else if (a.k == 2) combine_fwd_kernel<T, 2, Y><<<grid, 256, 0, st>>>(a, out);
+    else combine_fwd_kernel<T, 4, Y><<<grid, 256, 0, st>>>(a, out);
+}
+
+int expert_join_f32(const float* y, int64_t R, int n, const int32_t* positions, int64_t T, int top_k, void* out, int dtype, hipStream_t st) {
+    if (T == 0) return NSX_OK;
+    const CombineArgs a{y, n, nullptr, positions, nullptr, T, top_k, (int)R, n / 8, nullptr};
+    if (dtype == NSX_DTYPE_F16) combine_fwd_launch<float>(a, (half_t*)out, st);
+    else combine_fwd_launch<float>(a, (bf16_t*)out, st);
+    NSX_LAUNCH_CHECK("expert_join_f32");
+    return NSX_OK;
 }
 
 }  // namespace nsx
@@ -167,12 +180,9 @@ int nsx_expert_combine_fwd(const void* y, int dtype, int64_t y_stride, int64_t R
     if (T == 0) return NSX_OK;
     NSX_REQUIRE(positions && out && (y || R == 0) && aligned16(out), "nsx_expert_combine_fwd: NULL or unaligned pointer");
     CombineArgs a{y, y_stride, weights, positions, nullptr, T, top_k, (int)R, n / 8, n_device};
-    const int64_t items = T * (n / 8);
-    const int64_t blocks = (items + 255) / 256, most = (int64_t)num_cus() * 32;
-    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == NSX_DTYPE_F16) combine_fwd_launch(a, (half_t*)out, grid, st);
-    else combine_fwd_launch(a, (bf16_t*)out, grid, st);
+    if (dtype == NSX_DTYPE_F16) combine_fwd_launch<half_t>(a, (half_t*)out, st);
+    else combine_fwd_launch<bf16_t>(a, (bf16_t*)out, st);
     NSX_LAUNCH_CHECK("nsx_expert_combine_fwd");
     return NSX_OK;
 }

@@ -13,6 +13,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename T> struct Elem;
 template <> struct Elem<half_t> { typedef half_t x8 __attribute__((ext_vector_type(8))); typedef half_t x4 __attribute__((ext_vector_type(4))); };
 template <> struct Elem<bf16_t> { typedef bf16_t x8 __attribute__((ext_vector_type(8))); typedef bf16_t x4 __attribute__((ext_vector_type(4))); };
+template <> struct Elem<float> { typedef float x8 __attribute__((ext_vector_type(8), aligned(16))); typedef float x4 __attribute__((ext_vector_type(4))); };
 
 // n / d for 0 <= n < 2^31 by one high multiplication (the quotient's error of the rounded-up reciprocal is below 1 / d).
 struct FastDiv {
@@ -36,6 +37,9 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
+
+// expert_combine.hip: out [T][n] (dtype: 16 bits) = sum over a row's choices of y [R][n], which lies in 32 bits
+int expert_join_f32(const float* y, int64_t R, int n, const int32_t* positions, int64_t T, int top_k, void* out, int dtype, hipStream_t st);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

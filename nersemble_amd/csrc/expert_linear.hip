@@ -20,6 +20,7 @@
 // have, every workgroup finds its (expert, tile) by one scan of the offsets.
 #include "expert_common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace nsx {
 
@@ -333,8 +334,8 @@ __global__ __launch_bounds__(WM * WC * kWave, 2) void expert_linear_kernel(LinAr
 
     const int c_first = (MODE == LIN_DW ? c0 : a) + wc * (TC / WC), c_end = MODE == LIN_DW ? g.C : b, m_first = m0 + wm * (TM / WM);
     if (F32) {
-        float* D = g.chunk > 0 ? g.partial + (int64_t)chunk * g.C * g.M : reinterpret_cast<float*>(g.d) + e * g.d_expert;
-        const int64_t ldd = g.chunk > 0 ? g.M : g.ldd;
+        float* D = MODE == LIN_DW && g.chunk > 0 ? g.partial + (int64_t)chunk * g.C * g.M : reinterpret_cast<float*>(g.d) + (MODE == LIN_DW ? e * g.d_expert : 0);
+        const int64_t ldd = MODE == LIN_DW && g.chunk > 0 ? g.M : g.ldd;
 #pragma unroll
         for (int j = 0; j < FC; ++j) {
             const int c = c_first + j * 32 + (lane & 31);
@@ -455,20 +456,26 @@ __device__ __forceinline__ void narrow_matrix(const LinArgs& g, int e, u32x4 (&p
         }
     }
 }
-// 4 MT consecutive values of row `at`, from m on
-template <typename T, int MT>
+// 4 MT consecutive values of row `at`, from m on, in D (16 or 32 bits)
+template <typename D, int MT>
 __device__ __forceinline__ void narrow_store(const LinArgs& g, int at, const f32x4 (&acc)[MT], bool relu) {
     const int m = ((threadIdx.x & 63) >> 4) * (4 * MT);
-    alignas(16) T out[4 * MT];
+    D* d = reinterpret_cast<D*>(g.d) + (int64_t)at * g.ldd + m;
+    if constexpr (sizeof(D) == 4) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (m + t * 4 < g.M) *reinterpret_cast<f32x4*>(d + t * 4) = acc[t];
+        return;
+    }
+    alignas(16) D out[4 * MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             float v = acc[t][r];
             if (relu) v = v <= 0.f ? 0.f : v;                  // (NaN stays)
-            out[t * 4 + r] = (T)v;
+            out[t * 4 + r] = (D)v;
         }
-    T* d = reinterpret_cast<T*>(g.d) + (int64_t)at * g.ldd + m;
     if (MT == 1) {
         if (m < g.M) *reinterpret_cast<u32x2*>(d) = *reinterpret_cast<const u32x2*>(out);
     } else
@@ -477,7 +484,7 @@ __device__ __forceinline__ void narrow_store(const LinArgs& g, int at, const f32
             if (m + h * 8 < g.M) *reinterpret_cast<u32x4*>(d + h * 8) = *reinterpret_cast<const u32x4*>(out + h * 8);
 }
 
-template <typename T, int MODE, int MT, int QS, bool MASK>
+template <typename T, typename D, int MODE, int MT, int QS, bool MASK>
 __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, piece = lane >> 4;
     int e, a, b;
@@ -522,7 +529,7 @@ __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
         if (nothing)                                      // (the first expert's matrix may hold what is not finite)
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (a + u * 16 + c < b) narrow_store<T, MT>(g, a + u * 16 + c, acc, MODE == LIN_FWD && g.relu);
+        if (a + u * 16 + c < b) narrow_store<D, MT>(g, a + u * 16 + c, acc, MODE == LIN_FWD && g.relu);
     }
 }
 
@@ -556,7 +563,7 @@ __device__ __forceinline__ void put_turned(char* lds, const u32x4 (&v)[4][S], in
     }
 }
 
-template <typename T, int MT, int QS, bool MASK>
+template <typename T, typename D, int MT, int QS, bool MASK>
 __global__ __launch_bounds__(4 * kWave, 3) void expert_narrow_bwd_kernel(LinArgs g) {
     constexpr int XS = (MT + 1) / 2, CT = 2 * QS, MINE = (16 * MT + 32 * QS) * 128;
     static_assert(MT * CT * 1024 <= MINE, "the sums fit where the rows were");
@@ -565,9 +572,10 @@ __global__ __launch_bounds__(4 * kWave, 3) void expert_narrow_bwd_kernel(LinArgs
     int e, a, b;
     if (!find_tile(g.offsets, g.E, g.R, g.chunk, blockIdx.x, e, a, b)) return;
     if (e == g.E) {                                            // rows behind the last segment
-        const int m8 = g.M / 8;
-        for (int i = threadIdx.x; i < (b - a) * m8; i += 4 * kWave)
-            *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(g.d) + (int64_t)(a + i / m8) * g.ldd + i % m8 * 8) = u32x4{0, 0, 0, 0};
+        constexpr int PIECE = 16 / sizeof(D);
+        const int pieces = g.M / PIECE;
+        for (int i = threadIdx.x; i < (b - a) * pieces; i += 4 * kWave)
+            *reinterpret_cast<u32x4*>(reinterpret_cast<D*>(g.d) + (int64_t)(a + i / pieces) * g.ldd + i % pieces * PIECE) = u32x4{0, 0, 0, 0};
         return;
     }
     char* zt = turned[wave];
@@ -626,7 +634,7 @@ __global__ __launch_bounds__(4 * kWave, 3) void expert_narrow_bwd_kernel(LinArgs
             for (int s = 0; s < QS; ++s)
 #pragma unroll
                 for (int t = 0; t < MT; ++t) acc[t] = mfma16<T>(p[t][s], q[u][s], acc[t]);
-            if (r0 + u * 16 + c < b) narrow_store<T, MT>(g, r0 + u * 16 + c, acc, false);
+            if (r0 + u * 16 + c < b) narrow_store<D, MT>(g, r0 + u * 16 + c, acc, false);
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -657,22 +665,22 @@ __global__ __launch_bounds__(4 * kWave, 3) void expert_narrow_bwd_kernel(LinArgs
     }
 }
 
-template <typename T, int MT, int QS>
+template <typename T, typename D, int MT, int QS>
 static void narrow_bwd_tile(const LinArgs& g, hipStream_t st) {
     const unsigned blocks = (unsigned)(g.R / g.chunk + g.E + 1);
-    if (g.mask) expert_narrow_bwd_kernel<T, MT, QS, true><<<blocks, 4 * kWave, 0, st>>>(g);
-    else expert_narrow_bwd_kernel<T, MT, QS, false><<<blocks, 4 * kWave, 0, st>>>(g);
+    if (g.mask) expert_narrow_bwd_kernel<T, D, MT, QS, true><<<blocks, 4 * kWave, 0, st>>>(g);
+    else expert_narrow_bwd_kernel<T, D, MT, QS, false><<<blocks, 4 * kWave, 0, st>>>(g);
 }
-template <typename T, int MT>
+template <typename T, typename D, int MT>
 static void narrow_bwd_m(const LinArgs& g, hipStream_t st) {
-    if (g.K <= 32) narrow_bwd_tile<T, MT, 1>(g, st);
-    else narrow_bwd_tile<T, MT, 2>(g, st);
+    if (g.K <= 32) narrow_bwd_tile<T, D, MT, 1>(g, st);
+    else narrow_bwd_tile<T, D, MT, 2>(g, st);
 }
-template <typename T>
+template <typename T, typename D>
 static void narrow_bwd(const LinArgs& g, hipStream_t st) {
-    if (g.M <= 16) narrow_bwd_m<T, 1>(g, st);
-    else if (g.M <= 32) narrow_bwd_m<T, 2>(g, st);
-    else narrow_bwd_m<T, 4>(g, st);
+    if (g.M <= 16) narrow_bwd_m<T, D, 1>(g, st);
+    else if (g.M <= 32) narrow_bwd_m<T, D, 2>(g, st);
+    else narrow_bwd_m<T, D, 4>(g, st);
 }
 // rows per chunk where both gradients of a layer are made at once (0: they are not): a round of three workgroups per CU
 static int narrow_bwd_chunk(int64_t R, int n_in, int n_out) {
@@ -681,23 +689,23 @@ static int narrow_bwd_chunk(int64_t R, int n_in, int n_out) {
     return (int)std::min<int64_t>(chunk, 1 << 20);
 }
 
-template <typename T, int MODE, int MT, int QS>
+template <typename T, typename D, int MODE, int MT, int QS>
 static void narrow_launch_tile(const LinArgs& g, hipStream_t st) {
     const unsigned blocks = (unsigned)(g.R / NARROW_ROWS + g.E + 1);
     constexpr bool MAY_MASK = MODE != LIN_FWD;
-    if (MAY_MASK && g.mask) expert_narrow_kernel<T, MODE, MT, QS, MAY_MASK><<<blocks, 4 * kWave, 0, st>>>(g);
-    else expert_narrow_kernel<T, MODE, MT, QS, false><<<blocks, 4 * kWave, 0, st>>>(g);
+    if (MAY_MASK && g.mask) expert_narrow_kernel<T, D, MODE, MT, QS, MAY_MASK><<<blocks, 4 * kWave, 0, st>>>(g);
+    else expert_narrow_kernel<T, D, MODE, MT, QS, false><<<blocks, 4 * kWave, 0, st>>>(g);
 }
-template <typename T, int MODE, int MT>
+template <typename T, typename D, int MODE, int MT>
 static void narrow_launch_m(const LinArgs& g, hipStream_t st) {
-    if (g.K <= 32) narrow_launch_tile<T, MODE, MT, 1>(g, st);
-    else narrow_launch_tile<T, MODE, MT, 2>(g, st);
+    if (g.K <= 32) narrow_launch_tile<T, D, MODE, MT, 1>(g, st);
+    else narrow_launch_tile<T, D, MODE, MT, 2>(g, st);
 }
-template <typename T, int MODE>
+template <typename T, typename D, int MODE>
 static void narrow_launch(const LinArgs& g, hipStream_t st) {
-    if (g.M <= 16) narrow_launch_m<T, MODE, 1>(g, st);
-    else if (g.M <= 32) narrow_launch_m<T, MODE, 2>(g, st);
-    else narrow_launch_m<T, MODE, 4>(g, st);
+    if (g.M <= 16) narrow_launch_m<T, D, MODE, 1>(g, st);
+    else if (g.M <= 32) narrow_launch_m<T, D, MODE, 2>(g, st);
+    else narrow_launch_m<T, D, MODE, 4>(g, st);
 }
 
 // dz of the routed rows, once: where many tiles would read y and mask dy again.  Bound by memory: 32768 x 2048, 403 MB: 68 us (5.9 TB/s, partly from the caches).
@@ -809,12 +817,17 @@ static bool mask_once(int64_t R, int n_in, int n_out) { return n_in >= 1024 || (
 template <typename T, int MODE, bool F32>
 static int lin_launch(const LinArgs& g, bool small, hipStream_t st) {
     if constexpr (MODE != LIN_DW)
-        if (g.M <= 64 && g.K <= 64 && (MODE == LIN_FWD || g.M * g.K <= 2048)) { narrow_launch<T, MODE>(g, st); return NSX_OK; }
-    if (!g.mask && !F32) {              // (with a mask to apply they do not fit the registers)
-        const int64_t tm = (g.M + 127) / 128;
-        if (MODE != LIN_DW && !small && g.M > 128 && large_tiles((g.R / 128 + std::min(g.E, g.R)) * tm)) return lin_launch_tile<T, MODE, 256, 128, 2, 2, F32>(g, st);
-        if (MODE == LIN_DW && g.C > 128 && large_tiles(g.E * tm * ((g.C + 127) / 128))) return lin_launch_tile<T, MODE, 128, 256, 1, 4, F32>(g, st);
-    }
+        if (g.M <= 64 && g.K <= 64 && (MODE == LIN_FWD || g.M * g.K <= 2048)) {
+            narrow_launch<T, std::conditional_t<F32, float, T>, MODE>(g, st);
+            return NSX_OK;
+        }
+    if constexpr (MODE != LIN_DW || !F32)
+        if (!g.mask) {                  // (with a mask to apply they do not fit the registers)
+            const int64_t tm = (g.M + 127) / 128;
+            if constexpr (MODE != LIN_DW) {
+                if (!small && g.M > 128 && large_tiles((g.R / 128 + std::min(g.E, g.R)) * tm)) return lin_launch_tile<T, MODE, 256, 128, 2, 2, F32>(g, st);
+            } else if (g.C > 128 && large_tiles(g.E * tm * ((g.C + 127) / 128))) return lin_launch_tile<T, MODE, 128, 256, 1, 4, F32>(g, st);
+        }
     if (small) return lin_launch_tile<T, MODE, 64, 64, 1, 2, F32>(g, st);
     return lin_launch_tile<T, MODE, 128, 128, 2, 2, F32>(g, st);
 }
@@ -846,7 +859,8 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
 }
 
 // workspace: dx in the plan's order, dW's partial sums, masked dy (each a multiple of 16 bytes)
-static int64_t bwd_dx_bytes(int64_t R, int n_in, bool gather) { return gather ? R * n_in * 2 : 0; }
+// choices: of a row of x (0: x holds ordered rows).  One choice is rounded once as it is; more are summed in 32 bits.
+static int64_t bwd_dx_bytes(int64_t R, int n_in, int choices) { return choices > 0 ? R * n_in * (choices > 1 ? 4 : 2) : 0; }
 static int64_t bwd_dw_bytes(int64_t R, int E, int n_in, int n_out, bool with_dx) {
     int chunk = with_dx ? nsx::narrow_bwd_chunk(R, n_in, n_out) : 0;
     if (chunk == 0) chunk = nsx::dw_plan(R, E, n_in, n_out).chunk;
@@ -854,12 +868,13 @@ static int64_t bwd_dw_bytes(int64_t R, int E, int n_in, int n_out, bool with_dx)
 }
 static int64_t bwd_dz_bytes(int64_t R, int n_in, int n_out) { return nsx::mask_once(R, n_in, n_out) ? R * n_out * 2 : 0; }
 
-int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int gather, int want_dw, int masked) {
+int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int choices, int want_dw, int masked) {
     using namespace nsx;
     int32_t some = 0;
     const int rc = lin_check("nsx_expert_linear_bwd_workspace", NSX_DTYPE_F16, n_in, n_out, E, R, 1, &some);
     if (rc != NSX_OK) return rc;
-    return (want_dx ? bwd_dx_bytes(R, n_in, gather) : 0) + (want_dw ? bwd_dw_bytes(R, E, n_in, n_out, want_dx) : 0) +
+    NSX_REQUIRE(choices >= 0 && choices <= NSX_MAX_TOP_K, "nsx_expert_linear_bwd_workspace: %d choices of a row", choices);
+    return (want_dx ? bwd_dx_bytes(R, n_in, choices) : 0) + (want_dw ? bwd_dw_bytes(R, E, n_in, n_out, want_dx) : 0) +
            (masked ? bwd_dz_bytes(R, n_in, n_out) : 0);
 }
 
@@ -878,7 +893,7 @@ int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_
                 "nsx_expert_linear_bwd: dx needs aligned pointers, weight and, for gathered rows, positions");
     NSX_REQUIRE(!dw || (aligned16(dw) && (x || x_rows == 0) && aligned16(x) && lin_stride(x_stride, n_in)),
                 "nsx_expert_linear_bwd: dw needs aligned pointers and x (row stride %lld)", (long long)x_stride);
-    const int64_t dx_bytes = dx ? bwd_dx_bytes(R, n_in, rows) : 0, dw_bytes = dw ? bwd_dw_bytes(R, E, n_in, n_out, dx != nullptr) : 0;
+    const int64_t dx_bytes = dx ? bwd_dx_bytes(R, n_in, rows ? top_k : 0) : 0, dw_bytes = dw ? bwd_dw_bytes(R, E, n_in, n_out, dx != nullptr) : 0;
     const int64_t dz_bytes = y ? bwd_dz_bytes(R, n_in, n_out) : 0;
     NSX_REQUIRE(dx_bytes + dw_bytes + dz_bytes == 0 || (workspace && aligned16(workspace)), "nsx_expert_linear_bwd: no workspace");
     hipStream_t st = (hipStream_t)stream;
@@ -897,22 +912,26 @@ int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_
     }
     const int at_once = dx && dw ? narrow_bwd_chunk(R, n_in, n_out) : 0;
     if (dx && R > 0) {
+        const bool sums = rows && top_k > 1;
         LinArgs h = g;
         h.p = weight; h.ldp = n_in; h.p_expert = (int64_t)n_in * n_out; h.d = rows ? workspace : dx; h.K = n_out;
         if (at_once) {
             h.x = x; h.ldx = x_stride; h.chunk = at_once;
-            if (dtype == NSX_DTYPE_F16) narrow_bwd<half_t>(h, st);
-            else narrow_bwd<bf16_t>(h, st);
+            if (dtype == NSX_DTYPE_F16) sums ? narrow_bwd<half_t, float>(h, st) : narrow_bwd<half_t, half_t>(h, st);
+            else sums ? narrow_bwd<bf16_t, float>(h, st) : narrow_bwd<bf16_t, bf16_t>(h, st);
         } else {
             h.rows = nullptr; h.x_rows = (int)R;
-            rc = dtype == NSX_DTYPE_F16 ? lin_launch<half_t, LIN_DX, false>(h, small_tiles(h), st) : lin_launch<bf16_t, LIN_DX, false>(h, small_tiles(h), st);
+            const bool small = small_tiles(h);
+            if (dtype == NSX_DTYPE_F16) rc = sums ? lin_launch<half_t, LIN_DX, true>(h, small, st) : lin_launch<half_t, LIN_DX, false>(h, small, st);
+            else rc = sums ? lin_launch<bf16_t, LIN_DX, true>(h, small, st) : lin_launch<bf16_t, LIN_DX, false>(h, small, st);
             if (rc != NSX_OK) return rc;
         }
         NSX_LAUNCH_CHECK("nsx_expert_linear_bwd");
-        // A row's choices are summed in 32 bits; their gradients lie in 16 bits between the two launches (in 32 they would be twice
-        // the traffic): off by at most half a step of each term beside the sum's own rounding.
+        // A row's choices are summed, and lie between the two launches, in 32 bits: the sum is rounded, not its terms (rounded terms are
+        // off by half a step of each, and one beyond the type's range is infinite where the sum is not).
         if (rows) {
-            rc = nsx_expert_combine_fwd(workspace, dtype, n_in, R, n_in, nullptr, positions, x_rows, top_k, dx, nullptr, stream);
+            rc = sums ? expert_join_f32((const float*)workspace, R, n_in, positions, x_rows, top_k, dx, dtype, st)
+                      : nsx_expert_combine_fwd(workspace, dtype, n_in, R, n_in, nullptr, positions, x_rows, top_k, dx, nullptr, stream);
             if (rc != NSX_OK) return rc;
         }
     }

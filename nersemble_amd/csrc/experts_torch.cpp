@@ -158,7 +158,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         const auto sizes = ctx->saved_data["sizes"].toIntVector();
         const int64_t x_rows = sizes[0], E = sizes[1], N = sizes[2], K = sizes[3], R = rows.size(0);
         const Tensor g = like_rows(grads[0]);
-        const int64_t need = nsx_expert_linear_bwd_workspace(R, (int)E, (int)K, (int)N, need_x, gather, need_w, y.defined());
+        const int64_t need = nsx_expert_linear_bwd_workspace(R, (int)E, (int)K, (int)N, need_x, gather ? (int)positions.size(1) : 0, need_w, y.defined());
         if (need < 0) must((int)need, "nsx_expert_linear_bwd_workspace");
         Tensor ws, dx, dw, none;
         if (need) ws = at::empty({need}, g.options().dtype(at::kByte));

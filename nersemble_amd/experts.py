@@ -268,8 +268,8 @@ def _linear(x, x_stride, w16, plan, gather, relu):
     return y
 
 
-def _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w, masked):
-    n = lib().nsx_expert_linear_bwd_workspace(R, E, K, N, need_x, gather, need_w, masked)
+def _linear_bwd_bytes(R, E, K, N, need_x, choices, need_w, masked):
+    n = lib().nsx_expert_linear_bwd_workspace(R, E, K, N, need_x, choices, need_w, masked)
     if n < 0:
         check(n, "nsx_expert_linear_bwd_workspace")
     return n
@@ -285,7 +285,7 @@ def _linear_bwd(ctx, dy):
     else:
         g, g_stride = _rows_of(dy, 8)
     dev = _here(g)
-    need = _linear_bwd_bytes(R, E, K, N, need_x, gather, need_w, y is not None)
+    need = _linear_bwd_bytes(R, E, K, N, need_x, plan.top_k if gather else 0, need_w, y is not None)
     ws = g.new_empty((need // 2,)) if need else None
     dx = g.new_empty((x_rows, K)) if need_x else None
     dw = None if not need_w else g.new_empty((E, N, K)) if w_dtype == g.dtype else g.new_empty((E, N, K), dtype=w_dtype)

@@ -188,3 +188,14 @@ def test_python_layer_refuses_bad_arguments():
               lambda: X.expert_linear(half(T, 8), half(E, 8, 8), plan), lambda: X.expert_combine(half(T * k, 8), torch.zeros((T, k)), plan)):
         with pytest.raises(RuntimeError, match="device tensors"):
             f()
+
+
+def test_workspace_of_a_gathered_gradient():
+    """One choice of a row is rounded as it is; the terms of more are kept in 32 bits until they are summed."""
+    from nersemble_amd import _lib
+    ws = _lib.lib().nsx_expert_linear_bwd_workspace
+    assert ws(16, 4, 32, 64, 1, 1, 0, 0) == 16 * 32 * 2
+    assert ws(16, 4, 32, 64, 1, 2, 0, 0) == ws(16, 4, 32, 64, 1, 8, 0, 0) == 16 * 32 * 4
+    assert ws(16, 4, 32, 64, 1, 0, 0, 0) == 0
+    _refused(ws(16, 4, 32, 64, 1, -1, 0, 0), "choices")
+    _refused(ws(16, 4, 32, 64, 1, 65, 0, 0), "choices")

@@ -988,3 +988,54 @@ def test_route_pairs_that_32_bits_do_not_tell(E, k, G, tg, gt, sc, cuda):
     ww, wc = ox.route(x, k, sig, bias, G, tg, gt)
     assert clear.mean() > 0.9 and np.array_equal(c.cpu().numpy()[clear], wc[clear])
     _close(w.cpu()[clear], ww[clear], _route_tol(x, ww, k)[clear], "weights")
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# gathered gradients are rounded once
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T,k,E,K,N,relu,only_x", [
+    (211, 2, 5, 72, 48, False, False), (900, 3, 7, 264, 136, True, False), (9000, 2, 7, 32, 64, True, False), (9000, 2, 7, 64, 64, False, False),
+    (5003, 8, 16, 16, 24, False, False), (4000, 3, 7, 32, 64, True, True), (4000, 2, 5, 64, 64, False, True), (700, 1, 4, 40, 72, False, False),
+    (3, 64, 70, 1024, 64, False, False), (6000, 2, 3, 1024, 264, True, False), (16384, 2, 17, 1000, 2056, False, False)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_gathered_gradient_is_rounded_once(T, k, E, K, N, relu, only_x, dtype, cuda):
+    """dx of a gathered product: a row's choices are summed in 32 bits (off by at most (N + 2 + k) 2 u sum |terms|) and the sum is rounded,
+    not its terms: h * |sum|, where h more of each term would pass it by far."""
+    from nersemble_amd import experts as X
+    g = torch.Generator(device=cuda).manual_seed(T + K)
+    dt, (h, tiny) = DT[dtype], HALF[DT[dtype]]
+    c = torch.rand((T, E), generator=g, device=cuda).topk(k, dim=1).indices.int()
+    c[::7] = -1
+    plan = X.expert_plan(c, E)
+    x = torch.randn((T, K), generator=g, device=cuda).to(dt).requires_grad_(True)
+    w = (torch.randn((E, N, K), generator=g, device=cuda) / K ** 0.5).to(dt).requires_grad_(not only_x)
+    y = X.expert_linear(x, w, plan, relu=relu)
+    dy = torch.randn(y.shape, generator=g, device=cuda).to(dt)
+    dx = torch.autograd.grad(y, [x] if only_x else [x, w], dy)[0].double()
+    want, mag = torch.zeros((T, K), dtype=torch.float64, device=cuda), torch.zeros((T, K), dtype=torch.float64, device=cuda)
+    off = plan.offsets.tolist()
+    for e in range(E):
+        a, b = off[e], off[e + 1]
+        r = (plan.rows[a:b] // k).long()
+        dz, we = dy[a:b].double(), w.detach()[e].double()
+        if relu:
+            dz = dz * (y[a:b] > 0)
+        want.index_add_(0, r, dz @ we)
+        mag.index_add_(0, r, dz.abs() @ we.abs())
+    tol = h * want.abs() + tiny + (1 + h) * (N + 2 + k) * 2 * U * mag
+    worst = ((dx - want).abs() / tol).max()
+    assert worst <= 1.0, float(worst)
+
+
+@pytest.mark.parametrize("T,K,N", [(40, 8, 8), (40, 72, 80), (3000, 32, 64), (3000, 8, 8), (600, 256, 136)])
+def test_gathered_gradient_whose_terms_alone_pass_fp16(T, K, N, cuda):
+    """Two choices whose gradients are +80000 and -79600 (fp16 ends at 65504): their sum is 400, exactly."""
+    from nersemble_amd import experts as X
+    plan = X.expert_plan(torch.tensor([[0, 1]], dtype=torch.int32, device=cuda).repeat(T, 1), 2)
+    x = torch.ones((T, K), dtype=torch.float16, device=cuda, requires_grad=True)
+    w = torch.zeros((2, N, K), dtype=torch.float16, device=cuda)
+    w[0, :8], w[1, :8] = 200.0, -199.0
+    w.requires_grad_(True)
+    y = X.expert_linear(x, w, plan)
+    dx, _ = torch.autograd.grad(y, [x, w], torch.full_like(y, 50.0))
+    assert (dx == 400).all()
