@@ -127,10 +127,17 @@ __device__ __forceinline__ void choose(const RouteArgs& a, typename Order<K>::ty
     wave_lds_fence();
 }
 
-// groups that stay: the values of the others become none.  Returns the distance between the last group that stays and the first
-// that does not, and the former's value.
-template <typename K, int V>
-__device__ __forceinline__ K keep_groups(const RouteArgs& a, typename Order<K>::type (&c)[V], int r, int g, K& lowest) {
+// Distance below which two 32-bit values of the choice may have changed places: twice the error of one.  Sigmoid: the
+// exponential is off by (|x| + 2) 2^-23 relatively, which s (1 - s) takes below 3e-7; reciprocal and sums add 2e-7.  Softmax: the
+// exponential by |x - max| 2^-24 + 2^-23 relatively, at most 1.5e-7 of 1 after exp(x - max); its sum of up to 512 terms by
+// 3e-6 relatively.  Adding the bias rounds once more.
+__device__ __forceinline__ float unsure(float v, int sigmoid) { return (sigmoid ? 1e-6f : 8e-6f) + 2.5e-7f * fabsf(v); }
+
+// groups that stay: the values of the others become none.  DOUBT: returns whether the groups are beyond doubt -- each that stays is
+// above each that does not by more than their errors.  A group's error is that of its members, which follows their sizes and not that of
+// their sum (two large biases may cancel in it), and the sum's rounding.
+template <bool DOUBT, typename K, int V>
+__device__ __forceinline__ bool keep_groups(const RouteArgs& a, typename Order<K>::type (&c)[V], int r, int g) {
     typedef Order<K> O;
     auto b1 = O::none(), b2 = O::none();
 #pragma unroll
@@ -156,16 +163,14 @@ __device__ __forceinline__ K keep_groups(const RouteArgs& a, typename Order<K>::
     if (!stays)
 #pragma unroll
         for (int i = 0; i < V; ++i) c[i] = O::none();
-    lowest = -row_all<TakeMax>(stays ? -mine : (K)-INFINITY, 1 << a.lg_L);
-    const K highest = row_all<TakeMax>(stays || g >= a.G ? (K)-INFINITY : mine, 1 << a.lg_L);
-    return lowest - highest;
+    if constexpr (!DOUBT) return true;
+    float off = 0.f;                                           // (infinite sums are what they are)
+    if (fabsf(mine) < INFINITY)
+        off = 0.5f * unsure(O::value(b1), a.sigmoid) + (a.group_top == 2 ? 0.5f * unsure(O::value(b2), a.sigmoid) + 6e-8f * fabsf(mine) : 0.f);
+    const float lowest = -row_all<TakeMax>(stays ? off - mine : -INFINITY, 1 << a.lg_L);
+    const float highest = row_all<TakeMax>(stays || g >= a.G ? -INFINITY : mine + off, 1 << a.lg_L);
+    return lowest - highest > 0.f;
 }
-
-// Distance below which two 32-bit values of the choice may have changed places: twice the error of one.  Sigmoid: the
-// exponential is off by (|x| + 2) 2^-23 relatively, which s (1 - s) takes below 3e-7; reciprocal and sums add 2e-7.  Softmax: the
-// exponential by |x - max| 2^-24 + 2^-23 relatively, at most 1.5e-7 of 1 after exp(x - max); its sum of up to 512 terms by
-// 3e-6 relatively.  Adding the bias rounds once more.
-__device__ __forceinline__ float unsure(float v, int sigmoid) { return (sigmoid ? 1e-6f : 8e-6f) + 2.5e-7f * fabsf(v); }
 
 // SCORES: the choice goes by scores, else by the logits themselves.  32 bits first; where neighbours of the choice lie closer than
 // `unsure`, the chosen and the one that just missed are compared in 64 bits, where more may have taken part all experts of the rows.
@@ -209,8 +214,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
     if (!SCORES) {
 #pragma unroll
         for (int i = 0; i < V; ++i) c[i] = bad ? Order<float>::none() : Order<float>::of(x[i]);
-        float lowest;
-        if (a.top_groups < a.G) keep_groups<float>(a, c, r, g, lowest);
+        if (a.top_groups < a.G) keep_groups<false, float>(a, c, r, g);
         choose<float>(a, c, e0, r, sub, 0, a.k, out);
     } else {
         float bias[V];
@@ -230,11 +234,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
             c[i] = (!bad && x[i] > -INFINITY && v == v) ? Order<float>::of(v) : Order<float>::none();
         }
         bool whole = false;                                    // the groups that stay, or more than one expert behind the choice, are in doubt
-        if (a.top_groups < a.G) {
-            float lowest;
-            const float gap = keep_groups<float>(a, c, r, g, lowest);                // (of sums of up to two)
-            whole = !(gap > 2.f * unsure(lowest, a.sigmoid)) && !bad;
-        }
+        if (a.top_groups < a.G) whole = !keep_groups<true, float>(a, c, r, g) && !bad;
         choose<float>(a, c, e0, r, sub, 0, a.k + 1, out);
         for (int j = sub; j < a.k; j += L) {
             const Chosen<float> p = out[j], q = out[j + 1];
@@ -271,8 +271,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
                     const double v = (a.sigmoid ? d[i] : d[i] / z) + (double)bias[i];
                     d[i] = (!bad && x[i] > -INFINITY && v == v) ? v : -INFINITY;
                 }
-                double lowest;
-                if (a.top_groups < a.G) keep_groups<double>(a, d, r, g, lowest);
+                if (a.top_groups < a.G) keep_groups<false, double>(a, d, r, g);
                 choose<double>(a, d, e0, r, sub, 0, a.k, wide);
                 // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from)
                 if (sub == 0)

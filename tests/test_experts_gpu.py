@@ -1039,3 +1039,36 @@ def test_gathered_gradient_whose_terms_alone_pass_fp16(T, K, N, cuda):
     y = X.expert_linear(x, w, plan)
     dx, _ = torch.autograd.grad(y, [x, w], torch.full_like(y, 50.0))
     assert (dx == 400).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# groups whose members have large biases of opposite signs
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("big", [8.0, 64.0, 1000.0, 30000.0])
+@pytest.mark.parametrize("E,G,tg", [(4, 2, 1), (32, 4, 2), (64, 8, 3)])
+@pytest.mark.parametrize("sc", ["sigmoid", "softmax"])
+def test_route_groups_of_large_biases_that_cancel(E, G, tg, big, sc, cuda):
+    """A group's two best are s + B and s' - B: their sum is of the size of a score, its error in 32 bits of the size of B's steps.  Sums of
+    two groups a few 1e-6 apart: the groups that stay are those of 64 bits."""
+    from nersemble_amd import experts as X
+    rng = np.random.default_rng(E)
+    T, per = 2000, E // G
+    bias = np.full((G, per), -2 * big, np.float32)
+    bias[:, 0], bias[:, 1] = big, -big
+    s = rng.uniform(0.1, 0.9, (T, G, per))
+    # groups in pairs: the second's sum is the first's and a few 1e-6
+    other = s[:, 0::2, 0] + s[:, 0::2, 1] - s[:, 1::2, 0] + rng.uniform(-4e-6, 4e-6, (T, G // 2))
+    fine = (other > 0.05) & (other < 0.95)
+    s[:, 1::2, 1] = np.where(fine, other, s[:, 1::2, 1])
+    s = s.reshape(T, E)
+    x = (np.log(s / (1 - s)) if sc == "sigmoid" else np.log(s)).astype(np.float32)
+    bias = bias.reshape(-1)
+    k = min(3, tg * per)
+    _, wc = ox.route(x, k, sc == "sigmoid", bias, G, tg, 2)
+    by = np.sort((ox.scores(x, sc == "sigmoid") + bias).reshape(T, G, per), axis=2)[:, :, -2:].sum(2)
+    gaps = np.diff(np.sort(by, axis=1), axis=1)
+    clear = (gaps > big * 2.0 ** -48).all(1)                                # (64-bit sums are themselves off by steps of B)
+    assert clear.mean() > 0.9 and (gaps < 1e-5).any(1).mean() > 0.5
+    _, c = X.route_experts(torch.from_numpy(x).to(cuda), k, scores=sc, bias=torch.from_numpy(bias).to(cuda), n_groups=G, top_groups=tg, group_top=2)
+    wrong = (c.cpu().numpy()[clear] != wc[clear]).any(1).mean()
+    assert wrong == 0, wrong
