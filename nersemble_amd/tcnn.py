@@ -130,7 +130,8 @@ class RoutedNetwork(nn.Module):
                                "(mask the rows behind it with `selector` instead)")
         if selector is not None:                    # (the gate's gradient is a product over all rows: 0 times what is not finite is not 0)
             x2 = torch.where(selector.reshape(-1, 1) != 0, x2, x2.new_zeros(()))
-        logits = x2.float() @ self.gate.t()
+        with torch.autocast(device_type=x2.device.type, enabled=False):      # (a trainer's autocast would make the product in 16 bits)
+            logits = x2.float() @ self.gate.t()
         weights, chosen = experts.route_experts(logits, self.top_k, bias=self.balance, selector=selector, **self.routing)
         plan = experts.expert_plan(chosen, self.n_experts)
         if self.training:

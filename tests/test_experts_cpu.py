@@ -199,3 +199,21 @@ def test_workspace_of_a_gathered_gradient():
     assert ws(16, 4, 32, 64, 1, 0, 0, 0) == 0
     _refused(ws(16, 4, 32, 64, 1, -1, 0, 0), "choices")
     _refused(ws(16, 4, 32, 64, 1, 65, 0, 0), "choices")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_routed_networks_logits_are_32_bits_under_autocast(dtype, monkeypatch):
+    from nersemble_amd import experts as X
+    from nersemble_amd import tcnn
+    net = tcnn.RoutedNetwork(20, 5, {"n_neurons": 64}, {"n_experts": 6, "top_k": 2})
+    seen = []
+
+    def route(logits, *args, **kw):
+        seen.append(logits)
+        raise InterruptedError
+    monkeypatch.setattr(X, "route_experts", route)
+    x = torch.randn((30, 20), generator=torch.Generator().manual_seed(0))
+    for on in (False, True):
+        with torch.autocast("cpu", dtype=dtype, enabled=on), pytest.raises(InterruptedError):
+            net(x)
+    assert seen[1].dtype == torch.float32 and torch.equal(seen[0], seen[1])

@@ -1072,3 +1072,26 @@ def test_route_groups_of_large_biases_that_cancel(E, G, tg, big, sc, cuda):
     _, c = X.route_experts(torch.from_numpy(x).to(cuda), k, scores=sc, bias=torch.from_numpy(bias).to(cuda), n_groups=G, top_groups=tg, group_top=2)
     wrong = (c.cpu().numpy()[clear] != wc[clear]).any(1).mean()
     assert wrong == 0, wrong
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# autocast, forward mode, refusals
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_routed_network_under_autocast_is_the_one_without(dtype, cuda):
+    """The router's product stays in 32 bits where the step runs under autocast (as a trainer's does): equal bits, forward and backward."""
+    from nersemble_amd import tcnn
+    net = tcnn.RoutedNetwork(20, 5, {"n_neurons": 64, "n_hidden_layers": 2}, {"n_experts": 32, "top_k": 2}).to(cuda)
+    g = torch.Generator().manual_seed(6)
+    for fill in (torch.float32, torch.float16):
+        x = torch.randn((3000, 20), generator=g).to(fill).to(cuda).requires_grad_(True)
+        sel = (torch.arange(3000, device=cuda) % 4 != 0).to(torch.uint8)
+        go = torch.randn((3000, 5), generator=g).half().to(cuda)
+        for s in (None, sel):
+            res = []
+            for on in (False, True):
+                with torch.autocast(device_type="cuda", dtype=dtype, enabled=on, cache_enabled=False):
+                    out = net(x, s)
+                res.append([out.detach()] + list(torch.autograd.grad(out, [x, net.gate, net.params], go)))
+            for name, a, b in zip(("out", "dx", "dgate", "dparams"), *res):
+                assert a.dtype == b.dtype and torch.equal(a, b), name
