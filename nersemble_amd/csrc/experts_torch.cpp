@@ -29,6 +29,8 @@ int dtype_of(const Tensor& t) {
 }
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 bool here(const Tensor& t) { return t.is_cuda() && t.get_device() == c10::hip::current_device(); }
+// forward-mode derivatives are refused (by experts.py)
+bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
 // consecutive values on the current device
 bool plain(const Tensor& t, int64_t dims) { return t.dim() == dims && t.is_contiguous() && here(t); }
 bool half_rows(const Tensor& t) { return plain(t, 2) && dtype_of(t) > 0 && t.size(1) % 8 == 0 && aligned(t); }
@@ -99,7 +101,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
 std::optional<std::pair<Tensor, Tensor>> route_experts(const Tensor& logits, int64_t top_k, int64_t sigmoid, const std::optional<Tensor>& bias,
                                                        const std::optional<Tensor>& selector, int64_t n_groups, int64_t top_groups, int64_t group_top,
                                                        int64_t renormalise, double scale) {
-    if (!plain(logits, 2) || dtype_of(logits) < 0) return {};
+    if (!plain(logits, 2) || dtype_of(logits) < 0 || dual(logits)) return {};
     const int64_t T = logits.size(0), E = logits.size(1);
     Choice c{{}, {}, top_k, sigmoid, n_groups, top_groups, group_top, renormalise, scale};
     if (bias) {
@@ -175,7 +177,8 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 std::optional<Tensor> expert_linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& copy, const Tensor& offsets, const Tensor& rows,
                                     const Tensor& positions, bool gather, bool relu) {
     const Tensor& w16 = copy ? *copy : weight;
-    if (!half_rows(x) || !plain(w16, 3) || w16.scalar_type() != x.scalar_type() || !aligned(w16) || !plan_at(offsets, rows, positions)) return {};
+    if (!half_rows(x) || !plain(w16, 3) || w16.scalar_type() != x.scalar_type() || !aligned(w16) || !plan_at(offsets, rows, positions) ||
+        dual(x) || dual(weight) || dual(w16)) return {};
     if (copy && (!here(weight) || weight.sizes() != w16.sizes() || (weight.scalar_type() != at::kFloat && weight.scalar_type() != x.scalar_type()))) return {};
     if (w16.size(0) != offsets.size(0) - 1 || w16.size(2) != x.size(1) || x.size(0) != (gather ? positions.size(0) : rows.size(0))) return {};
     if (w16.size(1) < 8 || w16.size(1) % 8 || w16.size(1) > NSX_MAX_EXPERT_WIDTH || x.size(1) < 8 || x.size(1) > NSX_MAX_EXPERT_WIDTH) return {};
@@ -213,7 +216,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
 };
 
 std::optional<Tensor> expert_combine(const Tensor& y, const Tensor& w, const Tensor& offsets, const Tensor& rows, const Tensor& positions) {
-    if (!half_rows(y) || !plain(w, 2) || w.scalar_type() != at::kFloat || !plan_at(offsets, rows, positions)) return {};
+    if (!half_rows(y) || !plain(w, 2) || w.scalar_type() != at::kFloat || !plan_at(offsets, rows, positions) || dual(y) || dual(w)) return {};
     if (w.sizes() != positions.sizes() || y.size(0) != rows.size(0) || y.size(1) < 8 || y.size(1) > NSX_MAX_EXPERT_WIDTH) return {};
     if ((y.requires_grad() || w.requires_grad()) && at::GradMode::is_enabled()) return CombineNode::apply(y, w, Plan{offsets, rows, positions});
     Tensor out;

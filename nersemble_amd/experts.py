@@ -15,6 +15,7 @@ the host and can be captured into a graph.  Under
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -113,6 +114,12 @@ def _at(t: torch.Tensor, dev: int) -> int:
     return t.data_ptr()
 
 
+def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Dual tensors (forward mode) have no ``requires_grad``: without this their tangents would be lost silently."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented")
+
+
 # ------------------------------------------------------------------------------------------------
 # choice
 # ------------------------------------------------------------------------------------------------
@@ -186,6 +193,7 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
                                   int(bool(renormalise)), float(scale))
         if out is not None:
             return out
+    _no_tangent("route_experts", logits)
     if logits.dim() != 2 or logits.dtype not in _DTYPE:
         raise RuntimeError(f"route_experts: logits are [T, E] in fp32, fp16 or bf16 (got {tuple(logits.shape)} {logits.dtype})")
     if sigmoid is None:
@@ -330,6 +338,7 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gathe
         out = _fast.expert_linear(x, weight, w16, plan._offsets, plan._rows, plan._positions, bool(gather), bool(relu))
         if out is not None:
             return out
+    _no_tangent("expert_linear", x, weight, w16)
     xs, ws, xt, wt = x.shape, weight.shape, x.dtype, weight.dtype
     if len(xs) != 2 or xt not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"expert_linear: x is [rows, n_in] in fp16 or bf16 (got {tuple(xs)} {xt})")
@@ -416,6 +425,7 @@ def expert_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) -> 
         out = _fast.expert_combine(y, weights, plan._offsets, plan._rows, plan._positions)
         if out is not None:
             return out
+    _no_tangent("expert_combine", y, weights)
     ys = y.shape
     if len(ys) != 2 or ys[0] != plan.n_entries or y.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"expert_combine: y is [{plan.n_entries}, n] in fp16 or bf16 (got {tuple(ys)} {y.dtype})")

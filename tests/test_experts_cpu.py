@@ -217,3 +217,25 @@ def test_routed_networks_logits_are_32_bits_under_autocast(dtype, monkeypatch):
         with torch.autocast("cpu", dtype=dtype, enabled=on), pytest.raises(InterruptedError):
             net(x)
     assert seen[1].dtype == torch.float32 and torch.equal(seen[0], seen[1])
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor has no ``requires_grad``: its tangent would be lost without a word."""
+    import torch.autograd.forward_ad as fwd
+    from nersemble_amd import experts as X
+    T, k, E = 4, 2, 3
+    i32 = torch.int32
+    plan = X.ExpertPlan(torch.zeros(E + 1, dtype=i32), torch.zeros(T * k, dtype=i32), torch.zeros((T, k), dtype=i32))
+    half = lambda *s: torch.zeros(s, dtype=torch.float16)                    # noqa: E731
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))                # noqa: E731
+        for call in (lambda: X.route_experts(dual(torch.zeros((T, E))), k), lambda: X.expert_linear(dual(half(T, 8)), half(E, 8, 8), plan),
+                     lambda: X.expert_linear(half(T, 8), dual(half(E, 8, 8)), plan),
+                     lambda: X.expert_linear(half(T, 8), dual(torch.zeros((E, 8, 8))), plan, w16=half(E, 8, 8)),
+                     lambda: X.expert_linear(half(T, 8), torch.zeros((E, 8, 8)), plan, w16=dual(half(E, 8, 8))),
+                     lambda: X.expert_combine(dual(half(T * k, 8)), torch.zeros((T, k)), plan),
+                     lambda: X.expert_combine(half(T * k, 8), dual(torch.zeros((T, k))), plan)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="device tensors"):            # (no tangent: as outside)
+            X.route_experts(torch.zeros((T, E)), k)

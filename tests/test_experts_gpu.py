@@ -1095,3 +1095,25 @@ def test_routed_network_under_autocast_is_the_one_without(dtype, cuda):
                 res.append([out.detach()] + list(torch.autograd.grad(out, [x, net.gate, net.params], go)))
             for name, a, b in zip(("out", "dx", "dgate", "dparams"), *res):
                 assert a.dtype == b.dtype and torch.equal(a, b), name
+
+
+def test_forward_mode_derivatives_are_refused(cuda):
+    """A dual tensor has a tangent that these calls do not carry: refused, not dropped."""
+    import torch.autograd.forward_ad as fwd
+    from nersemble_amd import experts as X
+    (x, logits, w1, w2), _ = _mixture_inputs(30, 4, 32, 64, 16, 5, cuda)
+    x, logits, w1 = x.detach(), logits.detach(), w1.detach()
+    weights, chosen = X.route_experts(logits, 2)
+    plan = X.expert_plan(chosen, 4)
+    y = X.expert_linear(x, w1, plan)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))                # noqa: E731
+        for call in (lambda: X.route_experts(dual(logits), 2), lambda: X.expert_linear(dual(x), w1, plan),
+                     lambda: X.expert_linear(x, dual(w1), plan), lambda: X.expert_combine(dual(y), weights, plan),
+                     lambda: X.expert_combine(y, dual(weights), plan), lambda: X.expert_linear(x, dual(w1.float()), plan, w16=w1)):
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        # (what has no tangent goes through inside a level too)
+        assert torch.equal(X.expert_linear(x, w1, plan), y)
