@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 
@@ -64,7 +65,6 @@ struct Choice { Tensor bias, selector; int64_t top_k, sigmoid, n_groups, top_gro
 
 int route(const Tensor& x, const Choice& c, Tensor& weights, Tensor& chosen) {
     const int64_t T = x.size(0), E = x.size(1);
-    if (c.top_k < 1 || c.top_k > NSX_MAX_TOP_K || E > NSX_MAX_EXPERTS) return NSX_ERR_INVALID;
     weights = at::empty({T, c.top_k}, x.options().dtype(at::kFloat));
     chosen = at::empty({T, c.top_k}, x.options().dtype(at::kInt));
     return nsx_expert_route_fwd(x.data_ptr(), dtype_of(x), T, (int)E, E, c.bias.defined() ? c.bias.data_ptr<float>() : nullptr,
@@ -103,6 +103,7 @@ std::optional<std::pair<Tensor, Tensor>> route_experts(const Tensor& logits, int
                                                        int64_t renormalise, double scale) {
     if (!plain(logits, 2) || dtype_of(logits) < 0 || dual(logits)) return {};
     const int64_t T = logits.size(0), E = logits.size(1);
+    if (E < 1 || E > NSX_MAX_EXPERTS || top_k < 1 || top_k > std::min<int64_t>(E, NSX_MAX_TOP_K)) return {};
     Choice c{{}, {}, top_k, sigmoid, n_groups, top_groups, group_top, renormalise, scale};
     if (bias) {
         if (!plain(*bias, 1) || bias->size(0) != E || bias->scalar_type() != at::kFloat) return {};

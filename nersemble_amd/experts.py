@@ -199,6 +199,10 @@ def route_experts(logits: torch.Tensor, top_k: int, scores: str = "softmax", bia
     if sigmoid is None:
         raise RuntimeError(f"route_experts: scores are 'softmax' or 'sigmoid' (got {scores!r})")
     T, E = logits.shape
+    if not 1 <= E <= _lib.NSX_MAX_EXPERTS:
+        raise RuntimeError(f"route_experts: n_experts {E} not in [1,{_lib.NSX_MAX_EXPERTS}]")
+    if not 1 <= int(top_k) <= min(E, _lib.NSX_MAX_TOP_K):
+        raise RuntimeError(f"route_experts: top_k {top_k} not in [1,{_lib.NSX_MAX_TOP_K}] or more than the {E} experts")
     if bias is not None:
         if bias.shape != (E,) or bias.dtype != _F32:
             raise RuntimeError(f"route_experts: bias is {tuple(bias.shape)} {bias.dtype}, not ({E},) fp32")

@@ -239,3 +239,10 @@ def test_forward_mode_derivatives_are_refused():
                 call()
         with pytest.raises(RuntimeError, match="device tensors"):            # (no tangent: as outside)
             X.route_experts(torch.zeros((T, E)), k)
+
+
+@pytest.mark.parametrize("E,k", [(16, 0), (16, 17), (128, 65), (16, -1), (4, 1 << 40), (0, 1), (513, 1)])
+def test_route_refuses_sizes_before_it_makes_results(E, k):
+    from nersemble_amd import experts as X
+    with pytest.raises(RuntimeError, match="n_experts" if E in (0, 513) else "top_k"):
+        X.route_experts(torch.zeros((4, E)), k)

@@ -1117,3 +1117,18 @@ def test_forward_mode_derivatives_are_refused(cuda):
                 call()
         # (what has no tangent goes through inside a level too)
         assert torch.equal(X.expert_linear(x, w1, plan), y)
+
+
+def test_route_says_what_it_refuses(cuda):
+    """The reason of this call, not that of an earlier failure."""
+    from nersemble_amd import experts as X
+    with pytest.raises(RuntimeError, match="scale"):
+        X.route_experts(torch.zeros((4, 16), device=cuda), 2, scale=0.0)
+    for E, k in ((16, 0), (16, 17), (128, 65), (16, -1), (4, 1 << 40)):
+        with pytest.raises(RuntimeError, match="top_k"):
+            X.route_experts(torch.zeros((4, E), device=cuda), k)
+    for E in (0, 513):
+        with pytest.raises(RuntimeError, match="n_experts|top_k"):
+            X.route_experts(torch.zeros((4, E), device=cuda), 1)
+    with pytest.raises(RuntimeError, match="n_experts"):
+        X.route_experts(torch.zeros((4, 513), device=cuda, requires_grad=True), 1)
