@@ -603,11 +603,16 @@ static void launch_plan(int blocks, const int32_t* experts, int n, int k, int E,
     plan_place_kernel<WAVES><<<blocks, WAVES * kWave, 0, st>>>(experts, n, k, E, lg2_ceil(E), per, counts, offsets, rows, positions, n_dev);
 }
 
+// bytes of LDS that a workgroup's entries take
+static size_t route_lds_bytes(int lg_L, int k, bool by_scores) {
+    return (size_t)ROUTE_WAVES * (kWave >> lg_L) * (by_scores ? (k + 2) * sizeof(Chosen<double>) : k * sizeof(Chosen<float>));
+}
+
 template <typename T, int V>
 static void launch_route(const RouteArgs& a, bool by_scores, bool vec, hipStream_t st) {
     const int rpw = kWave >> a.lg_L;
     const unsigned blocks = (unsigned)((a.T + (int64_t)rpw * ROUTE_WAVES - 1) / ((int64_t)rpw * ROUTE_WAVES));
-    const size_t lds = (size_t)ROUTE_WAVES * rpw * (by_scores ? (a.k + 2) * sizeof(Chosen<double>) : a.k * sizeof(Chosen<float>));
+    const size_t lds = route_lds_bytes(a.lg_L, a.k, by_scores);
     if (by_scores) {
         if (vec) route_fwd_kernel<T, V, true, true><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
         else route_fwd_kernel<T, V, false, true><<<blocks, ROUTE_WAVES * kWave, lds, st>>>(a);
@@ -672,12 +677,16 @@ int nsx_expert_route_fwd(const void* logits, int dtype, int64_t T, int E, int64_
     const int esize = dtype == NSX_DTYPE_F32 ? 4 : 2;
     while (V > 4 && Eg % V) V >>= 1;
     while (lg_G + lg2_ceil((Eg + V - 1) / V) > 6) V <<= 1;
+    const bool wide = bias || (top_groups < n_groups && group_top == 2);
+    // (rows of few lanes and many choices: more lanes per row where a workgroup's entries would pass 64 KB)
+    while (V > 4 && route_lds_bytes(lg_G + lg2_ceil((Eg + V - 1) / V), top_k, wide) > 65536) V >>= 1;
     const bool vec = route_vec(logits, V, esize, row_stride, Eg);
     a.lg_Lg = lg2_ceil((Eg + V - 1) / V);
     a.lg_L = lg_G + a.lg_Lg;
+    NSX_REQUIRE(a.lg_L <= 6 && route_lds_bytes(a.lg_L, top_k, wide) <= 65536, "nsx_expert_route_fwd: no layout for %d choices of %d groups of %d experts",
+                top_k, n_groups, Eg);
     NSX_REQUIRE((T << a.lg_L) + 256 < ((int64_t)1 << 32), "nsx_expert_route_fwd: %lld rows of %d lanes are more than one launch",
                 (long long)T, 1 << a.lg_L);
-    const bool wide = bias || (top_groups < n_groups && group_top == 2);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype * 32 + V) {
         case 4: launch_route<float, 4>(a, wide, vec, st); break;

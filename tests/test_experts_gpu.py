@@ -1132,3 +1132,121 @@ def test_route_says_what_it_refuses(cuda):
             X.route_experts(torch.zeros((4, E), device=cuda), 1)
     with pytest.raises(RuntimeError, match="n_experts"):
         X.route_experts(torch.zeros((4, 513), device=cuda, requires_grad=True), 1)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# choice in large batches (8 and 16 values per lane)
+# ---------------------------------------------------------------------------------------------------------------------
+def _route64(x, k, sigmoid, bias, G, tg, gt, renorm, scale, selector):
+    """(weights, chosen, scores, rows whose order 64 bits tell beyond the order of their own sums) on the device, in 64 bits."""
+    T, E = x.shape
+    xd = x.double()
+    live = xd > -np.inf
+    any_live = live.any(1, keepdim=True)
+    s = torch.sigmoid(xd) if sigmoid else torch.where(any_live, torch.softmax(torch.where(any_live, xd, torch.zeros_like(xd)), 1), torch.zeros_like(xd))
+    s = torch.where(live, s, torch.zeros_like(s))
+    c = s if bias is None else s + bias.double()
+    c = torch.where(live, c, torch.full_like(c, -np.inf))
+
+    def close(v):
+        d = torch.diff(torch.sort(v, dim=1).values, dim=1)
+        return ((d > 0) & (d < 1e-13)).any(1)
+    clear = ~close(c)
+    if tg < G:
+        by = torch.sort(c.view(T, G, E // G), dim=2, descending=True).values[..., :gt].sum(2)
+        clear &= ~close(by)
+        kept = torch.sort(by, dim=1, descending=True, stable=True).indices[:, :tg]
+        on = torch.zeros((T, G), dtype=torch.bool, device=x.device).scatter_(1, kept, True)
+        c = torch.where(on.repeat_interleave(E // G, 1), c, torch.full_like(c, -np.inf))
+    top = torch.sort(c, dim=1, descending=True, stable=True)
+    chosen, there = top.indices[:, :k], top.values[:, :k] > -np.inf
+    if selector is not None:
+        there = there & (selector != 0)[:, None]
+    u = torch.where(there, s.gather(1, chosen), torch.zeros((), dtype=torch.float64, device=x.device))
+    w = scale * (u / u.sum(1, keepdim=True).clamp(min=1e-300) if renorm else u)
+    return w, torch.where(there, chosen, -1), s, clear
+
+
+LARGE_ROUTES = [
+    # rows, E, k, scores, bias, groups, top_groups, group_top, renorm, scale
+    (131075, 32, 2, "softmax", False, 1, 1, 1, True, 1.0),               # above 2^22 values: 16 per lane
+    (131075, 32, 5, "softmax", True, 1, 1, 1, False, 2.5),
+    (131075, 32, 32, "sigmoid", True, 1, 1, 1, True, 1.0),               # entries of many choices: fewer values per lane
+    (131075, 32, 31, "softmax", True, 1, 1, 1, True, 1.0),
+    (131075, 32, 32, "softmax", False, 1, 1, 1, False, 1.0),
+    (65541, 64, 64, "softmax", True, 1, 1, 1, True, 1.0),
+    (65541, 64, 32, "sigmoid", False, 2, 1, 2, True, 1.0),
+    (65541, 64, 64, "sigmoid", True, 2, 2, 1, True, 1.0),
+    (65541, 64, 6, "sigmoid", True, 1, 1, 1, True, 1.0),
+    (131075, 33, 3, "softmax", True, 1, 1, 1, True, 1.0),
+    (131075, 48, 4, "sigmoid", True, 3, 2, 2, True, 1.0),
+    (524291, 8, 8, "softmax", True, 1, 1, 1, True, 1.0),
+    (262147, 16, 16, "sigmoid", True, 1, 1, 1, False, 1.0),
+    (16411, 256, 8, "sigmoid", True, 8, 4, 2, True, 2.5),
+    (16411, 256, 8, "softmax", False, 8, 3, 1, False, 16.0),
+    (16411, 256, 8, "softmax", False, 1, 1, 1, True, 1.0),
+    (8209, 512, 64, "softmax", True, 1, 1, 1, True, 1.0),
+    (8209, 512, 16, "sigmoid", True, 16, 4, 2, True, 1.0),
+    (8195, 96, 7, "softmax", True, 1, 1, 1, True, 1.0),                  # between 2^19 and 2^22: 8 per lane
+    (8195, 64, 64, "sigmoid", True, 1, 1, 1, True, 1.0),
+    (4111, 256, 8, "sigmoid", True, 8, 4, 2, True, 2.5),
+    (20011, 160, 6, "softmax", True, 8, 3, 2, False, 16.0),
+    (17003, 32, 32, "softmax", False, 1, 1, 1, True, 1.0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("cfg", LARGE_ROUTES, ids=lambda c: f"T{c[0]}E{c[1]}k{c[2]}{c[3][:3]}{'b' if c[4] else ''}g{c[5]}")
+def test_route_of_large_batches(cfg, dtype, cuda):
+    """Choice, weights and gradient against 64 bits: ordinary rows, rows of equal values, of values that 32-bit scores do not tell apart, rows
+    with experts taken out and rows that are not routed; rows side by side and strided ones."""
+    from nersemble_amd import experts as X
+    T, E, k, sc, has_bias, G, tg, gt, renorm, scale = cfg
+    sig = sc == "sigmoid"
+    g = torch.Generator(device=cuda).manual_seed(E * 100 + k)
+    x = torch.randn((T, E), generator=g, device=cuda) * 2
+    x[1::5] = torch.round(x[1::5] * 2) / 2                                    # equal ones
+    near = torch.rand((T, E), generator=g, device=cuda).argsort(1)[2::5].float()
+    x[2::5] = torch.randn((T, 1), generator=g, device=cuda)[2::5] + near * 2.0 ** -22      # neighbours a step of fp32 apart
+    x[3::5][torch.rand((T, E), generator=g, device=cuda)[3::5] < 0.3] = -np.inf
+    x[7] = -np.inf
+    x = x.to(DT[dtype])
+    bias = torch.randn(E, generator=g, device=cuda) * 0.1 if has_bias else None
+    if has_bias:
+        bias[E // 2:] = bias[:E - E // 2].clone()                                     # (equal biases as well)
+    sel = (torch.rand(T, generator=g, device=cuda) > 0.1).to(torch.uint8)
+    dw = torch.randn((T, k), generator=g, device=cuda)
+    for layout in ("side by side", "strided"):
+        if layout == "strided":
+            wide = torch.zeros((T, E + 40), dtype=x.dtype, device=cuda)
+            wide[:, 3:3 + E] = x
+            xd, s = wide[:, 3:3 + E].requires_grad_(True), sel
+        else:
+            xd, s = x.detach().clone().requires_grad_(True), None
+        w, c = X.route_experts(xd, k, scores=sc, bias=bias, n_groups=G, top_groups=tg, group_top=gt, renormalise=renorm, scale=scale, selector=s)
+        ww, wc, score, clear = _route64(x, k, sig, bias, G, tg, gt, renorm, scale, s)
+        assert clear.double().mean() > 0.75
+        assert torch.equal(c[clear].long(), wc[clear])
+        # as _route_tol: span of the logits (what is taken out has none)
+        span = float(torch.where(torch.isfinite(x), x.double().abs(), torch.zeros((), dtype=torch.float64, device=cuda)).max()) * 2
+        rel = (span + (k if renorm else E) + 10) * 2 * U
+        assert ((w.double() - ww).abs() <= rel * ww.abs() + 1e-37)[clear].all()
+        (d,) = torch.autograd.grad(w, [xd], dw)
+        assert d.dtype == x.dtype and d.shape == x.shape
+        on, at = (wc >= 0).double(), wc.clamp(min=0)
+        gw = dw.double() * ww * on
+        total = gw.sum(1, keepdim=True)
+        mag = gw.abs().sum(1, keepdim=True)
+        val = gw - ww * total / scale if renorm else gw
+        size = gw.abs() + (ww.abs() * mag / abs(scale) if renorm else 0.0)
+        if sig:
+            val, size = val * torch.sigmoid(-x.double()).gather(1, at), size * torch.sigmoid(-x.double()).gather(1, at)
+        want = torch.zeros((T, E), dtype=torch.float64, device=cuda).scatter_add_(1, at, val * on)
+        size = torch.zeros((T, E), dtype=torch.float64, device=cuda).scatter_add_(1, at, size * on)
+        if not sig and not renorm:
+            want, size = want - score * total, size + score * mag
+        tol = 3 * (rel * size + 1e-37)
+        if dtype != "fp32":
+            h, tiny = HALF[DT[dtype]]
+            tol = tol + h * want.abs() + tiny
+        assert torch.isfinite(d).all() and ((d.double() - want).abs() <= tol)[clear].all()
