@@ -273,9 +273,15 @@ __global__ __launch_bounds__(ROUTE_WAVES * kWave) void route_fwd_kernel(RouteArg
                 }
                 if (a.top_groups < a.G) keep_groups<false, double>(a, d, r, g);
                 choose<double>(a, d, e0, r, sub, 0, a.k, wide);
-                // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from)
+                // (back to the narrow entries; a row's first lane moves them in order: entry j lies in front of what it comes from.  Byte by
+                // byte for the compiler, which may take a store of one type for no business of a load of another.)
                 if (sub == 0)
-                    for (int j = 0; j < a.k; ++j) { const Chosen<double> w = wide[j]; out[j] = Chosen<float>{(float)w.c, w.e}; }
+                    for (int j = 0; j < a.k; ++j) {
+                        Chosen<double> w;
+                        __builtin_memcpy(&w, wide + j, sizeof w);
+                        const Chosen<float> narrow{(float)w.c, w.e};
+                        __builtin_memcpy(out + j, &narrow, sizeof narrow);
+                    }
             } else {
                 // The k + 1 candidates in 64 bits, an entry to a lane, then by their rank.
                 double* v = reinterpret_cast<double*>(mine + slots * sizeof(Chosen<float>));

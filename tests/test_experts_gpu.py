@@ -1250,3 +1250,20 @@ def test_route_of_large_batches(cfg, dtype, cuda):
             h, tiny = HALF[DT[dtype]]
             tol = tol + h * want.abs() + tiny
         assert torch.isfinite(d).all() and ((d.double() - want).abs() <= tol)[clear].all()
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 7, 16, 30, 32])
+@pytest.mark.parametrize("T", [50, 16500, 131075])
+def test_route_rows_that_are_compared_whole_in_64_bits(k, T, cuda):
+    """Every row has more candidates in doubt than one: the wide entries of the redo move over to the narrow ones, which lie in the same
+    memory, at 4, 8 and 16 values per lane."""
+    from nersemble_amd import experts as X
+    g = torch.Generator(device=cuda).manual_seed(k)
+    E = 32
+    x = torch.rand((T, E), generator=g, device=cuda).argsort(1).float() * 2.0 ** -23 + 0.25
+    bias = torch.zeros(E, device=cuda)
+    for sc in ("sigmoid", "softmax"):
+        w, c = X.route_experts(x, k, scores=sc, bias=bias)
+        ww, wc, _, clear = _route64(x, k, sc == "sigmoid", bias, 1, 1, 1, True, 1.0, None)
+        assert clear.all() and torch.equal(c.long(), wc)
+        assert ((w.double() - ww).abs() <= (1 + k + 10) * 2 * U * ww).all()
