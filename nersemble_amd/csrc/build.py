@@ -12,6 +12,7 @@ INCLUDE = os.path.join(ROOT, "include")
 OBJ = os.path.join(HERE, "_obj")
 SO = os.path.join(HERE, "libnsx.so")
 BINDING = os.path.join(HERE, "_experts.so")
+STAMP = os.path.join(OBJ, "_experts.txt")          # what BINDING was built against
 ARCH = "gfx950"
 
 
@@ -70,9 +71,26 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or jobs or _stale(SO, objs):
         run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", SO, *objs])
     src = os.path.join(HERE, "experts_torch.cpp")
-    if force or _stale(BINDING, [src, os.path.join(INCLUDE, "nsx.h"), __file__]):
+    if force or binding_is_stale(BINDING, STAMP, [src, os.path.join(INCLUDE, "nsx.h"), __file__]):
+        if os.path.exists(STAMP):
+            os.remove(STAMP)
         run(_binding(src))
+        with open(STAMP, "w") as f:
+            f.write(_built_against())
     return SO
+
+
+def _built_against() -> str:
+    """The torch and the interpreter whose classes BINDING is compiled with."""
+    import torch
+    return f"{torch.__version__} {torch.version.git_version} {sys.version}"
+
+
+def binding_is_stale(binding, stamp, deps) -> bool:
+    if _stale(binding, deps) or not os.path.exists(stamp):
+        return True
+    with open(stamp) as f:
+        return f.read() != _built_against()
 
 
 def _binding(src):
@@ -82,7 +100,7 @@ def _binding(src):
     root = os.path.join(os.path.dirname(torch.__file__))
     inc = os.path.join(root, "include")
     return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE, "-I", inc,
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DNSX_TORCH="{torch.__version__}"', "-I", INCLUDE, "-I", inc,
             "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"], "-I", "/opt/rocm/include",
             src, "-o", BINDING, "-L", os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-ltorch_python",
             "-L", HERE, "-lnsx", "-Wl,-rpath,$ORIGIN"]

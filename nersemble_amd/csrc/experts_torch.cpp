@@ -228,6 +228,8 @@ std::optional<Tensor> expert_combine(const Tensor& y, const Tensor& w, const Ten
 }  // namespace
 
 PYBIND11_MODULE(_experts, m) {
+    m.attr("nsx_version") = NSX_VERSION;           // (experts.py compares both with what runs)
+    m.attr("torch_version") = NSX_TORCH;
     m.def("route_experts", &route_experts);
     m.def("plan", &plan);
     m.def("expert_linear", &expert_linear);

@@ -33,12 +33,16 @@ class _FastNotLoaded:
 
     def __getattr__(self, name):
         global _fast
-        lib()
+        version = lib().nsx_version()
         try:
             from .csrc import _experts
         except ImportError as e:
             raise RuntimeError(f"nersemble_amd: the native binding csrc/_experts.so cannot be loaded ({e}). Build it with "
                                f"`python -c 'import __graft_entry__ as g; g.build()'`.") from e
+        if _experts.nsx_version != version or _experts.torch_version != torch.__version__:
+            raise RuntimeError(f"nersemble_amd: csrc/_experts.so was built against libnsx.so {_experts.nsx_version} and torch "
+                               f"{_experts.torch_version}, not {version} and {torch.__version__}. Build it again with "
+                               f"`python -c 'import __graft_entry__ as g; g.build()'`.")
         _fast = _experts
         return getattr(_fast, name)
 

@@ -246,3 +246,33 @@ def test_route_refuses_sizes_before_it_makes_results(E, k):
     from nersemble_amd import experts as X
     with pytest.raises(RuntimeError, match="n_experts" if E in (0, 513) else "top_k"):
         X.route_experts(torch.zeros((4, E)), k)
+
+
+def test_binding_of_another_torch_is_built_again(tmp_path, monkeypatch):
+    from nersemble_amd.csrc import build
+    so, stamp, src = (str(tmp_path / n) for n in ("b.so", "b.txt", "b.cpp"))
+    open(src, "w").close()
+    assert build.binding_is_stale(so, stamp, [src])
+    open(so, "w").close()
+    assert build.binding_is_stale(so, stamp, [src])                     # (nothing says what it was built against)
+    with open(stamp, "w") as f:
+        f.write(build._built_against())
+    assert not build.binding_is_stale(so, stamp, [src])
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert build.binding_is_stale(so, stamp, [src])
+
+
+@pytest.mark.parametrize("what", ["nsx_version", "torch_version"])
+def test_binding_of_another_library_or_torch_is_not_used(what, monkeypatch):
+    """Its calls would pass other arguments, or tensors of another layout."""
+    from nersemble_amd import csrc, experts as X
+    X._FastNotLoaded().plan                                             # (loads the one that is there)
+    from nersemble_amd.csrc import _experts
+
+    class Other:
+        nsx_version, torch_version, plan = _experts.nsx_version, _experts.torch_version, None
+    setattr(Other, what, "other")
+    monkeypatch.setattr(csrc, "_experts", Other)
+    monkeypatch.setattr(X, "_fast", X._FastNotLoaded())
+    with pytest.raises(RuntimeError, match="Build it again"):
+        X.expert_plan(torch.zeros((4, 2), dtype=torch.int32), 3)
