@@ -153,7 +153,8 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, typename Order<K
         b2 = p2 > b2 ? p2 : b2;
         b2 = lo > b2 ? lo : b2;
     }
-    const K mine = a.group_top == 2 ? O::value(b1) + O::value(b2) : O::value(b1);
+    // (a group without two experts to choose counts nothing: an infinite bias and none would have no sum)
+    const K mine = a.group_top == 2 ? (b2 > O::none() ? O::value(b1) + O::value(b2) : (K)-INFINITY) : O::value(b1);
     int before = 0;
     for (int h = 0; h < a.G; ++h) {
         const K other = __shfl(mine, (r << a.lg_L) + (h << a.lg_Lg));

@@ -1267,3 +1267,25 @@ def test_route_rows_that_are_compared_whole_in_64_bits(k, T, cuda):
         ww, wc, _, clear = _route64(x, k, sc == "sigmoid", bias, 1, 1, 1, True, 1.0, None)
         assert clear.all() and torch.equal(c.long(), wc)
         assert ((w.double() - ww).abs() <= (1 + k + 10) * 2 * U * ww).all()
+
+
+@pytest.mark.parametrize("sc", ["sigmoid", "softmax"])
+def test_route_groups_with_infinite_biases_and_one_expert_left(sc, cuda):
+    """A group whose second expert is taken out counts nothing, whatever the first one's bias: no more groups stay than were asked for."""
+    from nersemble_amd import experts as X
+    inf = np.float32(np.inf)
+    rng = np.random.default_rng(1)
+    E, G, T = 32, 8, 300
+    x = rng.standard_normal((T, E)).astype(np.float32)
+    bias = (rng.standard_normal(E) * 0.1).astype(np.float32)
+    bias[8] = inf                                    # group 2: one expert with an infinite bias, the others taken out
+    x[:, 9:12] = -inf
+    bias[20], bias[21] = inf, inf                    # group 5: two of them
+    bias[25] = -inf                                  # (an infinite bias takes out as well)
+    x[::3, 28:31] = -inf
+    for tg, k in ((1, 3), (2, 5), (3, 8)):
+        with np.errstate(invalid="ignore"):
+            ww, wc = ox.route(x, k, sc == "sigmoid", bias, G, tg, 2)
+        w, c = X.route_experts(torch.from_numpy(x).to(cuda), k, scores=sc, bias=torch.from_numpy(bias).to(cuda), n_groups=G, top_groups=tg, group_top=2)
+        assert np.array_equal(c.cpu().numpy(), wc), (tg, k)
+        _close(w, ww, _route_tol(x, ww, k), "weights")
