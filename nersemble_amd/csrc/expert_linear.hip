@@ -63,8 +63,8 @@ __device__ __forceinline__ uint32_t keep_where(uint32_t v, uint32_t y) {
 }
 
 // 0 for gathered rows that are not there: what is loaded without a branch is loaded from here
-__device__ u32x4 lin_zeros[NSX_MAX_EXPERT_WIDTH / 8 + LIN_BQ / 8];
-__device__ __forceinline__ const char* zero_row() { return reinterpret_cast<const char*>(lin_zeros); }
+__device__ u32x4 lin_zeros;
+__device__ __forceinline__ const char* zero_row() { return reinterpret_cast<const char*>(&lin_zeros); }
 __device__ __forceinline__ u32x4 load16(const char* p) { return *reinterpret_cast<const u32x4*>(p); }
 // reads behind `bytes` give 0
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t lin_buffer(const char* p, int64_t bytes) {
