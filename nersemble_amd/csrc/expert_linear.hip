@@ -420,7 +420,7 @@ __global__ __launch_bounds__(256) void expert_sum_chunks_kernel(LinArgs g, T* __
 // that a lane's 4 MT values are consecutive (m = (lane / 16) 4 MT + 4 t + r).
 // us, tiles of 64 x 64 through LDS | this, 262144 rows x 2 of 16 experts, bf16 (dx with the ReLU's mask):
 //   forward  32 -> 64  30.2 | 23.7   64 -> 64  30.1 | 29.1   64 -> 16  26.1 | 16.0   (100000 x 2 of 61: 128 -> 64  18.6 | 24.2)
-//   dx       32 -> 64  35.9 | 27.7   64 -> 64  39.1 | 43.1   64 -> 16  28.7 | 22.8   16 -> 64  32.7 | 24.8
+//   dx       32 -> 64  35.9 | 27.7   64 -> 64  39.1 | 43.1   64 -> 16  28.7 | 22.8   16 -> 64  32.7 | 24.8   (in 16 bits)
 // (dx gathers its matrix's fragments 2 bytes at a time, and with the mask's they leave fewer waves: up to 2048 weights.)
 constexpr int NARROW_ROWS = 256;      // ordered rows per workgroup of 4 waves
 
@@ -538,11 +538,14 @@ __global__ __launch_bounds__(4 * kWave) void expert_narrow_kernel(LinArgs g) {
 // own) turned: a lane holds the same 8 features of the rows c, 16 + c, 32 + c and 48 + c, which it stores side by side -- the
 // order of a sum over rows is free as long as both operands have it.  dW's 32-bit sums stay in registers for a whole chunk of a
 // segment, the four waves' are added in their order at its end; expert_sum_chunks_kernel adds the chunks.
-// Bound by memory: 262144 x 2 of 16 experts, 32 -> 64 with ReLU: 46 us for 185 MB (4.0 TB/s); dx and dW apart read dy and y
-// twice: 69.  us, both gradients with the join and the sum of the chunks, apart | at once:
-//   32 -> 64  84 | 60 (ReLU)  62 | 44 (none)    64 -> 64  112 | 94   87 | 76    64 -> 16  71 | 60    16 -> 64  75 | 49    64 -> 32  82 | 66
-//   2048 rows x 2 of 16, 32 -> 64  22 | 16      100000 x 2 of 61  43 | 30
-// Chunks for 2, 3, 4, 6 workgroups per CU: 48.9, 46.3, 45.5, 47.9 (32 -> 64), without ReLU 30.8, 30.8, 29.9, 32.5.
+// Bound by memory: 262144 x 2 of 16 experts, 32 -> 64 with ReLU, dx in 32 bits: 52 us for 218 MB (4.2 TB/s); dx and dW apart read dy
+// and y twice.  us, both gradients of gathered rows with the join and the sum of the chunks, apart | at once:
+//   32 -> 64  89 | 66 (ReLU)  69 | 53 (none)    64 -> 64  142 | 124   109 | 110    64 -> 16  98 | 86    16 -> 64  73 | 48    64 -> 32  108 | 97
+//   2048 rows x 2 of 16, 32 -> 64  18 | 12      100000 x 2 of 61, 32 -> 64  48 | 54, 64 -> 64  62 | 75 (chunks of two tiles: many are half full)
+// Chunks for 2, 3, 4, 6 workgroups per CU, dx in 16 bits: 48.9, 46.3, 45.5, 47.9 (32 -> 64), without ReLU 30.8, 30.8, 29.9, 32.5.
+// The widest tile's 64 KB of LDS and 240 to 270 registers leave room for one or two workgroups.  us, registers and chunks for three | for
+// two, 64 -> 64 with ReLU: 262144 x 2 of 16  124 | 125;  2^20 x 2 of 4  458 | 483;  100000 x 2 of 61  75 | 69;  2^20 x 2 of 16, 48 -> 40
+// 359 | 375: one rule for all tiles.
 // Feature f's row of 128 bytes lies at f with the lowest bit turned by bit 3, its 16-byte pieces permuted by f / 2: neither the
 // stores (features 8 apart) nor the fragment reads (16 features) meet on a bank.
 __device__ __forceinline__ uint32_t turned_at(int f, int piece) { return (f ^ (f >> 3 & 1)) * 128 + ((piece ^ (f >> 1)) & 7) * 16; }
@@ -682,7 +685,7 @@ static void narrow_bwd(const LinArgs& g, hipStream_t st) {
     else if (g.M <= 32) narrow_bwd_m<T, D, 2>(g, st);
     else narrow_bwd_m<T, D, 4>(g, st);
 }
-// rows per chunk where both gradients of a layer are made at once (0: they are not): a round of three workgroups per CU
+// rows per chunk where both gradients of a layer are made at once (0: they are not): for three workgroups per CU, as the table above says
 static int narrow_bwd_chunk(int64_t R, int n_in, int n_out) {
     if (n_in > 64 || n_out > 64 || R < 8 * NARROW_ROWS) return 0;
     const int64_t chunk = (R / (3 * (int64_t)num_cus()) + NARROW_ROWS) / NARROW_ROWS * NARROW_ROWS;
@@ -800,6 +803,7 @@ static DwPlan dw_plan(int64_t R, int E, int n_in, int n_out) {
 //   16384 x 2 of 8,  2048 -> 2048   forward 319 | 298 | 310   dx 305 | 309 | 305   dW 355 | 336 | 293
 //    8192 x 2 of 16, 1024 -> 1024   forward  52 |  58 |  63   dx  54 |  57 |  62   dW  56 |  65 |  55
 //    2048 x 8 of 256, 2048 -> 1024  forward 257 | 243 |       dx 253 | 233     (64 x 64: 269, 276)
+// dx of gathered rows, in 32 bits and with the join, 128 x 128 | 256 x 128: first line 240 | 229, second 407 | 415, last 300 | 283.
 // As time = f + q s the forward of the first line has f = 36 us (its result's bytes alone 27), s = 133 us per 1024 of q, 1030 TFLOP/s.
 // Matrix units busy 37 % of the cycles, LDS 32 %; the rest is the chain of a step (its loads, two barriers, stores, first fragments)
 // that two workgroups per CU cover in part: without loads it takes 22 us less, without stores into LDS 30 less again.  256 x 256
@@ -810,8 +814,8 @@ static bool large_tiles(int64_t tiles128) { return tiles128 >= 6 * (int64_t)num_
 
 // dz in a pass of its own (3 R n_out 16-bit values) or masked wherever dy is read (y once more per 128 input features in both
 // gradients, registers that large tiles do not have).  us, both gradients, masked in place | once:
-//   16384 x 2 of 16, 1024 -> 2048  616 | 455    2048 -> 1024  573 | 413    8192 x 2, 1024 -> 1024  165 | 143    64 x 8 of 64, 1024 -> 1024  106 | 83
-//   65536 x 2 of 16,  512 -> 128   215 | 183     256 -> 256   172 | 168    128 -> 128  66 | 71                  4096 x 2, 512 -> 512  42.4 | 43.9
+//   16384 x 2 of 16, 1024 -> 2048  583 | 454    2048 -> 1024  605 | 470    8192 x 2, 1024 -> 1024  158 | 144    64 x 8 of 64, 1024 -> 1024  92 | 72
+//   65536 x 2 of 16,  512 -> 128   263 | 246     256 -> 256   198 | 188    128 -> 128  76 | 79                  4096 x 2, 512 -> 512  49 | 47
 static bool mask_once(int64_t R, int n_in, int n_out) { return n_in >= 1024 || (n_in >= 256 && R * n_out >= 1 << 23); }
 
 template <typename T, int MODE, bool F32>

@@ -17,8 +17,8 @@
 // lanes that hold it, and the first of them takes its expert out.  The entries lie in LDS, a lane each computes their weights.
 // Bound by memory where few are chosen: 2^20 x 32 fp32, top 2: 32 us (151 MB, 4.7 TB/s; a copy reaches 4.96).  By the rounds'
 // instructions where many are: 65536 x 256 bf16, top 8: 25 us (38 MB, 1.5 TB/s); with a bias 55 us in fp32; 30011 rows of 8 groups
-// 27 us.  (With all experts of a wave in 64 bits wherever two entries were close these two took 62 and 35: the few waves that do
-// it end last.)
+// 27 us.  (Calls repeated on the same logits, which the caches hold in part: with other data in between the first takes 37, the last 32.
+// With all experts of a wave in 64 bits wherever two entries were close the last two took 62 and 35: the few waves that do it end last.)
 #include "expert_common.h"
 #include <algorithm>
 
