@@ -119,7 +119,9 @@ class RoutedNetwork(nn.Module):
         self.register_buffer("balance", torch.zeros(self.n_experts) if balance else None)
         self.register_buffer("load", torch.zeros(self.n_experts), persistent=False)
 
-    half_weights = Network.half_weights
+    def half_weights(self) -> torch.Tensor:
+        """fp16 copy of ``params`` as they are now.  (Nothing is kept: the replays of a captured step change weights without a word.)"""
+        return F.f32_to_f16(self.params.detach())
 
     def forward(self, x: torch.Tensor, selector: torch.Tensor = None) -> torch.Tensor:
         """x [B, n_input_dims] (fp16 or fp32) -> [B, n_output_dims] fp16; ``selector`` uint8 [B]: rows with 0 are not evaluated

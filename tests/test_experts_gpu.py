@@ -1289,3 +1289,48 @@ def test_route_groups_with_infinite_biases_and_one_expert_left(sc, cuda):
         w, c = X.route_experts(torch.from_numpy(x).to(cuda), k, scores=sc, bias=torch.from_numpy(bias).to(cuda), n_groups=G, top_groups=tg, group_top=2)
         assert np.array_equal(c.cpu().numpy(), wc), (tg, k)
         _close(w, ww, _route_tol(x, ww, k), "weights")
+
+
+def test_routed_network_follows_its_weights_through_captured_steps(cuda):
+    """Weights that change without a word to the autograd engine -- a captured optimizer's replays, ``.data`` -- and replays of a forward whose
+    weights an eager step changed: what runs next reads them as they are."""
+    from nersemble_amd import tcnn
+    args = (20, 5, {"n_neurons": 64, "n_hidden_layers": 2}, {"n_experts": 6, "top_k": 2})
+    net, fresh = tcnn.RoutedNetwork(*args).to(cuda), tcnn.RoutedNetwork(*args).to(cuda)
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.randn((700, 20), generator=g, device=cuda)
+    go = torch.randn((700, 5), generator=g, device=cuda).half()
+
+    def now():
+        """What a network made for these weights says."""
+        other = tcnn.RoutedNetwork(*args).to(cuda)
+        other.load_state_dict(net.state_dict())
+        with torch.no_grad():
+            return other(x)
+
+    def step():
+        out = net(x)
+        (d,) = torch.autograd.grad(out, [net.params], go)
+        with torch.no_grad():
+            net.params.sub_(d, alpha=0.01)
+        return out.detach()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.no_grad():
+        net(x)                                          # (whatever a forward keeps, it has now)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for turn in range(3):
+        want = now()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(res, want), turn             # the captured forward read the weights of its time
+        with torch.no_grad():
+            assert torch.equal(net(x), now()), turn     # an eager one those that the replay left
+            net.params.data.mul_(1.01)
+            assert torch.equal(net(x), now()), turn
+            net.params.copy_(fresh.params * (1 + turn))
