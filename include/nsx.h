@@ -1062,8 +1062,8 @@ int nsx_expert_linear_fwd(const void* x, int dtype, int64_t x_stride, int64_t x_
 /* Gradients of the above.  dx (or NULL): [R][n_in] where x holds ordered rows (rows NULL), else [x_rows][n_in], a row's choices
  * summed (rows without choices: 0).  dw (or NULL): [E][n_out][n_in], of x's dtype or (dw_f32) in 32 bits, 0 for an expert without
  * rows.  y: the forward's result if it had the ReLU (dy counts where y is not 0), else NULL.  weight is read for dx, x for dw.
- * workspace: nsx_expert_linear_bwd_workspace bytes (0: none), choices = top_k if rows are given, else 0 (the choices of a
- * row are summed in 32 bits); masked = y is given. */
+ * workspace: nsx_expert_linear_bwd_workspace bytes (0: none).  choices = top_k where rows are given, else 0 -- a number, not a truth
+ * value (as it was up to version 129): the choices of a row lie there in 32 bits; masked = y is given. */
 int64_t nsx_expert_linear_bwd_workspace(int64_t R, int E, int n_in, int n_out, int want_dx, int choices, int want_dw,
                                         int masked);
 int nsx_expert_linear_bwd(const void* x, int dtype, int64_t x_stride, int64_t x_rows, const int32_t* rows, const int32_t* positions,
